@@ -316,6 +316,109 @@ lh_status lh_activation(const float* x, size_t count, uint32_t activation, float
 /* First maximal index per row (main_decoder.cpp:102). */
 lh_status lh_argmax(const float* logits, size_t rows, size_t width, uint32_t* out, lh_stream stream);
 
+/* ------------------------------------------------- 8-bit KV cache in blocks
+ * One pool of blocks holds the keys and values of many requests, 8 bits a
+ * value with a scale for each block and KV head.  A step of a serving loop is
+ *   lh_kv_assign      blocks, positions and slots for the step's tokens,
+ *   lh_rope_kv8       RoPE, and the tokens' keys and values into their slots,
+ *   lh_attention_kv8  attention of the tokens over their requests' blocks
+ * (the last two once for each layer, over that layer's lh_kv8).  Lengths and
+ * tables stay on the device: no call reads them on the host, so a step can be
+ * captured and replayed.  No counterpart in the reference, which serves one
+ * sequence from an f32 cache; lh_set_kernel_numerics has no bearing on them. */
+#define LH_KV_MAX_REQUESTS 4000
+
+/* A step's batch.  All pointers are device pointers.  A request's new tokens
+ * are consecutive rows of the step's arrays, the requests in order; rows behind
+ * the last request's are padding and stay as they were. */
+typedef struct lh_kv_batch {
+    uint32_t requests;      /* 1..LH_KV_MAX_REQUESTS */
+    uint32_t tokens;        /* rows of the step's arrays */
+    uint32_t max_rows;      /* no request has more new tokens than this; a request that has is turned away */
+    uint32_t block;         /* tokens a block holds: 16, 32, 64 or 128 */
+    uint32_t blocks;        /* blocks of the pool */
+    uint32_t width;         /* table entries of a request */
+    /* read by lh_kv_assign: */
+    const int32_t* cached;      /* [requests] tokens a request has in the cache */
+    const int32_t* fresh;       /* [requests] its new tokens; negative: it has ended, its blocks go back */
+    int32_t* free_blocks;       /* [blocks] stack of free blocks: entries [0, *free_count); returned blocks are written behind */
+    const int32_t* free_count;  /* [1] */
+    /* written by lh_kv_assign: */
+    int32_t* free_left;         /* [1] the free blocks after the step; may be free_count itself */
+    int32_t* table;             /* [requests][width] blocks of a request in the order of its tokens (new ones are added) */
+    int32_t* lengths;           /* [requests] tokens in the cache after the step; may be cached itself */
+    int32_t* starts;            /* [requests + 1] first row of each request */
+    int32_t* rows;              /* [requests] new tokens that were taken in: fresh, or 0 */
+    int32_t* positions;         /* [tokens] position in the request, -1 for rows of none and of requests turned away */
+    int32_t* slots;             /* [tokens] block * lh_kv_batch.block + place in the block, or -1 */
+} lh_kv_batch;
+
+#define LH_KV8_INT8 0 /* two's complement, -127..127, scale = largest magnitude / 127 */
+#define LH_KV8_E4M3 1 /* 8-bit floating point (4 exponent, 3 mantissa bits, no infinities), scale a power of two */
+
+/* One layer's cache: a value is its code times the scale of its block and KV head. */
+typedef struct lh_kv8 {
+    void* keys;             /* [blocks][kv_heads][block][dim] codes, 16-byte aligned */
+    void* values;           /* [blocks][kv_heads][dim][block] codes (a dim's tokens are consecutive), 16-byte aligned */
+    float* key_scales;      /* [blocks][kv_heads] */
+    float* value_scales;    /* [blocks][kv_heads] */
+    uint32_t kv_heads;
+    uint32_t dim;           /* a multiple of 16, at most 256 */
+    uint32_t format;        /* LH_KV8_* */
+} lh_kv8;
+
+/* Block tables and slot maps of a step, from the requests' lengths alone.
+ * Ended requests' blocks are put on the free stack, in the requests' order.
+ * Then each request takes the blocks that its new tokens need from the top of
+ * the stack, in order; from the first that the stack has too few for, all that
+ * need one are turned away (rows 0, length and table as they were).  So is a
+ * request with more than max_rows new tokens, with more tokens than its table
+ * has room for, or whose rows pass `tokens`.  Needs all of the batch's pointers. */
+lh_status lh_kv_assign(const lh_kv_batch* batch, lh_stream stream);
+
+/* lh_rope_kv for a batch over an 8-bit cache: qkv [tokens, (heads + 2 kv_heads)
+ * * dim], token t rotated for position positions[t] with the first
+ * `table_positions` rows of cosines and sines [table_positions][rotary_dim / 2]:
+ * q -> q_heads [heads, tokens, dim], k and v -> slot slots[t] of the cache.  A
+ * token whose slot or position is outside the pool or the tables is skipped, its
+ * row of q_heads left as it was.  Reads the batch's positions and slots.
+ *
+ * A block's new tokens stand in rows that rise with their slots, one row for one
+ * slot; the tokens it holds already are the slots before the first.  (Where a skipped
+ * row parts them, those before the gap are written first, then those behind it.)  In
+ * each block and KV head, for keys and for values:
+ *   INT8  scale = max(largest magnitude / 127, 1e-12, the scale of tokens it
+ *         holds), code = value / scale to the nearest, ties to even; where the
+ *         scale has grown, codes it holds become code * old scale / scale, rounded alike;
+ *   E4M3  the same with scale = the smallest power of two (from 2^-40) that is
+ *         at least largest magnitude / 448, and the nearest 8-bit floating point values.
+ * A new value that is not finite makes its block's scale NaN (and the new codes
+ * 0): every query that sees a token of the block gets NaN, until the block is
+ * written from its first slot again.  qkv, q_heads, cosines and sines are 16-byte aligned. */
+lh_status lh_rope_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float* qkv, uint32_t heads,
+                      uint32_t rotary_dim, const float* cosines, const float* sines, size_t table_positions,
+                      float* q_heads, lh_stream stream);
+
+/* Causal GQA attention of a batch over an 8-bit cache: row i of a request with
+ * `rows` new tokens and length n stands at position n - rows + i and sees the keys
+ * up to its own, the last `window` of them where window is not 0.  q_heads [heads,
+ * tokens, dim], out [tokens, heads * dim], both 16-byte aligned.  The products are
+ * those of lh_attention, in f32 accuracy.  Reads the batch's table, lengths, starts
+ * and rows (of any source: a request whose rows or length do not fit the batch is
+ * passed over, its rows of out left as they were, as are padding rows).  A query
+ * that is not finite, a block with a scale of NaN and a table entry that is no block
+ * give NaN in the rows that see them, and only there.
+ *
+ * Long contexts are split over the GPU; the parts' results pass through a workspace
+ * of lh_attention_kv8_workspace bytes, 16-byte aligned: the caller's, or with NULL (and 0)
+ * the scratch of the stream, under the rules of lh_attention's (run the call once before
+ * capturing it; launch the graph in order with that stream's calls).  Graphs that may run
+ * at the same time need workspaces of their own. */
+lh_status lh_attention_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,
+                           uint32_t window, float* out, void* workspace, size_t workspace_bytes, lh_stream stream);
+/* Bytes that any call of the batch's sizes needs, whatever the lengths. */
+lh_status lh_attention_kv8_workspace(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

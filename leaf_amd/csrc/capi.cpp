@@ -224,6 +224,59 @@ leafhip::WeightView view_of(const lh_weight* w) {
     return v;
 }
 
+leafhip::KvBatchView view_of(const lh_kv_batch* b) {
+    require_arg(b != nullptr, "KV batch is null");
+    require_arg(b->requests >= 1 && b->requests <= LH_KV_MAX_REQUESTS, "KV batch requests must be 1..4000");
+    require_arg(b->block == 16 || b->block == 32 || b->block == 64 || b->block == 128,
+                "KV block must hold 16, 32, 64 or 128 tokens");
+    require_arg(b->blocks >= 1 && uint64_t(b->blocks) * b->block <= 0x7fffffff, "KV pool has no blocks or too many");
+    require_arg(b->width >= 1 && uint64_t(b->requests) * b->width <= 0x7fffffff, "KV table is empty or too large");
+    require_arg(b->tokens >= 1 && b->tokens <= 0x7fffffff && b->max_rows >= 1, "KV batch has no rows or too many");
+    leafhip::KvBatchView v;
+    v.requests = int(b->requests);
+    v.tokens = int(b->tokens);
+    v.max_rows = int(std::min(b->max_rows, b->tokens));
+    v.block = int(b->block);
+    v.block_shift = __builtin_ctz(b->block);
+    v.blocks = int(b->blocks);
+    v.width = int(b->width);
+    v.cached = b->cached; v.fresh = b->fresh; v.free_blocks = b->free_blocks; v.free_count = b->free_count;
+    v.free_left = b->free_left; v.table = b->table; v.lengths = b->lengths; v.starts = b->starts; v.rows = b->rows;
+    v.positions = b->positions; v.slots = b->slots;
+    return v;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+leafhip::Kv8View view_of(const lh_kv8* c, bool pointers = true) {
+    require_arg(c != nullptr, "KV cache is null");
+    require_arg(!pointers || (c->keys && c->values && c->key_scales && c->value_scales), "KV cache is empty");
+    require_arg(aligned16(c->keys) && aligned16(c->values), "KV cache codes must be 16-byte aligned");
+    require_arg(c->kv_heads >= 1 && c->kv_heads <= 65535, "KV heads must be 1..65535");
+    require_arg(c->dim >= 16 && c->dim <= 256 && c->dim % 16 == 0, "head dim of an 8-bit cache must be a multiple of 16 up to 256");
+    require_arg(c->format == LH_KV8_INT8 || c->format == LH_KV8_E4M3, "unknown 8-bit KV format");
+    leafhip::Kv8View v;
+    v.keys = static_cast<uint8_t*>(c->keys);
+    v.values = static_cast<uint8_t*>(c->values);
+    v.key_scales = c->key_scales;
+    v.value_scales = c->value_scales;
+    v.kv_heads = int(c->kv_heads);
+    v.dim = int(c->dim);
+    v.e4m3 = c->format == LH_KV8_E4M3;
+    return v;
+}
+
+leafhip::AttentionKv8Call attention_kv8_call(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads,
+                                             bool pointers) {
+    leafhip::AttentionKv8Call a;
+    a.batch = view_of(batch);
+    a.cache = view_of(cache, pointers);
+    require_arg(heads >= 1 && heads <= 65535 && heads % cache->kv_heads == 0, "heads must be a multiple of the KV heads, at most 65535");
+    require_arg(uint64_t(batch->tokens) * heads <= 0x7fffffff, "too many rows of attention");
+    a.heads = int(heads);
+    return a;
+}
+
 lh_status linear_impl(const lh_weight* weight, const float* x, const int8_t* q, const float* qs, size_t tokens,
                       uint32_t activation_bits, float* y, int32_t* acc, lh_stream stream, int force_path,
                       unsigned required_bits, bool no_alloc = false) {
@@ -815,6 +868,71 @@ lh_status lh_argmax(const float* logits, size_t rows, size_t width, uint32_t* ou
         require_arg(logits && out && rows && width && rows <= 0x7fffffff && width <= 0x7fffffff, "invalid argmax call");
         leafhip::launch_argmax(logits, int(rows), int(width), out, as_stream(stream));
         leafhip::hip_check(hipGetLastError(), "argmax launch");
+    });
+}
+
+
+lh_status lh_kv_assign(const lh_kv_batch* batch, lh_stream stream) {
+    return guarded([&] {
+        const leafhip::KvBatchView b = view_of(batch);
+        require_arg(b.cached && b.fresh && b.free_blocks && b.free_count && b.free_left && b.table && b.lengths &&
+                        b.starts && b.rows && b.positions && b.slots,
+                    "KV assignment needs all arrays of the batch");
+        leafhip::launch_kv_assign(b, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "KV assignment launch");
+    });
+}
+lh_status lh_rope_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float* qkv, uint32_t heads,
+                      uint32_t rotary_dim, const float* cosines, const float* sines, size_t table_positions,
+                      float* q_heads, lh_stream stream) {
+    return guarded([&] {
+        leafhip::RopeKv8Call r;
+        r.batch = view_of(batch);
+        r.cache = view_of(cache);
+        require_arg(r.batch.positions && r.batch.slots && qkv && q_heads, "invalid rope call");
+        require_arg(heads >= 1 && heads <= 65535 && heads % cache->kv_heads == 0,
+                    "heads must be a multiple of the KV heads, at most 65535");
+        require_arg(rotary_dim <= cache->dim && rotary_dim % 2 == 0 && (!rotary_dim || (cosines && sines)), "invalid rotary dim");
+        require_arg(table_positions >= 1 && table_positions <= 0x7fffffff, "RoPE tables are empty or too long");
+        require_arg((uint64_t(heads) + 2 * uint64_t(cache->kv_heads)) * cache->dim <= 0x7fffffff &&
+                        uint64_t(batch->tokens) * heads <= 0x7fffffff, "too many heads");
+        require_arg(aligned16(qkv) && aligned16(q_heads) && aligned16(cosines) && aligned16(sines),
+                    "rope arrays must be 16-byte aligned");
+        r.qkv = qkv; r.cosines = cosines; r.sines = sines; r.heads = int(heads); r.rotary = int(rotary_dim);
+        r.positions = int(table_positions); r.q_heads = q_heads;
+        leafhip::launch_rope_kv8(r, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "rope launch");
+    });
+}
+lh_status lh_attention_kv8_workspace(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads, size_t* bytes) {
+    return guarded([&] {
+        require_arg(bytes != nullptr, "output pointer is null");
+        *bytes = leafhip::attention_kv8_workspace_bytes(attention_kv8_call(batch, cache, heads, false));
+    });
+}
+lh_status lh_attention_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,
+                           uint32_t window, float* out, void* workspace, size_t workspace_bytes, lh_stream stream) {
+    return guarded([&] {
+        leafhip::AttentionKv8Call a = attention_kv8_call(batch, cache, heads, true);
+        require_arg(a.batch.table && a.batch.lengths && a.batch.starts && a.batch.rows && q_heads && out,
+                    "invalid attention call");
+        require_arg(aligned16(q_heads) && aligned16(out) && aligned16(workspace),
+                    "attention arrays and workspace must be 16-byte aligned");
+        a.q_heads = q_heads;
+        a.out = out;
+        a.window = int(std::min<uint32_t>(window, 0x7fffffff));
+        a.scale = 1.0f / std::sqrt(static_cast<float>(cache->dim));
+        const size_t bytes = leafhip::attention_kv8_workspace_bytes(a);
+        std::optional<ScratchUse> scratch;
+        if (workspace) {
+            require_arg(workspace_bytes >= bytes, "attention workspace is too small (lh_attention_kv8_workspace)");
+            a.partial = static_cast<float*>(workspace);
+        } else if (bytes) {
+            scratch.emplace(as_stream(stream));
+            a.partial = static_cast<float*>(scratch->work(bytes));
+        }
+        leafhip::launch_attention_kv8(a, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "attention launch");
     });
 }
 

@@ -251,4 +251,37 @@ bool launch_sequential_sum(const float* x, int n, int count, float* sums, long l
 bool launch_linear_fp_reference_order(const WeightView& w, const float* x, int tokens, float* y, int epilogue,
                                       hipStream_t stream);
 
+// ---- 8-bit KV cache in blocks (include/leafhip.h: lh_kv_batch, lh_kv8)
+struct KvBatchView {
+    int requests = 0, tokens = 0, max_rows = 0, block = 0, block_shift = 0, blocks = 0, width = 0;
+    const int *cached = nullptr, *fresh = nullptr, *free_count = nullptr;
+    int *free_blocks = nullptr, *free_left = nullptr, *table = nullptr, *lengths = nullptr, *starts = nullptr;
+    int *rows = nullptr, *positions = nullptr, *slots = nullptr;
+};
+struct Kv8View {
+    uint8_t *keys = nullptr, *values = nullptr;   // [blocks][kv_heads][block][dim], [blocks][kv_heads][dim][block]
+    float *key_scales = nullptr, *value_scales = nullptr;
+    int kv_heads = 0, dim = 0, e4m3 = 0;
+};
+void launch_kv_assign(const KvBatchView& batch, hipStream_t stream);
+struct RopeKv8Call {
+    KvBatchView batch;
+    Kv8View cache;
+    const float *qkv = nullptr, *cosines = nullptr, *sines = nullptr;
+    int heads = 0, rotary = 0, positions = 0;
+    float* q_heads = nullptr;
+};
+void launch_rope_kv8(const RopeKv8Call& call, hipStream_t stream);
+struct AttentionKv8Call {
+    KvBatchView batch;
+    Kv8View cache;
+    const float* q_heads = nullptr;
+    float* out = nullptr;
+    int heads = 0, window = 0;
+    float scale = 1.0f;             // of q.k: 1 / sqrt(dim)
+    float* partial = nullptr;       // attention_kv8_workspace_bytes(call) bytes
+};
+size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call);
+void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream);
+
 }  // namespace leafhip

@@ -58,6 +58,21 @@ class Weight(C.Structure):
                 ("rows", C.c_uint32), ("cols", C.c_uint32), ("bits", C.c_uint32), ("group", C.c_uint32)]
 
 
+class KvBatch(C.Structure):
+    """lh_kv_batch: sizes and the device arrays of one step's requests (addresses, or None)."""
+    _fields_ = [(name, C.c_uint32) for name in ("requests", "tokens", "max_rows", "block", "blocks", "width")] + [
+        (name, C.c_void_p) for name in ("cached", "fresh", "free_blocks", "free_count", "free_left", "table", "lengths",
+                                        "starts", "rows", "positions", "slots")]
+
+
+class Kv8(C.Structure):
+    """lh_kv8: one layer's 8-bit keys and values in blocks (addresses on the device)."""
+    _fields_ = [(name, C.c_void_p) for name in ("keys", "values", "key_scales", "value_scales")] + [
+        (name, C.c_uint32) for name in ("kv_heads", "dim", "format")]
+
+
+KV8_FORMATS = {"int8": 0, "e4m3": 1}
+
 _lib = None
 _exiting = False
 
@@ -127,6 +142,10 @@ def library(path: Path | None = None) -> C.CDLL:
         "lh_layernorm": ([vp, sz, sz, vp, vp, C.c_float, vp, vp], i32),
         "lh_rope_kv": ([vp, sz, u32, u32, u32, u32, sz, vp, vp, vp, vp, vp, sz, vp], i32),
         "lh_attention": ([vp, vp, vp, sz, u32, u32, u32, sz, sz, u32, vp, vp], i32),
+        "lh_kv_assign": ([C.POINTER(KvBatch), vp], i32),
+        "lh_rope_kv8": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, sz, vp, vp], i32),
+        "lh_attention_kv8": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, sz, vp], i32),
+        "lh_attention_kv8_workspace": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, C.POINTER(sz)], i32),
         "lh_silu_gate": ([vp, sz, sz, vp, vp], i32),
         "lh_activation": ([vp, sz, u32, vp, vp], i32),
         "lh_argmax": ([vp, sz, sz, vp, vp], i32),
@@ -380,6 +399,71 @@ def sequential_sum(x: DeviceArray, n: int, count: int, sums: DeviceArray, cycles
 
 def quantize_rows(x: DeviceArray, rows: int, cols: int, q: DeviceArray, scales: DeviceArray, stream=None) -> None:
     check(library().lh_quantize_rows_i8(x.ptr, rows, cols, q.ptr, scales.ptr, stream))
+
+
+class BlockPool:
+    """The requests of a serving loop: their lengths, block tables and the free blocks (lh_kv_assign's arrays).
+
+    ``step`` takes each request's new tokens (negative: it has ended) to the device and assigns their blocks;
+    ``batch`` is what ``rope_kv8`` and ``attention_kv8`` take then.  Lengths and free blocks are kept on the device.
+    """
+
+    def __init__(self, requests: int, tokens: int, block: int, blocks: int, width: int, max_rows: int = 0):
+        def ints(*shape):
+            return DeviceArray(shape, np.int32).zero()
+        self.fresh, self.lengths, self.rows = ints(requests), ints(requests), ints(requests)
+        self.starts, self.positions, self.slots = ints(requests + 1), ints(tokens), ints(tokens)
+        self.table = DeviceArray.of(np.full((requests, width), -1, np.int32))
+        self.free_blocks = DeviceArray.of(np.arange(blocks, dtype=np.int32)[::-1])
+        self.free_count = DeviceArray.of(np.array([blocks], np.int32))
+        self.batch = KvBatch(requests, tokens, max_rows or tokens, block, blocks, width, self.lengths.ptr, self.fresh.ptr,
+                             self.free_blocks.ptr, self.free_count.ptr, self.free_count.ptr, self.table.ptr,
+                             self.lengths.ptr, self.starts.ptr, self.rows.ptr, self.positions.ptr, self.slots.ptr)
+
+    def step(self, fresh, stream=None) -> None:
+        fresh = np.ascontiguousarray(fresh, np.int32)
+        if fresh.shape != self.fresh.shape:
+            raise ValueError(f"new tokens of {self.fresh.shape[0]} requests are needed, got {fresh.shape}")
+        check(library().lh_copy_to_device(self.fresh.ptr, _ptr(fresh), fresh.nbytes))
+        kv_assign(self.batch, stream)
+
+
+class BlockCache:
+    """One layer's 8-bit keys and values in the blocks of a pool (lh_kv8)."""
+
+    def __init__(self, pool: BlockPool, kv_heads: int, dim: int, format: str = "int8"):
+        blocks, block = pool.batch.blocks, pool.batch.block
+        self.keys = DeviceArray((blocks, kv_heads, block, dim), np.uint8)
+        self.values = DeviceArray((blocks, kv_heads, dim, block), np.uint8)
+        self.key_scales, self.value_scales = (DeviceArray((blocks, kv_heads), np.float32) for _ in range(2))
+        self.desc = Kv8(self.keys.ptr, self.values.ptr, self.key_scales.ptr, self.value_scales.ptr, kv_heads, dim,
+                        KV8_FORMATS[format])
+
+
+def kv_assign(batch: KvBatch, stream=None) -> None:
+    check(library().lh_kv_assign(C.byref(batch), stream))
+
+
+def rope_kv8(batch: KvBatch, cache: Kv8, qkv: DeviceArray, heads: int, rotary_dim: int, cosines: DeviceArray | None,
+             sines: DeviceArray | None, q_heads: DeviceArray, stream=None, table_positions: int = 0) -> None:
+    """RoPE and the step's keys and values into their slots; table_positions: rows of the tables (default: theirs)."""
+    check(library().lh_rope_kv8(C.byref(batch), C.byref(cache), qkv.ptr, heads, rotary_dim,
+                                cosines.ptr if cosines is not None else None, sines.ptr if sines is not None else None,
+                                table_positions or (cosines.shape[0] if cosines is not None else 0x7fffffff),
+                                q_heads.ptr, stream))
+
+
+def attention_kv8(batch: KvBatch, cache: Kv8, q_heads: DeviceArray, heads: int, out: DeviceArray, window: int = 0,
+                  workspace: DeviceArray | None = None, stream=None) -> None:
+    check(library().lh_attention_kv8(C.byref(batch), C.byref(cache), q_heads.ptr, heads, window, out.ptr,
+                                     workspace.ptr if workspace is not None else None,
+                                     workspace.nbytes if workspace is not None else 0, stream))
+
+
+def attention_kv8_workspace(batch: KvBatch, cache: Kv8, heads: int) -> int:
+    n = C.c_size_t()
+    check(library().lh_attention_kv8_workspace(C.byref(batch), C.byref(cache), heads, C.byref(n)))
+    return n.value
 
 
 class Stream:
