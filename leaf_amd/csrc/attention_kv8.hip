@@ -38,6 +38,7 @@ constexpr int kStep = 64;                           // keys
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kFewRows = 16;                        // rows of a KV head in one tile
+constexpr int kHeader = 4;                          // integers before a plan's requests
 constexpr float kNoBase = -1e30f;
 constexpr float kSlack = 6.0f, kLift = 8.0f;
 
@@ -219,44 +220,59 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
 }
 
 // How a batch's work is shared out.  A request's rows of a KV head make tiles of
-// `tile_rows`; a tile's keys are cut into equal parts of at most `per` steps,
-// per chosen so that all parts of the batch are about `target` workgroups.
+// `tile_rows`; a tile's steps are cut into equal parts of at most `per`, per
+// chosen so that all parts of the batch are about `target` workgroups.  A request
+// has workgroups for as many parts of each tile as its longest tile has.
 struct Share {
     int tile_rows, target, least;                   // least: steps a part has at least
     int few;                                        // requests of at most kFewRows rows (1) or of more (0)
+    int items;                                      // of a KV head, that there are workgroups and partial results for
+    size_t at;                                      // where its partial results begin: in floats
 };
 __device__ __forceinline__ int tiles_of(const Kv8Request& q, int group, const Share& share) {
     const int rows = q.rows * group;
     if (rows == 0 || (rows <= kFewRows) != (share.few != 0)) return 0;
     return (rows + share.tile_rows - 1) / share.tile_rows;
 }
-// Steps of the longest tile of a request.
-__device__ __forceinline__ int steps_of(const Kv8Request& q, int window) {
-    const int first = window ? max(0, q.length - q.rows + 1 - window) : 0;
-    return (q.length + kStep - 1) / kStep - first / kStep;
+// The steps that a tile's rows see.
+struct Steps {
+    int begin, end;
+};
+__device__ __forceinline__ Steps steps_of(const Kv8Request& q, int group, int window, int tile_rows, int tile) {
+    const int r0 = tile * tile_rows, last = min(r0 + tile_rows, q.rows * group) - 1, before = q.length - q.rows;
+    return Steps{window ? max(0, before + r0 / group + 1 - window) / kStep : 0, (before + last / group) / kStep + 1};
 }
+// No tile of a request has more.
+__device__ __forceinline__ int most_steps(const Kv8Request& q, int group, int window, int tile_rows) {
+    const int all = (q.length - 1) / kStep + 1;
+    return window ? (int)min((long long)all, ((long long)window + tile_rows / group) / kStep + 3) : all;
+}
+__device__ __forceinline__ int parts_of(int steps, int per) { return (steps + per - 1) / per; }
 
 struct Item {
-    int request, tile, part, parts, first;          // first: number of the request's first item of its KV head
+    int request, tile, part, index;                 // index: of the tile's first part among the KV head's items
     Kv8Request q;
 };
 
 // Which part of which tile of which request is item `index` (of one KV head);
 // request -1: none.  Every workgroup sums the whole batch, 256 requests at a time.
-__device__ __forceinline__ Item find_item(const KvBatchView& b, int kv_heads, int group, int window, const Share& share, int index,
-                                          int& per) {
+// The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first item.
+__device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
+    const KvBatchView& b = p.batch;
+    const int window = p.window;
     __shared__ int sums[kWaves];
     __shared__ Item found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    auto steps = [&](const Kv8Request& q) { return tiles_of(q, group, share) * steps_of(q, window); };
+    auto steps = [&](const Kv8Request& q) {
+        return (float)tiles_of(q, group, share) * (float)most_steps(q, group, window, share.tile_rows);
+    };
     Kv8Request mine{0, 0, 0};
-    long long total = 0;
+    float all = 0.0f;
     for (int r = threadIdx.x; r < b.requests; r += kThreads) {
         mine = kv8_request(b, r);
-        total += steps(mine);
+        all += steps(mine);
     }
-    // (in f32: a share of work, not a sum that anything else depends on)
-    float all = wave_sum_f32((float)total);
+    all = wave_sum_f32(all);
     __shared__ float totals[kWaves];
     if (lane == 0) totals[wave] = all;
     if (threadIdx.x == 0) found.request = -1;
@@ -264,12 +280,12 @@ __device__ __forceinline__ Item find_item(const KvBatchView& b, int kv_heads, in
     all = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all += totals[w];
-    per = max(share.least, (int)fminf(all * (float)kv_heads / (float)share.target + 1.0f, 1e9f));
+    per = max(share.least, (int)fminf(all * (float)p.cache.kv_heads / (float)share.target * 1.0001f + 1.0f, 1e9f));
     int before = 0;
     for (int base = 0; base < b.requests; base += kThreads) {
         const int r = base + threadIdx.x;
         if (b.requests > kThreads) mine = r < b.requests ? kv8_request(b, r) : Kv8Request{0, 0, 0};
-        const int tiles = tiles_of(mine, group, share), parts = (steps_of(mine, window) + per - 1) / per;
+        const int tiles = tiles_of(mine, group, share), parts = parts_of(most_steps(mine, group, window, share.tile_rows), per);
         const int items = tiles ? tiles * parts : 0;
         int s = items;
 #pragma unroll
@@ -288,11 +304,14 @@ __device__ __forceinline__ Item find_item(const KvBatchView& b, int kv_heads, in
         if (index >= start && index < start + items) {
             const int i = index - start;
             // the longest tiles (the last) first
-            found = Item{r, tiles - 1 - i / parts, i % parts, parts, start, mine};
+            found = Item{r, tiles - 1 - i / parts, i % parts, start + i / parts * parts, mine};
         }
+        // the first workgroup leaves the plan for the merge
+        if (blockIdx.x == 0 && r < b.requests) ((int*)p.partial)[share.at + kHeader + r] = start;
+        if (blockIdx.x == 0 && r == 0) ((int*)p.partial)[share.at] = per;
         before += all_items;
         __syncthreads();
-        if (index < before) break;
+        if (index < before && blockIdx.x) break;
     }
     return found;
 }
@@ -303,9 +322,12 @@ __device__ __forceinline__ Keys keys_of(const AttentionKv8Call& p, int request, 
                 b.block_shift, b.blocks, p.cache.kv_heads, kvh, p.cache.dim, end};
 }
 
-// Partial results: a tile of rows by dim floats and each row's (base, sum), one after the other by item.
-__device__ __forceinline__ float* partial_rows(const AttentionKv8Call& p, size_t item, int tile_rows) {
-    return p.partial + 64 + p.batch.requests + item * tile_rows * (p.cache.dim + 2);
+// Partial results: of each item its rows by dim floats; behind all of them each row's base and sum.
+__device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, const Share& share, size_t item) {
+    return p.partial + share.at + (kHeader + p.batch.requests + 3) / 4 * 4 + item * share.tile_rows * p.cache.dim;
+}
+__device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Share& share, size_t item) {
+    return (v2f*)partial_values(p, share, (size_t)share.items * p.cache.kv_heads) + item * share.tile_rows;
 }
 
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
@@ -316,17 +338,18 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item(p.batch, kv_heads, group, p.window, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, row = min(li, rows - 1);
     const int token = q.start + row / group, head = kvh * group + row % group;
     const int position = q.length - q.rows + row / group;
     const int low = q.length - q.rows;                             // of the first row
-    const int first = p.window ? max(0, low + 1 - p.window) / kStep : 0;
-    const int steps = (q.length + kStep - 1) / kStep - first;
-    const int begin = first + (int)((long long)item.part * steps / item.parts);
-    const int end = first + (int)((long long)(item.part + 1) * steps / item.parts);
+    const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
+    const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
+    if (item.part >= parts) return;
+    const int begin = seen.begin + (int)((long long)item.part * steps / parts);
+    const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys = keys_of(p, item.request, kvh, q.length);
 
     v4u kr[4][CC], vr[TILES];
@@ -429,17 +452,14 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
         alpha[w] = __builtin_amdgcn_exp2f(bases[w][li] - base);
         sum = fmaf(sums[w][li], alpha[w], sum);
     }
-    if (p.partial && threadIdx.x == 0) {
-        // for the merge: parts' steps, and the first item of the request
-        if (blockIdx.x == 0) *(int*)p.partial = per;
-        if (item.parts > 1 && item.part == 0 && kvh == 0) ((int*)p.partial)[64 + item.request] = item.first;
-    }
     if (li >= rows) return;
-    const bool whole = item.parts == 1;
-    float* part = whole ? nullptr : partial_rows(p, (size_t)(item.first + item.part) * kv_heads + kvh, share.tile_rows) + (size_t)li * (dim + 2);
-    if (part && wave == 0 && lq == 0) {
-        part[dim] = base;
-        part[dim + 1] = sum;
+    const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+    float* to = p.out + ((size_t)token * p.heads + head) * dim;
+    float scale = 1.0f / sum;
+    if (parts > 1) {
+        to = partial_values(p, share, slot) + (size_t)li * dim;
+        scale = 1.0f;
+        if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = v2f{base, sum};
     }
     for (int t = wave; t < tiles; t += kWaves) {
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -449,148 +469,328 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha[w], x[r]);
         }
-        const int d = 16 * t + 4 * lq;
-        if (whole) {
-            *(v4f*)(p.out + ((size_t)token * p.heads + head) * dim + d) = v4f{x[0] / sum, x[1] / sum, x[2] / sum, x[3] / sum};
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) part[d + r] = x[r];
-        }
+        *(v4f*)(to + 16 * t + 4 * lq) = x * scale;
     }
 }
 
-// ---- rows whose keys were parted: one wave a row
-__global__ __launch_bounds__(kThreads) void attention_kv8_merge_kernel(AttentionKv8Call p, Share share) {
-    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
-    const int request = blockIdx.x, kvh = blockIdx.y;
-    const Kv8Request q = kv8_request(p.batch, request);
-    const int tiles = tiles_of(q, group, share);
-    if (!tiles) return;
-    const int per = *(const int*)p.partial, steps = steps_of(q, p.window), parts = (steps + per - 1) / per;
-    if (parts == 1) return;
-    const int first = ((const int*)p.partial)[64 + request];
-    for (int row = threadIdx.x >> 6; row < q.rows * group; row += kWaves) {
-        const int tile = row / share.tile_rows;
-        const float* part = partial_rows(p, (size_t)(first + (tiles - 1 - tile) * parts) * p.cache.kv_heads + kvh, share.tile_rows) +
-                            (size_t)(row % share.tile_rows) * (dim + 2);
-        const size_t stride = (size_t)p.cache.kv_heads * share.tile_rows * (dim + 2);
-        float base = kNoBase, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < parts; ++i) base = fmaxf(base, part[i * stride + dim]);
-        for (int i = 0; i < parts; ++i) {
-            const float alpha = __builtin_amdgcn_exp2f(part[i * stride + dim] - base);
-            sum = fmaf(part[i * stride + dim + 1], alpha, sum);
+// ---- more rows of a KV head: tiles of 64 or 128, K and V widened once for all of them through LDS
+// Rows per wave: two tiles of 16 up to heads of 128, one beyond (registers).
+constexpr int row_tiles(int cc) { return cc <= 2 ? 2 : 1; }
+
+template <int CC, bool FULL, bool E4M3>
+__global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC, QT = row_tiles(CC), ROWS = 16 * QT * kWaves;
+    constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
+    constexpr int kKeyBytes = 4 * CC * 2 * kOperand, kBuffer = 2 * kKeyBytes;
+    extern __shared__ __align__(16) uint8_t lds[];                 // two of [tile of keys][cc][half][lane], [tile of dims][half][lane]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+    const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
+    const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
+    int per;
+    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
+    if (item.request < 0) return;
+    const Kv8Request& q = item.q;
+    const int rows = q.rows * group, r0 = item.tile * ROWS, w0 = r0 + 16 * QT * wave;
+    const int before = q.length - q.rows;                          // position of the first row
+    const Steps seen = steps_of(q, group, p.window, ROWS, item.tile);
+    const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
+    if (item.part >= parts) return;
+    const int begin = seen.begin + (int)((long long)item.part * steps / parts);
+    const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
+    const Keys keys = keys_of(p, item.request, kvh, q.length);
+    int position[QT], token[QT], head[QT];
+    v8h qh[QT][CC][2], ql[QT][CC][2];
+    float c[QT];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (lane + 64 * k < dim) x[k] = fmaf(part[i * stride + lane + 64 * k], alpha, x[k]);
+    for (int i = 0; i < QT; ++i) {
+        const int row = min(w0 + 16 * i + li, rows - 1);
+        token[i] = q.start + row / group;
+        head[i] = kvh * group + row % group;
+        position[i] = before + row / group;
+        load_query<CC, FULL>(p.q_heads + ((size_t)head[i] * p.batch.tokens + token[i]) * dim, dim, lq, p.scale, qh[i], ql[i], c[i]);
+    }
+    // of the wave's rows: the first sees every key up to `low`, the last none after `high`
+    const int low = before + min(w0, rows - 1) / group;
+    const int high = w0 < rows ? before + min(w0 + 16 * QT - 1, rows - 1) / group : -1;
+
+    // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
+    v4u kr[CC], vr[CC];
+    KeyScales scales, next_scales;
+    auto load = [&](int step, int ik, int iv) {
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            kr[cc] = keys.load_key<FULL>(ik, step, wave, li, 64 * cc + 16 * lq);
+            const int t = wave + 4 * cc;
+            vr[cc] = FULL || t < tiles ? keys.load_value(iv, step, lq, 16 * t + li) : v4u{0, 0, 0, 0};
         }
-        float* out = p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim;
+        next_scales = keys.scales(iv);
+    };
+    auto store = [&](int step) {
+        uint8_t* buffer = lds + (step & 1) * kBuffer;
+        const int at = step * kStep + 16 * lq;
+        const int written = next_scales.value == next_scales.value ? q.length - at : 0;
+        // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
+        const bool clear = E4M3 && (step * kStep + kStep > q.length || __any(written == 0));
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (lane + 64 * k < dim) out[lane + 64 * k] = x[k] / sum;
+        for (int cc = 0; cc < CC; ++cc) {
+            v8h a, b;
+            widen<E4M3>(kr[cc], a, b);
+            v8h* to = (v8h*)(buffer + ((wave * CC + cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+            if (clear) vr[cc] = first_codes(vr[cc], written);
+            widen<E4M3>(vr[cc], a, b);
+            to = (v8h*)(buffer + kKeyBytes + ((wave + 4 * cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+        }
+    };
+    auto block_k = [&](int step) { return keys.block_of(step * kStep + 16 * (li >> 2)); };
+    auto block_v = [&](int step) { return keys.block_of(step * kStep + 16 * lq); };
+
+    v4f o[QT][TILES];
+    Softmax m[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) o[i][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (begin < end) {
+        load(begin, block_k(begin), block_v(begin));
+        store(begin);
+        scales = next_scales;
+        load(begin + 1, block_k(begin + 1), block_v(begin + 1));
+    }
+    int ik = block_k(begin + 2), iv = block_v(begin + 2);
+    __syncthreads();
+    for (int step = begin; step < end; ++step) {
+        const uint8_t* buffer = lds + (step & 1) * kBuffer;
+        const KeyScales now = scales;
+        if (step + 1 < end) {
+            store(step + 1);
+            scales = next_scales;
+            load(step + 2, ik, iv);                                // (past the end: the last block's, not used)
+            ik = block_k(step + 3);
+            iv = block_v(step + 3);
+        }
+        const bool idle = step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window);
+        if (!idle) {
+            v4f acc[QT][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const v8h k = *((const v8h*)(buffer + ((j * CC + cc) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[i][cc][h], acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i][cc][h], acc[i][j], 0, 0, 0);
+                        }
+                    }
+            }
+            v8h hi[QT][2], lo[QT][2];
+            const int at = step * kStep + 16 * lq;
+            const bool masked = step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window);
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                if (masked) {
+                    const int from = p.window ? position[i] + 1 - p.window - at : 0;
+                    weigh<true>(acc[i], c[i], now, m[i], o[i], tiles, from, position[i] + 1 - at, hi[i], lo[i]);
+                } else {
+                    weigh<false>(acc[i], c[i], now, m[i], o[i], tiles, 0, 16, hi[i], lo[i]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+                if (FULL || t < tiles) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const v8h v = *((const v8h*)(buffer + kKeyBytes + (t * 2 + h) * kOperand) + lane);
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) {
+                            o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[i][h], o[i][t], 0, 0, 0);
+                            o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[i][h], o[i][t], 0, 0, 0);
+                        }
+                    }
+                }
+        }
+        __syncthreads();
+    }
+
+    const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const float sum = add_xor32(add_xor16(m[i].sum));
+        const int row = w0 + 16 * i + li;
+        if (row >= rows) continue;
+        float* to = p.out + ((size_t)token[i] * p.heads + head[i]) * dim;
+        float scale = 1.0f / sum;
+        if (parts > 1) {
+            to = partial_values(p, share, slot) + (size_t)(row - r0) * dim;
+            scale = 1.0f;
+            if (lq == 0) partial_sums(p, share, slot)[row - r0] = v2f{m[i].base, sum};
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[i][t] * scale;
     }
 }
 
-// One wave a row (token, head), a key at a time.
-__global__ __launch_bounds__(64) void attention_kv8_row_kernel(AttentionKv8Call p) {
+// ---- rows whose keys were parted: a wave for each token and head, every lane four values of one part at a time
+__global__ __launch_bounds__(1024) void attention_kv8_merge_kernel(AttentionKv8Call p, Share few, Share many) {
     const KvBatchView& b = p.batch;
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, dim = p.cache.dim;
-    const int kv_heads = p.cache.kv_heads, kvh = h / (p.heads / kv_heads);
+    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
+    const int t = blockIdx.x, kvh = blockIdx.y;
+    // the request of the token: number t where all have one, else the one whose rows hold it
+    int request = -1;
     Kv8Request q{0, 0, 0};
-    int r = 0;
-    for (int base = 0; base < b.requests; base += 64) {
+    if (t < b.requests) {
+        q = kv8_request(b, t);
+        if (q.rows && t >= q.start && t < q.start + q.rows) request = t;
+    }
+    for (int base = 0; request < 0 && base < b.requests; base += 64) {
         Kv8Request mine{0, 0, 0};
         if (base + lane < b.requests) mine = kv8_request(b, base + lane);
-        const uint64_t found = __ballot(t >= mine.start && t < mine.start + mine.rows);
-        if (!found) continue;
-        const int from = __builtin_ctzll(found);
-        r = base + from;
+        const uint64_t holds = __ballot(t >= mine.start && t < mine.start + mine.rows);
+        if (!holds) continue;
+        const int from = __builtin_ctzll(holds);
+        request = base + from;
         q = Kv8Request{__shfl(mine.start, from, 64), __shfl(mine.rows, from, 64), __shfl(mine.length, from, 64)};
-        break;
     }
-    if (q.rows * (p.heads / kv_heads) <= kFewRows) return;
-    const int last = q.length - q.rows + (t - q.start), first = p.window ? max(0, last + 1 - p.window) : 0;
-    float x[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-    bool spoilt = false;
+    if (request < 0) return;
+    const Share& share = q.rows * group <= kFewRows ? few : many;
+    const int tiles = tiles_of(q, group, share);
+    const int* plan = (const int*)p.partial + share.at;
+    const int per = plan[0], first = plan[kHeader + request];
+    const int most = parts_of(most_steps(q, group, p.window, share.tile_rows), per);
+    for (int g = threadIdx.x >> 6; g < group; g += blockDim.x >> 6) {
+        const int row = (t - q.start) * group + g, tile = row / share.tile_rows;
+        const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
+        const int parts = parts_of(seen.end - seen.begin, per), item = first + (tiles - 1 - tile) * most;
+        if (parts == 1) continue;
+        // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
+        if (item < 0 || item > share.items - parts) continue;
+        const size_t slot = (size_t)item * p.cache.kv_heads + kvh, kv_heads = p.cache.kv_heads;
+        const v2f* sums = partial_sums(p, share, slot) + row % share.tile_rows;
+        const float* values = partial_values(p, share, slot) + (size_t)(row % share.tile_rows) * dim;
+        const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+        float base = kNoBase, sum = 0.0f;
+        for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
+        base = wave_max_f32(base);
+        // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
+        const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
+        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (own < abreast) {
+#pragma unroll 4
+            for (int i = own; i < parts; i += abreast) {
+                const v2f s = sums[i * sum_stride];
+                const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
+                const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+                sum = fmaf(s.y, alpha, sum);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        x[c] = lane + 64 * c < dim ? p.q_heads[((size_t)h * b.tokens + t) * dim + lane + 64 * c] : 0.0f;
-        spoilt = spoilt || !finite_f32(x[c]);
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+            }
+        }
+        // the parts abreast together, in their order
+        v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float total = 0.0f;
+        for (int k = 0; k < abreast; ++k) {
+            total += __shfl(sum, k * quads + quad, 64);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
+        }
+        if (own == 0) {
+            const float scale = 1.0f / total;
+            *(v4f*)(p.out + ((size_t)t * p.heads + kvh * group + g) * dim + 4 * quad) = all * scale;
+        }
     }
-    spoilt = __any(spoilt);
-    auto decode = [&](uint8_t c) { return p.cache.e4m3 ? __builtin_amdgcn_cvt_f32_fp8(c, 0) : (float)(int8_t)c; };
-    for (int k = first; k <= last; ++k) {
-        int id = b.table[(size_t)r * b.width + (k >> b.block_shift)];
-        const bool known = (unsigned)id < (unsigned)b.blocks;
-        if (!known) id = 0;
-        const size_t at = (size_t)id * kv_heads + kvh;
-        const int place = k & (b.block - 1);
-        float s = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < dim)
-                s = fmaf(x[c], decode(p.cache.keys[(at * b.block + place) * dim + lane + 64 * c]), s);
-        s = wave_sum_f32(s) * (p.cache.key_scales[at] * p.scale);
-        const float sv = p.cache.value_scales[at];
-        spoilt = spoilt || !known || !finite_f32(s) || !finite_f32(sv);
-        const float top = fmaxf(m, s), a = expf(m - top), e = expf(s - top);
-        m = top;
-        l = l * a + e;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < dim)
-                o[c] = o[c] * a + e * sv * decode(p.cache.values[(at * dim + lane + 64 * c) * b.block + place]);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < dim)
-            p.out[((size_t)t * p.heads + h) * dim + lane + 64 * c] = spoilt ? NAN : o[c] / l;
 }
 
 constexpr int kTarget = 768;                        // workgroups that the parts of a batch are cut for
+constexpr int kLeast = 4;                           // steps of a part at least
 
-Share few_share(const AttentionKv8Call&) { return Share{kFewRows, kTarget, kWaves, 1}; }
-
-// At most this many items: a request's parts are fewer than its steps / per + 1.
-size_t most_items(const AttentionKv8Call& call, const Share& share) {
-    const size_t kv = call.cache.kv_heads;
+// At most this many items of a KV head: a tile's parts are at most its steps / per + 1.
+int most_items(const AttentionKv8Call& call, const Share& share) {
+    const size_t kv = call.cache.kv_heads, group = call.heads / kv;
     const size_t longest = ((size_t)call.batch.width * call.batch.block + kStep - 1) / kStep + 1;
-    const size_t parts = std::min<size_t>((share.target + kv - 1) / kv + call.batch.requests,
-                                          call.batch.requests * ((longest + share.least - 1) / share.least));
-    return parts * kv;
+    size_t tiles = std::min(call.batch.requests, call.batch.tokens);
+    if (!share.few) tiles += (size_t)call.batch.tokens * group / share.tile_rows;
+    return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
+}
+
+size_t partial_floats(const AttentionKv8Call& call, const Share& share) {
+    return (kHeader + call.batch.requests + 3) / 4 * 4 + (size_t)share.items * call.cache.kv_heads * share.tile_rows * (call.cache.dim + 2);
+}
+
+bool has_few(const AttentionKv8Call& call) { return call.heads / call.cache.kv_heads <= kFewRows; }
+bool has_rows(const AttentionKv8Call& call) { return (size_t)call.batch.max_rows * (call.heads / call.cache.kv_heads) > kFewRows; }
+
+struct Shares {
+    Share few, many;
+    size_t floats;
+};
+Shares shares_of(const AttentionKv8Call& call) {
+    Shares s{{kFewRows, kTarget, kLeast, 1, 0, 0}, {16 * kWaves * row_tiles((call.cache.dim + 63) / 64), kTarget, kLeast, 0, 0, 0}, 0};
+    if (has_few(call)) {
+        s.few.items = most_items(call, s.few);
+        s.many.at = (partial_floats(call, s.few) + 3) / 4 * 4;
+        s.floats = s.many.at;
+    }
+    if (has_rows(call)) {
+        s.many.items = most_items(call, s.many);
+        s.floats = s.many.at + partial_floats(call, s.many);
+    }
+    return s;
+}
+
+template <int CC, bool FULL, bool E4M3>
+void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
+    const int grid = share.items * call.cache.kv_heads;
+    if (share.few) {
+        attention_kv8_few_kernel<CC, FULL, E4M3><<<grid, kThreads, 0, stream>>>(call, share);
+        return;
+    }
+    constexpr int kLds = 2 * 16 * CC * 1024;
+    if (kLds >= 65536) {                            // more than the default, with the static arrays
+        static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_kv8_rows_kernel<CC, FULL, E4M3>),
+                                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        (void)allowed;
+    }
+    attention_kv8_rows_kernel<CC, FULL, E4M3><<<grid, kThreads, kLds, stream>>>(call, share);
 }
 
 template <int CC, bool FULL>
-void launch_few(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
-    const int grid = (int)most_items(call, share);
-    if (call.cache.e4m3) attention_kv8_few_kernel<CC, FULL, true><<<grid, kThreads, 0, stream>>>(call, share);
-    else attention_kv8_few_kernel<CC, FULL, false><<<grid, kThreads, 0, stream>>>(call, share);
+void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
+    if (call.cache.e4m3) launch<CC, FULL, true>(call, share, stream);
+    else launch<CC, FULL, false>(call, share, stream);
 }
 
 }  // namespace
 
-size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call) {
-    const Share share = few_share(call);
-    return 4 * (64 + call.batch.requests + most_items(call, share) * share.tile_rows * (call.cache.dim + 2));
-}
+size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call) { return 4 * shares_of(call).floats; }
 
 void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
-    const int group = call.heads / call.cache.kv_heads, dim = call.cache.dim;
-    if (group <= kFewRows) {
-        const Share share = few_share(call);
+    const int dim = call.cache.dim, group = call.heads / call.cache.kv_heads;
+    const Shares shares = shares_of(call);
+    for (const Share& share : {shares.few, shares.many}) {
+        if (!share.items) continue;
         switch ((dim + 63) / 64 * 2 + (dim % 64 == 0)) {
-        case 2: launch_few<1, false>(call, share, stream); break;
-        case 3: launch_few<1, true>(call, share, stream); break;
-        case 4: launch_few<2, false>(call, share, stream); break;
-        case 5: launch_few<2, true>(call, share, stream); break;
-        case 6: launch_few<3, false>(call, share, stream); break;
-        case 7: launch_few<3, true>(call, share, stream); break;
-        case 8: launch_few<4, false>(call, share, stream); break;
-        default: launch_few<4, true>(call, share, stream); break;
+        case 2: launch<1, false>(call, share, stream); break;
+        case 3: launch<1, true>(call, share, stream); break;
+        case 4: launch<2, false>(call, share, stream); break;
+        case 5: launch<2, true>(call, share, stream); break;
+        case 6: launch<3, false>(call, share, stream); break;
+        case 7: launch<3, true>(call, share, stream); break;
+        case 8: launch<4, false>(call, share, stream); break;
+        default: launch<4, true>(call, share, stream); break;
         }
-        attention_kv8_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads), kThreads, 0, stream>>>(call, share);
     }
-    if (call.batch.max_rows * group > kFewRows)
-        attention_kv8_row_kernel<<<dim3(call.batch.tokens, call.heads), 64, 0, stream>>>(call);
+    if (((size_t)call.batch.width << call.batch.block_shift) <= (size_t)kLeast * kStep) return;   // no tile is parted
+    attention_kv8_merge_kernel<<<dim3(call.batch.tokens, call.cache.kv_heads), 64 * std::min(group, 16), 0, stream>>>(
+        call, shares.few, shares.many);
 }
 
 }  // namespace leafhip
