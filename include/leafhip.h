@@ -362,7 +362,7 @@ typedef struct lh_kv8 {
     void* values;           /* [blocks][kv_heads][dim][block] codes (a dim's tokens are consecutive), 16-byte aligned */
     float* key_scales;      /* [blocks][kv_heads] */
     float* value_scales;    /* [blocks][kv_heads] */
-    uint32_t kv_heads;
+    uint32_t kv_heads;      /* at most 1024 */
     uint32_t dim;           /* a multiple of 16, at most 256 */
     uint32_t format;        /* LH_KV8_* */
 } lh_kv8;

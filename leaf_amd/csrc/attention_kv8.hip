@@ -643,68 +643,70 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
 __global__ __launch_bounds__(1024) void attention_kv8_merge_kernel(AttentionKv8Call p, Share few, Share many) {
     const KvBatchView& b = p.batch;
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
-    const int t = blockIdx.x, kvh = blockIdx.y;
+    const int kvh = blockIdx.y;
+    for (int t = blockIdx.x; t < b.tokens; t += gridDim.x) {
     // the request of the token: number t where all have one, else the one whose rows hold it
-    int request = -1;
-    Kv8Request q{0, 0, 0};
-    if (t < b.requests) {
-        q = kv8_request(b, t);
-        if (q.rows && t >= q.start && t < q.start + q.rows) request = t;
-    }
-    for (int base = 0; request < 0 && base < b.requests; base += 64) {
-        Kv8Request mine{0, 0, 0};
-        if (base + lane < b.requests) mine = kv8_request(b, base + lane);
-        const uint64_t holds = __ballot(t >= mine.start && t < mine.start + mine.rows);
-        if (!holds) continue;
-        const int from = __builtin_ctzll(holds);
-        request = base + from;
-        q = Kv8Request{__shfl(mine.start, from, 64), __shfl(mine.rows, from, 64), __shfl(mine.length, from, 64)};
-    }
-    if (request < 0) return;
-    const Share& share = q.rows * group <= kFewRows ? few : many;
-    const int tiles = tiles_of(q, group, share);
-    const int* plan = (const int*)p.partial + share.at;
-    const int per = plan[0], first = plan[kHeader + request];
-    const int most = parts_of(most_steps(q, group, p.window, share.tile_rows), per);
-    for (int g = threadIdx.x >> 6; g < group; g += blockDim.x >> 6) {
-        const int row = (t - q.start) * group + g, tile = row / share.tile_rows;
-        const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
-        const int parts = parts_of(seen.end - seen.begin, per), item = first + (tiles - 1 - tile) * most;
-        if (parts == 1) continue;
-        // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
-        if (item < 0 || item > share.items - parts) continue;
-        const size_t slot = (size_t)item * p.cache.kv_heads + kvh, kv_heads = p.cache.kv_heads;
-        const v2f* sums = partial_sums(p, share, slot) + row % share.tile_rows;
-        const float* values = partial_values(p, share, slot) + (size_t)(row % share.tile_rows) * dim;
-        const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
-        float base = kNoBase, sum = 0.0f;
-        for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
-        base = wave_max_f32(base);
-        // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
-        const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
-        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        if (own < abreast) {
+        int request = -1;
+        Kv8Request q{0, 0, 0};
+        if (t < b.requests) {
+            q = kv8_request(b, t);
+            if (q.rows && t >= q.start && t < q.start + q.rows) request = t;
+        }
+        for (int base = 0; request < 0 && base < b.requests; base += 64) {
+            Kv8Request mine{0, 0, 0};
+            if (base + lane < b.requests) mine = kv8_request(b, base + lane);
+            const uint64_t holds = __ballot(t >= mine.start && t < mine.start + mine.rows);
+            if (!holds) continue;
+            const int from = __builtin_ctzll(holds);
+            request = base + from;
+            q = Kv8Request{__shfl(mine.start, from, 64), __shfl(mine.rows, from, 64), __shfl(mine.length, from, 64)};
+        }
+        if (request < 0) continue;
+        const Share& share = q.rows * group <= kFewRows ? few : many;
+        const int tiles = tiles_of(q, group, share);
+        const int* plan = (const int*)p.partial + share.at;
+        const int per = plan[0], first = plan[kHeader + request];
+        const int most = parts_of(most_steps(q, group, p.window, share.tile_rows), per);
+        for (int g = threadIdx.x >> 6; g < group; g += blockDim.x >> 6) {
+            const int row = (t - q.start) * group + g, tile = row / share.tile_rows;
+            const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
+            const int parts = parts_of(seen.end - seen.begin, per), item = first + (tiles - 1 - tile) * most;
+            if (parts == 1) continue;
+            // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
+            if (item < 0 || item > share.items - parts) continue;
+            const size_t slot = (size_t)item * p.cache.kv_heads + kvh, kv_heads = p.cache.kv_heads;
+            const v2f* sums = partial_sums(p, share, slot) + row % share.tile_rows;
+            const float* values = partial_values(p, share, slot) + (size_t)(row % share.tile_rows) * dim;
+            const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+            float base = kNoBase, sum = 0.0f;
+            for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
+            base = wave_max_f32(base);
+            // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
+            const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
+            v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            if (own < abreast) {
 #pragma unroll 4
-            for (int i = own; i < parts; i += abreast) {
-                const v2f s = sums[i * sum_stride];
-                const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
-                const float alpha = __builtin_amdgcn_exp2f(s.x - base);
-                sum = fmaf(s.y, alpha, sum);
+                for (int i = own; i < parts; i += abreast) {
+                    const v2f s = sums[i * sum_stride];
+                    const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
+                    const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+                    sum = fmaf(s.y, alpha, sum);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+                    for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+                }
             }
-        }
-        // the parts abreast together, in their order
-        v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        float total = 0.0f;
-        for (int k = 0; k < abreast; ++k) {
-            total += __shfl(sum, k * quads + quad, 64);
+            // the parts abreast together, in their order
+            v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            float total = 0.0f;
+            for (int k = 0; k < abreast; ++k) {
+                total += __shfl(sum, k * quads + quad, 64);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
-        }
-        if (own == 0) {
-            const float scale = 1.0f / total;
-            *(v4f*)(p.out + ((size_t)t * p.heads + kvh * group + g) * dim + 4 * quad) = all * scale;
+                for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
+            }
+            if (own == 0) {
+                const float scale = 1.0f / total;
+                *(v4f*)(p.out + ((size_t)t * p.heads + kvh * group + g) * dim + 4 * quad) = all * scale;
+            }
         }
     }
 }
@@ -789,7 +791,7 @@ void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
         }
     }
     if (((size_t)call.batch.width << call.batch.block_shift) <= (size_t)kLeast * kStep) return;   // no tile is parted
-    attention_kv8_merge_kernel<<<dim3(call.batch.tokens, call.cache.kv_heads), 64 * std::min(group, 16), 0, stream>>>(
+    attention_kv8_merge_kernel<<<dim3(std::min(call.batch.tokens, 1 << 20), call.cache.kv_heads), 64 * std::min(group, 16), 0, stream>>>(
         call, shares.few, shares.many);
 }
 

@@ -26,12 +26,12 @@ __device__ __forceinline__ bool finite_f32(float v) { return __builtin_fabsf(v) 
 // x / scale to the nearest whole number, ties to even, for |x| <= 127 scale
 // (1 + 2^-24): x * (1 / scale) rounds to it or, next to a border, to a
 // neighbour; x - q * scale is exact (a multiple of the smaller ulp, less than
-// scale), and decides.
+// scale), and decides.  (Of a NaN any code.)
 __device__ __forceinline__ int nearest_i8(float x, float scale, float inverse) {
     float q = __builtin_rintf(x * inverse);
     const float rest = fmaf(-q, scale, x), twice = 2.0f * __builtin_fabsf(rest);
-    if (twice > scale || (twice == scale && ((int)q & 1))) q += rest < 0.0f ? -1.0f : 1.0f;
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+    if (twice > scale || (twice == scale && ((int)q & 1))) q += __builtin_copysignf(1.0f, rest);
+    return (int)q;
 }
 
 // The smallest power of two, from 2^-40, times which 448 is at least `most`.

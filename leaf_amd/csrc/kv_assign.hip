@@ -151,9 +151,10 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
     };
     auto held_of = [&](int r) { return (cached[r] + b.block - 1) >> b.block_shift; };
 
-    const int thread = blockIdx.x * kThreads + threadIdx.x, threads = gridDim.x * kThreads;
+    const long long thread = blockIdx.x * kThreads + threadIdx.x, threads = gridDim.x * kThreads;
     const int rows = (int)min(all_rows, (long long)b.tokens);
-    for (int t = thread; t < b.tokens; t += threads) {
+    for (long long at = thread; at < b.tokens; at += threads) {
+        const int t = (int)at;
         int position = -1, slot = -1;
         if (t < rows) {
             const int r = find_last(starts, n, t);
@@ -167,11 +168,12 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
         b.positions[t] = position;
         b.slots[t] = slot;
     }
-    for (int u = thread; u < used; u += threads) {
+    for (long long at = thread; at < used; at += threads) {
+        const int u = (int)at;
         const int r = find_last(needed, n, u);
         b.table[(size_t)r * b.width + held_of(r) + (u - needed[r])] = taken_block(u);
     }
-    for (int g = thread; g < returned; g += threads) b.free_blocks[count + g] = returned_block(g);
+    for (long long at = thread; at < returned; at += threads) b.free_blocks[count + at] = returned_block((int)at);
 }
 
 }  // namespace
