@@ -25,6 +25,7 @@
 // dim's tokens together), and a lane's 16 keys lie in one block, with one scale.
 // Both K and V come as 16-byte loads; a key's dims are permuted alike in Q.
 #include <algorithm>
+#include <climits>
 
 #include "kv8.h"
 
@@ -66,10 +67,13 @@ __device__ __forceinline__ void widen(v4u codes, v8h& a, v8h& b) {
     }
 }
 
-// x = hi + lo to 22 bits, toward zero.
+// x = hi + lo to 22 bits, toward zero; x - hi in one instruction with hi as it is, an f16 half of a register.
 __device__ __forceinline__ void split2(float x, float y, v2h& hi, v2h& lo) {
     hi = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x, y));
-    lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x - (float)hi.x, y - (float)hi.y));
+    float dx, dy;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(dx) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(dy) : "v"(hi), "v"(y));
+    lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(dx, dy));
 }
 
 // A query row's operands for its lanes (one of four), and what its products are to be multiplied by.
@@ -113,39 +117,71 @@ __device__ __forceinline__ void load_query(const float* q, int dim, int lq, floa
 
 // What a lane's 16 keys of a step need of their block.
 struct KeyScales {
-    float key, value;                               // NaN where the block spoils the rows that see it
+    float key, value;
+    bool known;                                     // a block of the pool
+    // NaN where the block spoils the rows that see it.  (Apart from the loads: what looks at a value waits for it, and
+    // a step's are loaded a step ahead.)
+    __device__ __forceinline__ KeyScales checked() const {
+        return KeyScales{known && key >= 0.0f && key < INFINITY ? key : NAN,
+                         known && value >= 0.0f && value < INFINITY ? value : NAN, known};
+    }
 };
 
-// The keys of one request and KV head.
+// The keys of one request and KV head, for one lane.  A block's codes of a KV head are block * dim consecutive bytes,
+// those of all heads `stride`; a step begins at the start of a block or 64 tokens into one of 128.
 struct Keys {
     const int* table;
-    const uint8_t *keys, *values;
+    const uint8_t *keys, *values;                   // of the KV head, in block 0
     const float *key_scales, *value_scales;
-    int shift, blocks, kv_heads, kvh, dim, end;     // end: keys of the request
+    uint32_t stride, kv_heads;
+    int shift, blocks, dim, end;                    // end: keys of the request
+    uint32_t key_lane, value_lane;                  // offset of the lane's first code in a block
+    int key_group, value_group;                     // the lane's first key of a step, of its row of keys and its column of values
 
-    __device__ __forceinline__ int block_of(int key) const { return table[min(key, end - 1) >> shift]; }
+    __device__ __forceinline__ Keys(const AttentionKv8Call& p, int request, int kvh, int end_, int dim_, int li, int lq) {
+        const KvBatchView& b = p.batch;
+        table = b.table + (size_t)request * b.width;
+        shift = b.block_shift;
+        blocks = b.blocks;
+        kv_heads = p.cache.kv_heads;
+        dim = dim_;
+        end = end_;
+        const int mask = (1 << shift) - 1;
+        stride = kv_heads * (uint32_t)dim << shift;
+        keys = p.cache.keys + (size_t)kvh * (dim << shift);
+        values = p.cache.values + (size_t)kvh * (dim << shift);
+        key_scales = p.cache.key_scales + kvh;
+        value_scales = p.cache.value_scales + kvh;
+        key_group = 16 * (li >> 2);
+        value_group = 16 * lq;
+        key_lane = ((key_group & mask) + (li & 3)) * dim + 16 * lq;
+        value_lane = (li << shift) + (value_group & mask);
+    }
+    __device__ __forceinline__ int block_of(int key) const { return table[(uint32_t)min(key, end - 1) >> shift]; }
+    // The blocks of the lane's keys in a step: where its row of keys and its column of values are.
+    __device__ __forceinline__ int key_block(int step) const { return block_of(step * kStep + key_group); }
+    __device__ __forceinline__ int value_block(int step) const { return block_of(step * kStep + value_group); }
     __device__ __forceinline__ bool known(int id) const { return (unsigned)id < (unsigned)blocks; }
-    __device__ __forceinline__ size_t at(int id) const { return (size_t)(known(id) ? id : 0) * kv_heads + kvh; }
+    __device__ __forceinline__ uint32_t in_block(int step) const { return step * kStep & ((1 << shift) - 1); }
     __device__ __forceinline__ KeyScales scales(int id) const {
-        const size_t i = at(id);
-        KeyScales s{key_scales[i], value_scales[i]};
-        const bool fine = known(id);
-        if (!fine || !(s.key >= 0.0f && s.key < INFINITY)) s.key = NAN;
-        if (!fine || !(s.value >= 0.0f && s.value < INFINITY)) s.value = NAN;
-        return s;
+        const uint64_t i = (uint64_t)(known(id) ? (uint32_t)id : 0u) * kv_heads;
+        return KeyScales{key_scales[i], value_scales[i], known(id)};
     }
-    // Tile j of 16 keys: 16 codes of key 16 (li / 4) + 4 j + li % 4 from dim d on; id: the block of key 16 (li / 4).
+    // Where the lane's codes of a step begin.
+    __device__ __forceinline__ const uint8_t* key_codes(int id, int step) const {
+        return keys + (uint64_t)(known(id) ? (uint32_t)id : 0u) * stride + (key_lane + in_block(step) * dim);
+    }
+    __device__ __forceinline__ const uint8_t* value_codes(int id, int step) const {
+        return values + (uint64_t)(known(id) ? (uint32_t)id : 0u) * stride + (value_lane + in_block(step));
+    }
+    // 16 codes from dim 64 cc + 16 lq on of key 16 (li / 4) + 4 j + li % 4 (FULL: dim is a multiple of 64).
     template <bool FULL>
-    __device__ __forceinline__ v4u load_key(int id, int step, int j, int li, int d) const {
-        const int place = (step * kStep + 16 * (li >> 2) + 4 * j + (li & 3)) & ((1 << shift) - 1);
-        if (!FULL && d >= dim) return v4u{0, 0, 0, 0};
-        return *(const v4u*)(keys + ((at(id) << shift) + place) * dim + d);
+    __device__ __forceinline__ v4u load_key(const uint8_t* codes, int j, int cc, int lq) const {
+        if (!FULL && 64 * cc + 16 * lq >= dim) return v4u{0, 0, 0, 0};
+        return *(const v4u*)(codes + 4 * j * dim + 64 * cc);
     }
-    // 16 keys from 16 lq of dim d; id: the block of key 16 lq.
-    __device__ __forceinline__ v4u load_value(int id, int step, int lq, int d) const {
-        const int place = (step * kStep + 16 * lq) & ((1 << shift) - 1);
-        return *(const v4u*)(values + ((at(id) * dim + d) << shift) + place);
-    }
+    // 16 keys from 16 lq on of dim 16 t + li.
+    __device__ __forceinline__ v4u load_value(const uint8_t* codes, int t) const { return *(const v4u*)(codes + (16 * t << shift)); }
 };
 
 // Codes of `keys` tokens, the others zero.
@@ -225,13 +261,13 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
 // has workgroups for as many parts of each tile as its longest tile has.
 struct Share {
     int tile_rows, target, least;                   // least: steps a part has at least
-    int few;                                        // requests of at most kFewRows rows (1) or of more (0)
+    int from, to;                                   // takes the requests of from..to rows of a KV head
     int items;                                      // of a KV head, that there are workgroups and partial results for
     size_t at;                                      // where its partial results begin: in floats
 };
 __device__ __forceinline__ int tiles_of(const Kv8Request& q, int group, const Share& share) {
     const int rows = q.rows * group;
-    if (rows == 0 || (rows <= kFewRows) != (share.few != 0)) return 0;
+    if (rows < share.from || rows > share.to) return 0;
     return (rows + share.tile_rows - 1) / share.tile_rows;
 }
 // The steps that a tile's rows see.
@@ -255,9 +291,11 @@ struct Item {
 };
 
 // Which part of which tile of which request is item `index` (of one KV head);
-// request -1: none.  Every workgroup sums the whole batch, 256 requests at a time.
+// request -1: none.  Every workgroup sums the whole batch, a request a thread.
 // The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first item.
+template <int THREADS>
 __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
+    constexpr int kThreads = THREADS, kWaves = THREADS / 64;
     const KvBatchView& b = p.batch;
     const int window = p.window;
     __shared__ int sums[kWaves];
@@ -316,12 +354,6 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
     return found;
 }
 
-__device__ __forceinline__ Keys keys_of(const AttentionKv8Call& p, int request, int kvh, int end) {
-    const KvBatchView& b = p.batch;
-    return Keys{b.table + (size_t)request * b.width, p.cache.keys, p.cache.values, p.cache.key_scales, p.cache.value_scales,
-                b.block_shift, b.blocks, p.cache.kv_heads, kvh, p.cache.dim, end};
-}
-
 // Partial results: of each item its rows by dim floats; behind all of them each row's base and sum.
 __device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, const Share& share, size_t item) {
     return p.partial + share.at + (kHeader + p.batch.requests + 3) / 4 * 4 + item * share.tile_rows * p.cache.dim;
@@ -332,13 +364,13 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
 template <int CC, bool FULL, bool E4M3>
-__global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
+__global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item<kThreads>(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, row = min(li, rows - 1);
@@ -350,35 +382,37 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
     if (item.part >= parts) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
-    const Keys keys = keys_of(p, item.request, kvh, q.length);
+    const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
 
+    // Every load is issued a step ahead, as soon as its registers are free, and none under a condition, after which a
+    // wait for an older one would be for all: past its end a wave loads its last step again.
     v4u kr[4][CC], vr[TILES];
     KeyScales scales;
     auto load_keys = [&](int id, int step) {
+        const uint8_t* codes = keys.key_codes(id, step);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int cc = 0; cc < CC; ++cc) kr[j][cc] = keys.load_key<FULL>(id, step, j, li, 64 * cc + 16 * lq);
+            for (int cc = 0; cc < CC; ++cc) kr[j][cc] = keys.load_key<FULL>(codes, j, cc, lq);
     };
     auto load_values = [&](int id, int step) {
+        const uint8_t* codes = keys.value_codes(id, step);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-            if (FULL || t < tiles) vr[t] = keys.load_value(id, step, lq, 16 * t + li);
+        for (int t = 0; t < TILES; ++t) vr[t] = keys.load_value(codes, FULL ? t : min(t, tiles - 1));
         scales = keys.scales(id);
     };
-    auto block_k = [&](int step) { return keys.block_of(step * kStep + 16 * (li >> 2)); };
-    auto block_v = [&](int step) { return keys.block_of(step * kStep + 16 * lq); };
 
     v8h qh[CC][2], ql[CC][2];
     float c;
-    int step = begin + wave, ik = block_k(step), iv = block_v(step);
+    int step = begin + wave;
+    const int last = step < end ? step + (end - 1 - step) / kWaves * kWaves : begin;
+    auto after = [&](int s) { return min(s, last); };
+    int ik = keys.key_block(after(step)), iv = keys.value_block(after(step));
     load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
-    if (step < end) {
-        load_keys(ik, step);
-        load_values(iv, step);
-        ik = block_k(step + kWaves);
-        iv = block_v(step + kWaves);
-    }
+    load_keys(ik, after(step));
+    load_values(iv, after(step));
+    ik = keys.key_block(after(step + kWaves));
+    iv = keys.value_block(after(step + kWaves));
     v4f o[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -386,33 +420,36 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
     for (; step < end; step += kWaves) {
         v4f acc[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 4; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int cc = 0; cc < CC; ++cc) {
-                v8h k[2];
-                widen<E4M3>(kr[j][cc], k[0], k[1]);
+        for (int cc = 0; cc < CC; ++cc) {
+            v8h k[4][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], ql[cc][h], acc[j], 0, 0, 0);
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], qh[cc][h], acc[j], 0, 0, 0);
-                }
+            for (int j = 0; j < 4; ++j) widen<E4M3>(kr[j][cc], k[j][0], k[j][1]);
+            // (no product waits for the one before it)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][h], ql[cc][h], acc[j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][h], qh[cc][h], acc[j], 0, 0, 0);
             }
         }
-        const bool more = step + kWaves < end;
-        if (more) load_keys(ik, step + kWaves);
+        load_keys(ik, after(step + kWaves));
+        ik = keys.key_block(after(step + 2 * kWaves));
         v8h hi[2], lo[2];
+        const KeyScales now = scales.checked();
         const int at = step * kStep + 16 * lq;                     // the lane's first key
         if (step * kStep + kStep > low + 1 || p.window) {          // the wave's rows see different keys
             const int from = p.window ? position + 1 - p.window - at : 0;
-            weigh<true>(acc, c, scales, m, o, tiles, from, position + 1 - at, hi, lo);
+            weigh<true>(acc, c, now, m, o, tiles, from, position + 1 - at, hi, lo);
             // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
-            const int written = scales.value == scales.value ? q.length - at : 0;
+            const int written = now.known ? q.length - at : 0;
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
                 if (FULL || t < tiles) vr[t] = first_codes(vr[t], written);
         } else {
-            weigh<false>(acc, c, scales, m, o, tiles, 0, 16, hi, lo);
+            weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -425,11 +462,8 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
                     o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], hi[h], o[t], 0, 0, 0);
                 }
             }
-        if (more) {
-            load_values(iv, step + kWaves);
-            ik = block_k(step + 2 * kWaves);
-            iv = block_v(step + 2 * kWaves);
-        }
+        load_values(iv, after(step + kWaves));
+        iv = keys.value_block(after(step + 2 * kWaves));
     }
 
     // ---- the four waves' states together; wave w then has the tiles t % 4 = w
@@ -473,21 +507,26 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_few_kernel(AttentionKv
     }
 }
 
-// ---- more rows of a KV head: tiles of 64 or 128, K and V widened once for all of them through LDS
-// Rows per wave: two tiles of 16 up to heads of 128, one beyond (registers).
-constexpr int row_tiles(int cc) { return cc <= 2 ? 2 : 1; }
+// ---- more rows of a KV head: tiles of 128 or 256, K and V widened once for all of them through LDS
+// The softmax of a step's scores takes the vector pipes about as long as its products the matrix cores, so the waves
+// take turns: two groups of four waves, one of each on every SIMD, are half a step apart, and in each phase one group
+// has products only (those of the step's values before, then of its keys) and the other its softmax and its share of
+// the widening.  Barriers between the phases keep them so.
+constexpr int kRowsThreads = 512;
 
-template <int CC, bool FULL, bool E4M3>
-__global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
-    constexpr int TILES = 4 * CC, QT = row_tiles(CC), ROWS = 16 * QT * kWaves;
+template <int CC, int QT, bool FULL, bool E4M3>
+__global__ __launch_bounds__(kRowsThreads, 2) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC, ROWS = 16 * QT * 8;
     constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
     constexpr int kKeyBytes = 4 * CC * 2 * kOperand, kBuffer = 2 * kKeyBytes;
-    extern __shared__ __align__(16) uint8_t lds[];                 // two of [tile of keys][cc][half][lane], [tile of dims][half][lane]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+    // two sets: set n has the keys of step n, [tile of keys][cc][half][lane], and the values of step n - 1, [tile of dims][half][lane]
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
+    const bool second = wave >= 4;                                 // the group that is half a step behind
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item<kRowsThreads>(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, r0 = item.tile * ROWS, w0 = r0 + 16 * QT * wave;
@@ -497,7 +536,50 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     if (item.part >= parts) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
-    const Keys keys = keys_of(p, item.request, kvh, q.length);
+    const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
+
+    // staging: the 4 CC units of keys (tile, cc) and the 4 CC of values (tile of dims) of a set, every eighth by a wave
+    v4u code[CC];
+    bool known = true;
+    auto load = [&](int set, int ik, int iv) {
+        const uint8_t *k = keys.key_codes(ik, set), *v = keys.value_codes(iv, max(set - 1, begin));
+        known = keys.known(iv);
+#pragma unroll
+        for (int i = 0; i < CC; ++i) {
+            const int u = wave + 8 * i, t = u - 4 * CC;
+            if (u < 4 * CC) code[i] = keys.load_key<FULL>(k, u % 4, u / 4, lq);
+            else code[i] = keys.load_value(v, FULL ? t : min(t, tiles - 1));
+        }
+    };
+    auto store = [&](int set) {
+        uint8_t* buffer = lds + (set & 1) * kBuffer;
+#pragma unroll
+        for (int i = 0; i < CC; ++i) {
+            const int u = wave + 8 * i, t = u - 4 * CC;
+            v4u c = code[i];
+            // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
+            if (E4M3 && t >= 0 && (set * kStep > q.length || !__all(known)))
+                c = first_codes(c, known ? q.length - ((set - 1) * kStep + 16 * lq) : 0);
+            v8h a, b;
+            widen<E4M3>(c, a, b);
+            v8h* to = (v8h*)(buffer + (t < 0 ? ((u % 4) * CC + u / 4) * 2 * kOperand : kKeyBytes + t * 2 * kOperand)) + lane;
+            to[0] = a;
+            to[64] = b;
+        }
+    };
+    auto value_block = [&](int step) { return keys.value_block(max(step, begin)); };
+    // the first group stores set n + 1 with the softmax of step n, the second, which is later, set n + 2
+    const int lead = second ? 2 : 1;
+    load(begin, keys.key_block(begin), value_block(begin));
+    store(begin);
+    if (second) {
+        load(begin + 1, keys.key_block(begin + 1), value_block(begin));
+        store(begin + 1);
+    }
+    load(begin + lead, keys.key_block(begin + lead), value_block(begin + lead - 1));
+    KeyScales scales = keys.scales(value_block(begin));
+    int ik = keys.key_block(begin + lead + 1), iv = value_block(begin + lead), is = value_block(begin + 1);
+
     int position[QT], token[QT], head[QT];
     v8h qh[QT][CC][2], ql[QT][CC][2];
     float c[QT];
@@ -512,86 +594,86 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     // of the wave's rows: the first sees every key up to `low`, the last none after `high`
     const int low = before + min(w0, rows - 1) / group;
     const int high = w0 < rows ? before + min(w0 + 16 * QT - 1, rows - 1) / group : -1;
+    auto idle = [&](int step) { return step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window); };
 
-    // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
-    v4u kr[CC], vr[CC];
-    KeyScales scales, next_scales;
-    auto load = [&](int step, int ik, int iv) {
-#pragma unroll
-        for (int cc = 0; cc < CC; ++cc) {
-            kr[cc] = keys.load_key<FULL>(ik, step, wave, li, 64 * cc + 16 * lq);
-            const int t = wave + 4 * cc;
-            vr[cc] = FULL || t < tiles ? keys.load_value(iv, step, lq, 16 * t + li) : v4u{0, 0, 0, 0};
-        }
-        next_scales = keys.scales(iv);
-    };
-    auto store = [&](int step) {
-        uint8_t* buffer = lds + (step & 1) * kBuffer;
-        const int at = step * kStep + 16 * lq;
-        const int written = next_scales.value == next_scales.value ? q.length - at : 0;
-        // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
-        const bool clear = E4M3 && (step * kStep + kStep > q.length || __any(written == 0));
-#pragma unroll
-        for (int cc = 0; cc < CC; ++cc) {
-            v8h a, b;
-            widen<E4M3>(kr[cc], a, b);
-            v8h* to = (v8h*)(buffer + ((wave * CC + cc) * 2) * kOperand) + lane;
-            to[0] = a;
-            to[64] = b;
-            if (clear) vr[cc] = first_codes(vr[cc], written);
-            widen<E4M3>(vr[cc], a, b);
-            to = (v8h*)(buffer + kKeyBytes + ((wave + 4 * cc) * 2) * kOperand) + lane;
-            to[0] = a;
-            to[64] = b;
-        }
-    };
-    auto block_k = [&](int step) { return keys.block_of(step * kStep + 16 * (li >> 2)); };
-    auto block_v = [&](int step) { return keys.block_of(step * kStep + 16 * lq); };
-
-    v4f o[QT][TILES];
+    v4f o[QT][TILES], acc[QT][4];
+    v8h hi[QT][2], lo[QT][2];
     Softmax m[QT];
 #pragma unroll
     for (int i = 0; i < QT; ++i)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) o[i][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (begin < end) {
-        load(begin, block_k(begin), block_v(begin));
-        store(begin);
-        scales = next_scales;
-        load(begin + 1, block_k(begin + 1), block_v(begin + 1));
-    }
-    int ik = block_k(begin + 2), iv = block_v(begin + 2);
-    __syncthreads();
-    for (int step = begin; step < end; ++step) {
+    bool weighed = false;                                          // the step before has weights
+    lds_barrier();
+    if (second) lds_barrier();
+    for (int step = begin; step <= end; ++step) {
+        // ---- products
         const uint8_t* buffer = lds + (step & 1) * kBuffer;
-        const KeyScales now = scales;
-        if (step + 1 < end) {
-            store(step + 1);
-            scales = next_scales;
-            load(step + 2, ik, iv);                                // (past the end: the last block's, not used)
-            ik = block_k(step + 3);
-            iv = block_v(step + 3);
-        }
-        const bool idle = step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window);
-        if (!idle) {
-            v4f acc[QT][4];
+        if (weighed) {
+            // (the operands of a group of products are read before the products of the group before it; no product waits
+            // for the one before it)
+            v8h v[2][4];
+            auto read = [&](int g, v8h (&to)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+                for (int t = 0; t < 4; ++t)
+                    to[t] = *((const v8h*)(buffer + kKeyBytes + ((g / 2 * 4 + t) * 2 + g % 2) * kOperand) + lane);
+            };
+            read(0, v[0]);
 #pragma unroll
-                for (int i = 0; i < QT; ++i) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int g = 0; g < 2 * CC; ++g) {
+                const int t0 = g / 2 * 4, h = g % 2;
+                if (!FULL && t0 >= tiles) continue;                // (tiles past the last: of zeros)
+                if (g + 1 < 2 * CC) read(g + 1, v[(g + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int cc = 0; cc < CC; ++cc)
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const v8h k = *((const v8h*)(buffer + ((j * CC + cc) * 2 + h) * kOperand) + lane);
+                    for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][t], lo[i][h], o[i][t0 + t], 0, 0, 0);
 #pragma unroll
-                        for (int i = 0; i < QT; ++i) {
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[i][cc][h], acc[i][j], 0, 0, 0);
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i][cc][h], acc[i][j], 0, 0, 0);
-                        }
-                    }
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][t], hi[i][h], o[i][t0 + t], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            v8h hi[QT][2], lo[QT][2];
+        }
+        weighed = step < end && !idle(step);
+        if (weighed) {
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            v8h k[2][4];
+            auto read = [&](int g, v8h (&to)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to[j] = *((const v8h*)(buffer + (j * CC * 2 + g) * kOperand) + lane);
+            };
+            read(0, k[0]);
+#pragma unroll
+            for (int g = 0; g < 2 * CC; ++g) {
+                if (g + 1 < 2 * CC) read(g + 1, k[(g + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < QT; ++i)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[g & 1][j], ql[i][g / 2][g % 2], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < QT; ++i)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[g & 1][j], qh[i][g / 2][g % 2], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        lds_barrier();
+        // ---- softmax and staging.  (Every load is used a step later and none issued under a condition, after which a
+        // wait for an older one would be for all; past the end they are the last block's and not used.)
+        store(step + lead);
+        load(step + lead + 1, ik, iv);
+        ik = keys.key_block(step + lead + 2);
+        iv = value_block(step + lead + 1);
+        const KeyScales now = scales.checked();
+        if (weighed) {
             const int at = step * kStep + 16 * lq;
             const bool masked = step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window);
 #pragma unroll
@@ -603,22 +685,12 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
                     weigh<false>(acc[i], c[i], now, m[i], o[i], tiles, 0, 16, hi[i], lo[i]);
                 }
             }
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-                if (FULL || t < tiles) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const v8h v = *((const v8h*)(buffer + kKeyBytes + (t * 2 + h) * kOperand) + lane);
-#pragma unroll
-                        for (int i = 0; i < QT; ++i) {
-                            o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[i][h], o[i][t], 0, 0, 0);
-                            o[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[i][h], o[i][t], 0, 0, 0);
-                        }
-                    }
-                }
         }
-        __syncthreads();
+        scales = keys.scales(is);
+        is = value_block(step + 2);
+        lds_barrier();
     }
+    if (!second) lds_barrier();
 
     const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
 #pragma unroll
@@ -639,87 +711,143 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     }
 }
 
-// ---- rows whose keys were parted: a wave for each token and head, every lane four values of one part at a time
-__global__ __launch_bounds__(1024) void attention_kv8_merge_kernel(AttentionKv8Call p, Share few, Share many) {
-    const KvBatchView& b = p.batch;
+// ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
+// values of one part at a time
+__global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(AttentionKv8Call p, Share share) {
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
-    const int kvh = blockIdx.y;
-    for (int t = blockIdx.x; t < b.tokens; t += gridDim.x) {
-    // the request of the token: number t where all have one, else the one whose rows hold it
-        int request = -1;
-        Kv8Request q{0, 0, 0};
-        if (t < b.requests) {
-            q = kv8_request(b, t);
-            if (q.rows && t >= q.start && t < q.start + q.rows) request = t;
-        }
-        for (int base = 0; request < 0 && base < b.requests; base += 64) {
-            Kv8Request mine{0, 0, 0};
-            if (base + lane < b.requests) mine = kv8_request(b, base + lane);
-            const uint64_t holds = __ballot(t >= mine.start && t < mine.start + mine.rows);
-            if (!holds) continue;
-            const int from = __builtin_ctzll(holds);
-            request = base + from;
-            q = Kv8Request{__shfl(mine.start, from, 64), __shfl(mine.rows, from, 64), __shfl(mine.length, from, 64)};
-        }
-        if (request < 0) continue;
-        const Share& share = q.rows * group <= kFewRows ? few : many;
-        const int tiles = tiles_of(q, group, share);
-        const int* plan = (const int*)p.partial + share.at;
-        const int per = plan[0], first = plan[kHeader + request];
-        const int most = parts_of(most_steps(q, group, p.window, share.tile_rows), per);
-        for (int g = threadIdx.x >> 6; g < group; g += blockDim.x >> 6) {
-            const int row = (t - q.start) * group + g, tile = row / share.tile_rows;
-            const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
-            const int parts = parts_of(seen.end - seen.begin, per), item = first + (tiles - 1 - tile) * most;
-            if (parts == 1) continue;
-            // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
-            if (item < 0 || item > share.items - parts) continue;
-            const size_t slot = (size_t)item * p.cache.kv_heads + kvh, kv_heads = p.cache.kv_heads;
-            const v2f* sums = partial_sums(p, share, slot) + row % share.tile_rows;
-            const float* values = partial_values(p, share, slot) + (size_t)(row % share.tile_rows) * dim;
-            const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
-            float base = kNoBase, sum = 0.0f;
-            for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
-            base = wave_max_f32(base);
-            // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
-            const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
-            v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            if (own < abreast) {
+    const int request = blockIdx.x, kvh = blockIdx.y;
+    const Kv8Request q = kv8_request(p.batch, request);
+    if (!tiles_of(q, group, share)) return;
+    const int* plan = (const int*)p.partial + share.at;
+    const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
+    const int parts = parts_of(seen.end - seen.begin, plan[0]), item = plan[kHeader + request];
+    if (parts == 1) return;
+    // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
+    if (item < 0 || item > share.items - parts) return;
+    const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
+    const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+    // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
+    const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
+    for (int row = threadIdx.x >> 6; row < q.rows * group; row += blockDim.x >> 6) {
+        const v2f* sums = partial_sums(p, share, slot) + row;
+        const float* values = partial_values(p, share, slot) + (size_t)row * dim;
+        float base = kNoBase, sum = 0.0f;
+        for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
+        base = wave_max_f32(base);
+        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (own < abreast) {
 #pragma unroll 4
-                for (int i = own; i < parts; i += abreast) {
-                    const v2f s = sums[i * sum_stride];
-                    const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
-                    const float alpha = __builtin_amdgcn_exp2f(s.x - base);
-                    sum = fmaf(s.y, alpha, sum);
+            for (int i = own; i < parts; i += abreast) {
+                const v2f s = sums[i * sum_stride];
+                const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
+                const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+                sum = fmaf(s.y, alpha, sum);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
-                }
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
             }
-            // the parts abreast together, in their order
-            v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            float total = 0.0f;
-            for (int k = 0; k < abreast; ++k) {
-                total += __shfl(sum, k * quads + quad, 64);
+        }
+        // the parts abreast together, in their order
+        v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float total = 0.0f;
+        for (int k = 0; k < abreast; ++k) {
+            total += __shfl(sum, k * quads + quad, 64);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
-            }
-            if (own == 0) {
-                const float scale = 1.0f / total;
-                *(v4f*)(p.out + ((size_t)t * p.heads + kvh * group + g) * dim + 4 * quad) = all * scale;
-            }
+            for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
+        }
+        if (own == 0) {
+            const float scale = 1.0f / total;
+            *(v4f*)(p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim + 4 * quad) = all * scale;
         }
     }
 }
 
-constexpr int kTarget = 768;                        // workgroups that the parts of a batch are cut for
+// ---- the same of more rows: some workgroups a tile, a thread for four values of a row
+constexpr int kMergeSplit = 4;                      // workgroups of a tile
+__global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(AttentionKv8Call p, Share share) {
+    __shared__ int sums_of[kWaves], found[5];
+    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int kvh = blockIdx.x / kMergeSplit % p.cache.kv_heads, index = blockIdx.x / kMergeSplit / p.cache.kv_heads;
+    // tile `index` of the batch
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    int before = 0;
+    for (int base = 0; base < p.batch.requests; base += kThreads) {
+        const int r = base + threadIdx.x;
+        const Kv8Request mine = r < p.batch.requests ? kv8_request(p.batch, r) : Kv8Request{0, 0, 0};
+        const int tiles = tiles_of(mine, group, share);
+        int s = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(s, o, 64);
+            if (lane >= o) s += below;
+        }
+        if (lane == 63) sums_of[wave] = s;
+        __syncthreads();
+        int start = before + s - tiles;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) start += sums_of[w];
+            before += sums_of[w];
+        }
+        if (index >= start && index < start + tiles) {
+            found[0] = r;
+            found[1] = tiles - 1 - (index - start);
+            found[2] = mine.start;
+            found[3] = mine.rows;
+            found[4] = mine.length;
+        }
+        __syncthreads();
+        if (index < before) break;
+    }
+    if (found[0] < 0) return;
+    const int request = found[0], tile = found[1];
+    const Kv8Request q{found[2], found[3], found[4]};
+    const int* plan = (const int*)p.partial + share.at;
+    const int per = plan[0], first = plan[kHeader + request];
+    const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
+    const int parts = parts_of(seen.end - seen.begin, per);
+    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps(q, group, p.window, share.tile_rows), per);
+    if (parts == 1 || item < 0 || item > share.items - parts) return;
+    const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
+    const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+    const int r0 = tile * share.tile_rows, rows = min(share.tile_rows, q.rows * group - r0), quads = dim / 4;
+    for (int u = blockIdx.x % kMergeSplit * kThreads + threadIdx.x; u < rows * quads; u += kMergeSplit * kThreads) {
+        const int row = u / quads, quad = u % quads;
+        const v2f* sums = partial_sums(p, share, slot) + row;
+        const float* values = partial_values(p, share, slot) + (size_t)row * dim + 4 * quad;
+        float base = kNoBase, sum = 0.0f;
+        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) base = fmaxf(base, sums[i * sum_stride].x);
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            const v2f s = sums[i * sum_stride];
+            const v4f v = *(const v4f*)(values + i * stride);
+            const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+            sum = fmaf(s.y, alpha, sum);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+        }
+        const float scale = 1.0f / sum;
+        *(v4f*)(p.out + ((size_t)(q.start + (r0 + row) / group) * p.heads + kvh * group + (r0 + row) % group) * dim + 4 * quad) = x * scale;
+    }
+}
+
+constexpr int kTarget = 512;                        // workgroups that the parts of a batch are cut for
+constexpr int kRowsTarget = 256;
+constexpr int row_tiles(int cc) { return cc == 1 ? 2 : 1; }
+constexpr int kManyTokens = 64;
 constexpr int kLeast = 4;                           // steps of a part at least
 
-// At most this many items of a KV head: a tile's parts are at most its steps / per + 1.
-int most_items(const AttentionKv8Call& call, const Share& share) {
-    const size_t kv = call.cache.kv_heads, group = call.heads / kv;
-    const size_t longest = ((size_t)call.batch.width * call.batch.block + kStep - 1) / kStep + 1;
+// At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.
+int most_tiles(const AttentionKv8Call& call, const Share& share) {
+    const size_t group = call.heads / call.cache.kv_heads;
     size_t tiles = std::min(call.batch.requests, call.batch.tokens);
-    if (!share.few) tiles += (size_t)call.batch.tokens * group / share.tile_rows;
+    if (share.tile_rows > kFewRows) tiles += (size_t)call.batch.tokens * group / share.tile_rows;
+    return (int)tiles;
+}
+int most_items(const AttentionKv8Call& call, const Share& share) {
+    const size_t kv = call.cache.kv_heads, tiles = most_tiles(call, share);
+    const size_t longest = ((size_t)call.batch.width * call.batch.block + kStep - 1) / kStep + 1;
     return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
 }
 
@@ -727,21 +855,24 @@ size_t partial_floats(const AttentionKv8Call& call, const Share& share) {
     return (kHeader + call.batch.requests + 3) / 4 * 4 + (size_t)share.items * call.cache.kv_heads * share.tile_rows * (call.cache.dim + 2);
 }
 
-bool has_few(const AttentionKv8Call& call) { return call.heads / call.cache.kv_heads <= kFewRows; }
-bool has_rows(const AttentionKv8Call& call) { return (size_t)call.batch.max_rows * (call.heads / call.cache.kv_heads) > kFewRows; }
-
+// Which kernel takes which requests.  Where requests have kManyTokens new tokens on average the kernel of many rows
+// takes those of few too: the other's launch for the odd one is not worth it.
 struct Shares {
     Share few, many;
     size_t floats;
 };
 Shares shares_of(const AttentionKv8Call& call) {
-    Shares s{{kFewRows, kTarget, kLeast, 1, 0, 0}, {16 * kWaves * row_tiles((call.cache.dim + 63) / 64), kTarget, kLeast, 0, 0, 0}, 0};
-    if (has_few(call)) {
+    const int group = call.heads / call.cache.kv_heads;
+    const bool only_many = group > kFewRows || call.batch.tokens / kManyTokens >= call.batch.requests;
+    const bool only_few = (size_t)call.batch.max_rows * group <= kFewRows;
+    Shares s{{kFewRows, kTarget, kLeast, 1, kFewRows, 0, 0},
+             {16 * 8 * row_tiles((call.cache.dim + 63) / 64), kRowsTarget, kLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0}, 0};
+    if (only_few || !only_many) {
         s.few.items = most_items(call, s.few);
         s.many.at = (partial_floats(call, s.few) + 3) / 4 * 4;
         s.floats = s.many.at;
     }
-    if (has_rows(call)) {
+    if (!only_few) {
         s.many.items = most_items(call, s.many);
         s.floats = s.many.at + partial_floats(call, s.many);
     }
@@ -751,17 +882,18 @@ Shares shares_of(const AttentionKv8Call& call) {
 template <int CC, bool FULL, bool E4M3>
 void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
     const int grid = share.items * call.cache.kv_heads;
-    if (share.few) {
+    if (share.tile_rows == kFewRows) {
         attention_kv8_few_kernel<CC, FULL, E4M3><<<grid, kThreads, 0, stream>>>(call, share);
         return;
     }
     constexpr int kLds = 2 * 16 * CC * 1024;
+    constexpr auto kernel = attention_kv8_rows_kernel<CC, row_tiles(CC), FULL, E4M3>;
     if (kLds >= 65536) {                            // more than the default, with the static arrays
-        static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_kv8_rows_kernel<CC, FULL, E4M3>),
+        static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                               hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
         (void)allowed;
     }
-    attention_kv8_rows_kernel<CC, FULL, E4M3><<<grid, kThreads, kLds, stream>>>(call, share);
+    kernel<<<grid, kRowsThreads, kLds, stream>>>(call, share);
 }
 
 template <int CC, bool FULL>
@@ -791,8 +923,12 @@ void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
         }
     }
     if (((size_t)call.batch.width << call.batch.block_shift) <= (size_t)kLeast * kStep) return;   // no tile is parted
-    attention_kv8_merge_kernel<<<dim3(std::min(call.batch.tokens, 1 << 20), call.cache.kv_heads), 64 * std::min(group, 16), 0, stream>>>(
-        call, shares.few, shares.many);
+    if (shares.few.items)
+        attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
+                                         64 * std::min(kFewRows, group * call.batch.max_rows), 0, stream>>>(call, shares.few);
+    if (shares.many.items)
+        attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
+            call, shares.many);
 }
 
 }  // namespace leafhip
