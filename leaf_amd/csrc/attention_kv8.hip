@@ -293,9 +293,7 @@ struct Item {
 // Which part of which tile of which request is item `index` (of one KV head);
 // request -1: none.  Every workgroup sums the whole batch, a request a thread.
 // The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first item.
-template <int THREADS>
 __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
-    constexpr int kThreads = THREADS, kWaves = THREADS / 64;
     const KvBatchView& b = p.batch;
     const int window = p.window;
     __shared__ int sums[kWaves];
@@ -370,7 +368,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item<kThreads>(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, row = min(li, rows - 1);
@@ -507,208 +505,148 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
     }
 }
 
-// ---- more rows of a KV head: tiles of 128 or 256, K and V widened once for all of them through LDS
-// The softmax of a step's scores takes the vector pipes about as long as its products the matrix cores, so the waves
-// take turns: two groups of four waves, one of each on every SIMD, are half a step apart, and in each phase one group
-// has products only (those of the step's values before, then of its keys) and the other its softmax and its share of
-// the widening.  Barriers between the phases keep them so.
-constexpr int kRowsThreads = 512;
+// ---- more rows of a KV head: tiles of 64, 16 for a wave, K and V widened once for all of them through LDS
+constexpr int kTileRows = 16 * kWaves;
 
-template <int CC, int QT, bool FULL, bool E4M3>
-__global__ __launch_bounds__(kRowsThreads, 2) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
-    constexpr int TILES = 4 * CC, ROWS = 16 * QT * 8;
+template <int CC, bool FULL, bool E4M3>
+__global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC;
     constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
     constexpr int kKeyBytes = 4 * CC * 2 * kOperand, kBuffer = 2 * kKeyBytes;
-    // two sets: set n has the keys of step n, [tile of keys][cc][half][lane], and the values of step n - 1, [tile of dims][half][lane]
-    extern __shared__ __align__(16) uint8_t lds[];
+    extern __shared__ __align__(16) uint8_t lds[];                 // two of [tile of keys][cc][half][lane], [tile of dims][half][lane]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
-    const bool second = wave >= 4;                                 // the group that is half a step behind
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item<kRowsThreads>(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
-    const int rows = q.rows * group, r0 = item.tile * ROWS, w0 = r0 + 16 * QT * wave;
+    const int rows = q.rows * group, w0 = item.tile * kTileRows + 16 * wave;   // the wave's first row
     const int before = q.length - q.rows;                          // position of the first row
-    const Steps seen = steps_of(q, group, p.window, ROWS, item.tile);
+    const Steps seen = steps_of(q, group, p.window, kTileRows, item.tile);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
     if (item.part >= parts) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
+    const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
+    const int position = before + row / group;
+    v8h qh[CC][2], ql[CC][2];
+    float c;
+    load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
+    // of the wave's rows: the first sees every key up to `low`, the last none after `high`
+    const int low = before + min(w0, rows - 1) / group;
+    const int high = w0 < rows ? before + min(w0 + 15, rows - 1) / group : -1;
 
-    // staging: the 4 CC units of keys (tile, cc) and the 4 CC of values (tile of dims) of a set, every eighth by a wave
-    v4u code[CC];
+    // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
+    v4u kr[CC], vr[CC];
     bool known = true;
-    auto load = [&](int set, int ik, int iv) {
-        const uint8_t *k = keys.key_codes(ik, set), *v = keys.value_codes(iv, max(set - 1, begin));
+    auto load = [&](int step, int ik, int iv) {
+        const uint8_t *kc = keys.key_codes(ik, step), *vc = keys.value_codes(iv, step);
         known = keys.known(iv);
 #pragma unroll
-        for (int i = 0; i < CC; ++i) {
-            const int u = wave + 8 * i, t = u - 4 * CC;
-            if (u < 4 * CC) code[i] = keys.load_key<FULL>(k, u % 4, u / 4, lq);
-            else code[i] = keys.load_value(v, FULL ? t : min(t, tiles - 1));
+        for (int cc = 0; cc < CC; ++cc) {
+            kr[cc] = keys.load_key<FULL>(kc, wave, cc, lq);
+            vr[cc] = keys.load_value(vc, FULL ? wave + 4 * cc : min(wave + 4 * cc, tiles - 1));
         }
     };
-    auto store = [&](int set) {
-        uint8_t* buffer = lds + (set & 1) * kBuffer;
+    auto store = [&](int step) {
+        uint8_t* buffer = lds + (step & 1) * kBuffer;
+        // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
+        const bool clear = E4M3 && (step * kStep + kStep > q.length || !__all(known));
 #pragma unroll
-        for (int i = 0; i < CC; ++i) {
-            const int u = wave + 8 * i, t = u - 4 * CC;
-            v4u c = code[i];
-            // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
-            if (E4M3 && t >= 0 && (set * kStep > q.length || !__all(known)))
-                c = first_codes(c, known ? q.length - ((set - 1) * kStep + 16 * lq) : 0);
+        for (int cc = 0; cc < CC; ++cc) {
             v8h a, b;
-            widen<E4M3>(c, a, b);
-            v8h* to = (v8h*)(buffer + (t < 0 ? ((u % 4) * CC + u / 4) * 2 * kOperand : kKeyBytes + t * 2 * kOperand)) + lane;
+            widen<E4M3>(kr[cc], a, b);
+            v8h* to = (v8h*)(buffer + ((wave * CC + cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+            if (clear) vr[cc] = first_codes(vr[cc], known ? q.length - (step * kStep + 16 * lq) : 0);
+            widen<E4M3>(vr[cc], a, b);
+            to = (v8h*)(buffer + kKeyBytes + ((wave + 4 * cc) * 2) * kOperand) + lane;
             to[0] = a;
             to[64] = b;
         }
     };
-    auto value_block = [&](int step) { return keys.value_block(max(step, begin)); };
-    // the first group stores set n + 1 with the softmax of step n, the second, which is later, set n + 2
-    const int lead = second ? 2 : 1;
-    load(begin, keys.key_block(begin), value_block(begin));
+
+    v4f o[TILES];
+    Softmax m;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    // Every load is used a step later and none issued under a condition, after which a wait for an older one would be
+    // for all; past the end they are the last block's and not used.
+    load(begin, keys.key_block(begin), keys.value_block(begin));
     store(begin);
-    if (second) {
-        load(begin + 1, keys.key_block(begin + 1), value_block(begin));
-        store(begin + 1);
-    }
-    load(begin + lead, keys.key_block(begin + lead), value_block(begin + lead - 1));
-    KeyScales scales = keys.scales(value_block(begin));
-    int ik = keys.key_block(begin + lead + 1), iv = value_block(begin + lead), is = value_block(begin + 1);
-
-    int position[QT], token[QT], head[QT];
-    v8h qh[QT][CC][2], ql[QT][CC][2];
-    float c[QT];
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const int row = min(w0 + 16 * i + li, rows - 1);
-        token[i] = q.start + row / group;
-        head[i] = kvh * group + row % group;
-        position[i] = before + row / group;
-        load_query<CC, FULL>(p.q_heads + ((size_t)head[i] * p.batch.tokens + token[i]) * dim, dim, lq, p.scale, qh[i], ql[i], c[i]);
-    }
-    // of the wave's rows: the first sees every key up to `low`, the last none after `high`
-    const int low = before + min(w0, rows - 1) / group;
-    const int high = w0 < rows ? before + min(w0 + 16 * QT - 1, rows - 1) / group : -1;
-    auto idle = [&](int step) { return step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window); };
-
-    v4f o[QT][TILES], acc[QT][4];
-    v8h hi[QT][2], lo[QT][2];
-    Softmax m[QT];
-#pragma unroll
-    for (int i = 0; i < QT; ++i)
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) o[i][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    bool weighed = false;                                          // the step before has weights
+    load(begin + 1, keys.key_block(begin + 1), keys.value_block(begin + 1));
+    KeyScales scales = keys.scales(keys.value_block(begin));
+    int ik = keys.key_block(begin + 2), iv = keys.value_block(begin + 2), is = keys.value_block(begin + 1);
     lds_barrier();
-    if (second) lds_barrier();
-    for (int step = begin; step <= end; ++step) {
-        // ---- products
+    for (int step = begin; step < end; ++step) {
         const uint8_t* buffer = lds + (step & 1) * kBuffer;
-        if (weighed) {
-            // (the operands of a group of products are read before the products of the group before it; no product waits
-            // for the one before it)
-            v8h v[2][4];
-            auto read = [&](int g, v8h (&to)[4]) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    to[t] = *((const v8h*)(buffer + kKeyBytes + ((g / 2 * 4 + t) * 2 + g % 2) * kOperand) + lane);
-            };
-            read(0, v[0]);
-#pragma unroll
-            for (int g = 0; g < 2 * CC; ++g) {
-                const int t0 = g / 2 * 4, h = g % 2;
-                if (!FULL && t0 >= tiles) continue;                // (tiles past the last: of zeros)
-                if (g + 1 < 2 * CC) read(g + 1, v[(g + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][t], lo[i][h], o[i][t0 + t], 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][t], hi[i][h], o[i][t0 + t], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        weighed = step < end && !idle(step);
-        if (weighed) {
-#pragma unroll
-            for (int i = 0; i < QT; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            v8h k[2][4];
-            auto read = [&](int g, v8h (&to)[4]) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) to[j] = *((const v8h*)(buffer + (j * CC * 2 + g) * kOperand) + lane);
-            };
-            read(0, k[0]);
-#pragma unroll
-            for (int g = 0; g < 2 * CC; ++g) {
-                if (g + 1 < 2 * CC) read(g + 1, k[(g + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[g & 1][j], ql[i][g / 2][g % 2], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[g & 1][j], qh[i][g / 2][g % 2], acc[i][j], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        lds_barrier();
-        // ---- softmax and staging.  (Every load is used a step later and none issued under a condition, after which a
-        // wait for an older one would be for all; past the end they are the last block's and not used.)
-        store(step + lead);
-        load(step + lead + 1, ik, iv);
-        ik = keys.key_block(step + lead + 2);
-        iv = value_block(step + lead + 1);
+        store(step + 1);
+        load(step + 2, ik, iv);
+        ik = keys.key_block(step + 3);
+        iv = keys.value_block(step + 3);
         const KeyScales now = scales.checked();
-        if (weighed) {
-            const int at = step * kStep + 16 * lq;
-            const bool masked = step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window);
+        const bool idle = step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window);
+        if (!idle) {
+            v4f acc[4];
 #pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                if (masked) {
-                    const int from = p.window ? position[i] + 1 - p.window - at : 0;
-                    weigh<true>(acc[i], c[i], now, m[i], o[i], tiles, from, position[i] + 1 - at, hi[i], lo[i]);
-                } else {
-                    weigh<false>(acc[i], c[i], now, m[i], o[i], tiles, 0, 16, hi[i], lo[i]);
+            for (int j = 0; j < 4; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            // (no product waits for the one before it)
+#pragma unroll
+            for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8h k[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) k[j] = *((const v8h*)(buffer + ((j * CC + cc) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], ql[cc][h], acc[j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], qh[cc][h], acc[j], 0, 0, 0);
+                }
+            v8h hi[2], lo[2];
+            const int at = step * kStep + 16 * lq;
+            if (step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window)) {
+                const int from = p.window ? position + 1 - p.window - at : 0;
+                weigh<true>(acc, c, now, m, o, tiles, from, position + 1 - at, hi, lo);
+            } else {
+                weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
+            }
+#pragma unroll
+            for (int t0 = 0; t0 < TILES; t0 += 4) {
+                if (!FULL && t0 >= tiles) continue;                // (tiles past the last: copies of it, not kept)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8h v[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) v[t] = *((const v8h*)(buffer + kKeyBytes + ((t0 + t) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], lo[h], o[t0 + t], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], hi[h], o[t0 + t], 0, 0, 0);
                 }
             }
         }
         scales = keys.scales(is);
-        is = value_block(step + 2);
-        lds_barrier();
+        is = keys.value_block(step + 2);
+        lds_barrier();                                             // (the next loads stay in flight)
     }
-    if (!second) lds_barrier();
 
-    const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const float sum = add_xor32(add_xor16(m[i].sum));
-        const int row = w0 + 16 * i + li;
-        if (row >= rows) continue;
-        float* to = p.out + ((size_t)token[i] * p.heads + head[i]) * dim;
-        float scale = 1.0f / sum;
-        if (parts > 1) {
-            to = partial_values(p, share, slot) + (size_t)(row - r0) * dim;
-            scale = 1.0f;
-            if (lq == 0) partial_sums(p, share, slot)[row - r0] = v2f{m[i].base, sum};
-        }
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-            if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[i][t] * scale;
+    const float sum = add_xor32(add_xor16(m.sum));
+    if (w0 + li >= rows) return;
+    float* to = p.out + ((size_t)token * p.heads + head) * dim;
+    float scale = 1.0f / sum;
+    if (parts > 1) {
+        const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+        to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
+        scale = 1.0f;
+        if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = v2f{m.base, sum};
     }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+        if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[t] * scale;
 }
 
 // ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
@@ -832,11 +770,11 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     }
 }
 
-constexpr int kTarget = 512;                        // workgroups that the parts of a batch are cut for
-constexpr int kRowsTarget = 256;
-constexpr int row_tiles(int cc) { return cc == 1 ? 2 : 1; }
+// Workgroups that a batch's keys are cut for: those that the GPU holds at once.
+constexpr int few_target(int cc) { return cc <= 2 ? 512 : 256; }
+constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; }
 constexpr int kManyTokens = 64;
-constexpr int kLeast = 4;                           // steps of a part at least
+constexpr int kFewLeast = 4, kRowsLeast = 8;        // steps of a part at least
 
 // At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.
 int most_tiles(const AttentionKv8Call& call, const Share& share) {
@@ -865,8 +803,9 @@ Shares shares_of(const AttentionKv8Call& call) {
     const int group = call.heads / call.cache.kv_heads;
     const bool only_many = group > kFewRows || call.batch.tokens / kManyTokens >= call.batch.requests;
     const bool only_few = (size_t)call.batch.max_rows * group <= kFewRows;
-    Shares s{{kFewRows, kTarget, kLeast, 1, kFewRows, 0, 0},
-             {16 * 8 * row_tiles((call.cache.dim + 63) / 64), kRowsTarget, kLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0}, 0};
+    const int cc = (call.cache.dim + 63) / 64;
+    Shares s{{kFewRows, few_target(cc), kFewLeast, 1, kFewRows, 0, 0},
+             {kTileRows, rows_target(cc), kRowsLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0}, 0};
     if (only_few || !only_many) {
         s.few.items = most_items(call, s.few);
         s.many.at = (partial_floats(call, s.few) + 3) / 4 * 4;
@@ -887,13 +826,13 @@ void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream
         return;
     }
     constexpr int kLds = 2 * 16 * CC * 1024;
-    constexpr auto kernel = attention_kv8_rows_kernel<CC, row_tiles(CC), FULL, E4M3>;
+    constexpr auto kernel = attention_kv8_rows_kernel<CC, FULL, E4M3>;
     if (kLds >= 65536) {                            // more than the default, with the static arrays
         static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                               hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
         (void)allowed;
     }
-    kernel<<<grid, kRowsThreads, kLds, stream>>>(call, share);
+    kernel<<<grid, kThreads, kLds, stream>>>(call, share);
 }
 
 template <int CC, bool FULL>
@@ -922,11 +861,12 @@ void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
         default: launch<4, true>(call, share, stream); break;
         }
     }
-    if (((size_t)call.batch.width << call.batch.block_shift) <= (size_t)kLeast * kStep) return;   // no tile is parted
-    if (shares.few.items)
+    // (no tile is parted that has no more steps than a part at least)
+    const size_t steps = ((size_t)call.batch.width << call.batch.block_shift) / kStep + 1;
+    if (shares.few.items && steps > (size_t)kFewLeast)
         attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
                                          64 * std::min(kFewRows, group * call.batch.max_rows), 0, stream>>>(call, shares.few);
-    if (shares.many.items)
+    if (shares.many.items && steps > (size_t)kRowsLeast)
         attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
             call, shares.many);
 }

@@ -1,0 +1,1004 @@
+// Causal grouped-query attention of a ragged batch over an 8-bit cache in
+// blocks (include/leafhip.h: lh_attention_kv8), on the f16 matrix cores with
+// f32 accuracy.
+//
+// Operands.  A code is an f16 value exactly (8 bits fit 11).  A query row is
+// scaled by a power of two so that its largest value is below 2^15 and taken as
+// hi + lo, two f16 values of together 22 bits, and a weight likewise: two
+// products each for Q K^T and P V, summed in f32 (an f32 operand as bf16 values
+// would need three).
+//
+// Scales.  The score of a key is (q . code) c with c = query scale * key scale *
+// log2(e) / sqrt(dim).  A value's scale is 2^e f with 1 <= f < 2: weights are
+// formed as t = 2^(score + e - b + 8), relative to the largest weight times value
+// scale rather than the largest weight, so that w = t f, which is what meets the
+// value codes, keeps its 22 bits wherever it counts however far the scales of
+// blocks are apart, and the sum of weights adds t 2^-e.  b is a whole number per
+// row, at most 6 below the largest score + e so far (w < 2^15), so most steps
+// rescale nothing and a rescale is exact.
+//
+// Layout.  A step is 64 keys.  S^T = K Q^T by v_mfma_f32_16x16x32_f16 with lane
+// l = 16 lq + li: row li of its tile j of keys is key 16 (li / 4) + 4 j + li % 4
+// of the step, so that lane l then holds the scores of query row li for the 16
+// keys 16 lq + 4 j + r in a row: P is the other operand of O^T = V^T P^T without
+// leaving its registers, V's lanes read 16 codes of one dim (the cache keeps a
+// dim's tokens together), and a lane's 16 keys lie in one block, with one scale.
+// Both K and V come as 16-byte loads; a key's dims are permuted alike in Q.
+#include <algorithm>
+#include <climits>
+
+#include "kv8.h"
+
+namespace leafhip {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+constexpr int kStep = 64;                           // keys
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kFewRows = 16;                        // rows of a KV head in one tile
+constexpr int kHeader = 4;                          // integers before a plan's requests
+__host__ __device__ inline size_t plan_words(int requests) { return (kHeader + 2 * (size_t)requests + 3) / 4 * 4; }
+constexpr float kNoBase = -1e30f;
+constexpr float kSlack = 6.0f, kLift = 8.0f;
+
+// 16 codes as two operands.
+template <bool E4M3>
+__device__ __forceinline__ void widen(v4u codes, v8h& a, v8h& b) {
+    v2h h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (E4M3) {
+            h[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, false);
+            h[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], 1.0f, true);
+        } else {
+            // 0x6400 + (code + 128) is 1024 + code + 128
+            const uint32_t u = codes[i] ^ 0x80808080u;
+            const v2h offset = v2h{(_Float16)-1152.0f, (_Float16)-1152.0f};
+            h[2 * i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + offset;
+            h[2 * i + 1] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + offset;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[2 * i] = h[i].x; a[2 * i + 1] = h[i].y;
+        b[2 * i] = h[4 + i].x; b[2 * i + 1] = h[4 + i].y;
+    }
+}
+
+// x = hi + lo to 22 bits, toward zero; x - hi in one instruction with hi as it is, an f16 half of a register.
+__device__ __forceinline__ void split2(float x, float y, v2h& hi, v2h& lo) {
+    hi = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x, y));
+    float dx, dy;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(dx) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(dy) : "v"(hi), "v"(y));
+    lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(dx, dy));
+}
+
+// A query row's operands for its lanes (one of four), and what its products are to be multiplied by.
+template <int CC, bool FULL>
+__device__ __forceinline__ void load_query(const float* q, int dim, int lq, float scale, v8h (&hi)[CC][2], v8h (&lo)[CC][2], float& c) {
+    v4f f[CC][4];
+    float most = 0.0f;
+    bool spoilt = false;
+#pragma unroll
+    for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = 64 * cc + 16 * lq;
+            f[cc][e] = FULL || d < dim ? *(const v4f*)(q + d + 4 * e) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                most = fmaxf(most, __builtin_fabsf(f[cc][e][i]));
+                spoilt = spoilt || !finite_f32(f[cc][e][i]);
+            }
+        }
+    if (spoilt) most = INFINITY;
+    most = max_xor32(max_xor16(most));
+    // 2^k with the largest value in [2^14, 2^15) (from 2^-100 up; zeros and smaller values need none)
+    const int exponent = max((int)(__float_as_uint(most) >> 23), 127 - 100);
+    const float up = __uint_as_float((uint32_t)min(127 + 14 + 127 - exponent, 254) << 23);
+    const float down = __uint_as_float((uint32_t)max(exponent - 14, 1) << 23);
+#pragma unroll
+    for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v2h h, l;
+                split2(f[cc][e][2 * i] * up, f[cc][e][2 * i + 1] * up, h, l);
+                const int at = 4 * (e & 1) + 2 * i;
+                hi[cc][e >> 1][at] = h.x; hi[cc][e >> 1][at + 1] = h.y;
+                lo[cc][e >> 1][at] = l.x; lo[cc][e >> 1][at + 1] = l.y;
+            }
+    c = finite_f32(most) ? down * scale * 1.4426950408889634f : NAN;
+}
+
+// What a lane's 16 keys of a step need of their block.
+struct KeyScales {
+    float key, value;
+    bool known;                                     // a block of the pool
+    // NaN where the block spoils the rows that see it.  (Apart from the loads: what looks at a value waits for it, and
+    // a step's are loaded a step ahead.)
+    __device__ __forceinline__ KeyScales checked() const {
+        return KeyScales{known && key >= 0.0f && key < INFINITY ? key : NAN,
+                         known && value >= 0.0f && value < INFINITY ? value : NAN, known};
+    }
+};
+
+// The keys of one request and KV head, for one lane.  A block's codes of a KV head are block * dim consecutive bytes,
+// those of all heads `stride`; a step begins at the start of a block or 64 tokens into one of 128.
+struct Keys {
+    const int* table;
+    const uint8_t *keys, *values;                   // of the KV head, in block 0
+    const float *key_scales, *value_scales;
+    uint32_t stride, kv_heads;
+    int shift, blocks, dim, end;                    // end: keys of the request
+    uint32_t key_lane, value_lane;                  // offset of the lane's first code in a block
+    int key_group, value_group;                     // the lane's first key of a step, of its row of keys and its column of values
+
+    __device__ __forceinline__ Keys(const AttentionKv8Call& p, int request, int kvh, int end_, int dim_, int li, int lq) {
+        const KvBatchView& b = p.batch;
+        table = b.table + (size_t)request * b.width;
+        shift = b.block_shift;
+        blocks = b.blocks;
+        kv_heads = p.cache.kv_heads;
+        dim = dim_;
+        end = end_;
+        const int mask = (1 << shift) - 1;
+        stride = kv_heads * (uint32_t)dim << shift;
+        keys = p.cache.keys + (size_t)kvh * (dim << shift);
+        values = p.cache.values + (size_t)kvh * (dim << shift);
+        key_scales = p.cache.key_scales + kvh;
+        value_scales = p.cache.value_scales + kvh;
+        key_group = 16 * (li >> 2);
+        value_group = 16 * lq;
+        key_lane = ((key_group & mask) + (li & 3)) * dim + 16 * lq;
+        value_lane = (li << shift) + (value_group & mask);
+    }
+    __device__ __forceinline__ int block_of(int key) const { return table[(uint32_t)min(key, end - 1) >> shift]; }
+    // The blocks of the lane's keys in a step: where its row of keys and its column of values are.
+    __device__ __forceinline__ int key_block(int step) const { return block_of(step * kStep + key_group); }
+    __device__ __forceinline__ int value_block(int step) const { return block_of(step * kStep + value_group); }
+    __device__ __forceinline__ bool known(int id) const { return (unsigned)id < (unsigned)blocks; }
+    __device__ __forceinline__ uint32_t in_block(int step) const { return step * kStep & ((1 << shift) - 1); }
+    __device__ __forceinline__ KeyScales scales(int id) const {
+        const uint64_t i = (uint64_t)(known(id) ? (uint32_t)id : 0u) * kv_heads;
+        return KeyScales{key_scales[i], value_scales[i], known(id)};
+    }
+    // Where the lane's codes of a step begin.
+    __device__ __forceinline__ const uint8_t* key_codes(int id, int step) const {
+        return keys + (uint64_t)(known(id) ? (uint32_t)id : 0u) * stride + (key_lane + in_block(step) * dim);
+    }
+    __device__ __forceinline__ const uint8_t* value_codes(int id, int step) const {
+        return values + (uint64_t)(known(id) ? (uint32_t)id : 0u) * stride + (value_lane + in_block(step));
+    }
+    // 16 codes from dim 64 cc + 16 lq on of key 16 (li / 4) + 4 j + li % 4 (FULL: dim is a multiple of 64).
+    template <bool FULL>
+    __device__ __forceinline__ v4u load_key(const uint8_t* codes, int j, int cc, int lq) const {
+        if (!FULL && 64 * cc + 16 * lq >= dim) return v4u{0, 0, 0, 0};
+        return *(const v4u*)(codes + 4 * j * dim + 64 * cc);
+    }
+    // 16 keys from 16 lq on of dim 16 t + li.
+    __device__ __forceinline__ v4u load_value(const uint8_t* codes, int t) const { return *(const v4u*)(codes + (16 * t << shift)); }
+};
+
+// Codes of `keys` tokens, the others zero.
+__device__ __forceinline__ v4u first_codes(v4u codes, int keys) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = keys - 4 * i;
+        codes[i] = n >= 4 ? codes[i] : n <= 0 ? 0u : codes[i] & ((1u << 8 * n) - 1);
+    }
+    return codes;
+}
+
+// A row's online softmax: its base and its sum (this lane's keys).
+struct Softmax {
+    float base = kNoBase, sum = 0.0f;
+};
+
+// A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
+// MASKED: of these only keys [from, to) are visible.  Rescales o where the base moves.
+template <bool MASKED, int TILES>
+__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int tiles, int from, int to,
+                                      v8h (&hi)[2], v8h (&lo)[2]) {
+    const int exponent = min(max((int)(__float_as_uint(s.value) >> 23) - 127, -64), 64);
+    const float e = (float)exponent, down = __uint_as_float((uint32_t)(127 - exponent) << 23), f = s.value * down;
+    c *= s.key;
+    c = c < 1e-37f ? 1e-37f : c;                    // (a masked key is minus infinity times it)
+    if (MASKED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (4 * j + r < from || 4 * j + r >= to) acc[j][r] = -INFINITY;
+    }
+    float top = acc[0][0];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[j][r]);
+    top = fmaf(top, c, e);
+    top = max_xor32(max_xor16(top));
+    if (__any(top > m.base + kSlack)) {
+        const float base = top > m.base + kSlack ? __builtin_ceilf(top) : m.base;
+        const float alpha = __builtin_amdgcn_exp2f(m.base - base);
+        m.base = base;
+        m.sum *= alpha;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            if (t < tiles) o[t] = o[t] * alpha;
+    }
+    const float shift = e + (kLift - m.base);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float t = __builtin_amdgcn_exp2f(fmaf(acc[j][r], c, shift));
+            w[r] = t * f;
+            if (MASKED && (4 * j + r < from || 4 * j + r >= to)) t = w[r] = 0.0f;
+            sum += t;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v2h h, l;
+            split2(w[2 * i], w[2 * i + 1], h, l);
+            const int at = 4 * (j & 1) + 2 * i;
+            hi[j >> 1][at] = h.x; hi[j >> 1][at + 1] = h.y;
+            lo[j >> 1][at] = l.x; lo[j >> 1][at + 1] = l.y;
+        }
+    }
+    m.sum = fmaf(sum, down, m.sum);
+}
+
+// How a batch's work is shared out.  A request's rows of a KV head make tiles of
+// `tile_rows`; a tile's steps are cut into equal parts of at most `per`, per
+// chosen so that all parts of the batch are about `target` workgroups.  A request
+// has workgroups for as many parts of each tile as its longest tile has.
+struct Share {
+    int tile_rows, target, least;                   // least: steps a part has at least
+    int from, to;                                   // takes the requests of from..to rows of a KV head
+    int items;                                      // of a KV head, that there are workgroups and partial results for
+    size_t slots;                                   // partial results that there is room for
+    size_t at;                                      // where they begin: in floats
+};
+__device__ __forceinline__ int tiles_of(const Kv8Request& q, int group, const Share& share) {
+    const int rows = q.rows * group;
+    if (rows < share.from || rows > share.to) return 0;
+    return (rows + share.tile_rows - 1) / share.tile_rows;
+}
+// The steps that a tile's rows see.
+struct Steps {
+    int begin, end;
+};
+__device__ __forceinline__ Steps steps_of(const Kv8Request& q, int group, int window, int tile_rows, int tile) {
+    const int r0 = tile * tile_rows, last = min(r0 + tile_rows, q.rows * group) - 1, before = q.length - q.rows;
+    return Steps{window ? max(0, before + r0 / group + 1 - window) / kStep : 0, (before + last / group) / kStep + 1};
+}
+// No tile of a request has more.
+__device__ __forceinline__ int most_steps(const Kv8Request& q, int group, int window, int tile_rows) {
+    const int all = (q.length - 1) / kStep + 1;
+    return window ? (int)min((long long)all, ((long long)window + tile_rows / group) / kStep + 3) : all;
+}
+__device__ __forceinline__ int parts_of(int steps, int per) { return (steps + per - 1) / per; }
+
+struct Item {
+    int request, tile, part, index;                 // index: of the tile's first part among the KV head's items
+    Kv8Request q;
+};
+
+// Which part of which tile of which request is item `index` (of one KV head);
+// request -1: none.  Every workgroup sums the whole batch, a request a thread.
+// The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first item.
+template <int THREADS>
+__device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
+    constexpr int kThreads = THREADS, kWaves = THREADS / 64;
+    const KvBatchView& b = p.batch;
+    const int window = p.window;
+    __shared__ int sums[kWaves];
+    __shared__ Item found;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    auto steps = [&](const Kv8Request& q) {
+        return (float)tiles_of(q, group, share) * (float)most_steps(q, group, window, share.tile_rows);
+    };
+    Kv8Request mine{0, 0, 0};
+    float all = 0.0f;
+    for (int r = threadIdx.x; r < b.requests; r += kThreads) {
+        mine = kv8_request(b, r);
+        all += steps(mine);
+    }
+    all = wave_sum_f32(all);
+    __shared__ float totals[kWaves];
+    if (lane == 0) totals[wave] = all;
+    if (threadIdx.x == 0) found.request = -1;
+    __syncthreads();
+    all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += totals[w];
+    per = max(share.least, (int)fminf(all * (float)p.cache.kv_heads / (float)share.target * 1.0001f + 1.0f, 1e9f));
+    int before = 0;
+    for (int base = 0; base < b.requests; base += kThreads) {
+        const int r = base + threadIdx.x;
+        if (b.requests > kThreads) mine = r < b.requests ? kv8_request(b, r) : Kv8Request{0, 0, 0};
+        const int tiles = tiles_of(mine, group, share), parts = parts_of(most_steps(mine, group, window, share.tile_rows), per);
+        const int items = tiles ? tiles * parts : 0;
+        int s = items;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(s, o, 64);
+            if (lane >= o) s += below;
+        }
+        if (lane == 63) sums[wave] = s;
+        __syncthreads();
+        int start = before + s - items, all_items = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) start += sums[w];
+            all_items += sums[w];
+        }
+        if (index >= start && index < start + items) {
+            const int i = index - start;
+            // the longest tiles (the last) first
+            found = Item{r, tiles - 1 - i / parts, i % parts, start + i / parts * parts, mine};
+        }
+        // the first workgroup leaves the plan for the merge
+        if (blockIdx.x == 0 && r < b.requests) ((int*)p.partial)[share.at + kHeader + r] = start;
+        if (blockIdx.x == 0 && r == 0) ((int*)p.partial)[share.at] = per;
+        before += all_items;
+        __syncthreads();
+        if (index < before && blockIdx.x) break;
+    }
+    return found;
+}
+
+// Partial results: of each item its rows by dim floats; behind all of them each row's base and sum.
+__device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, const Share& share, size_t slot) {
+    return p.partial + share.at + plan_words(p.batch.requests) + slot * share.tile_rows * p.cache.dim;
+}
+__device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Share& share, size_t slot) {
+    return (v2f*)partial_values(p, share, share.slots) + slot * share.tile_rows;
+}
+
+// ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
+// All steps of the batch, request after request and KV head after KV head, are one line, cut into equal pieces of which
+// each workgroup takes one, however ragged the requests are; a piece is one segment of a request's KV head or several.
+// A segment's partial result has the number of its workgroup plus that of its request and KV head for a slot.
+struct Line {
+    long long total;                                // steps
+    int groups;                                     // workgroups that take a piece
+    __device__ __forceinline__ long long begin(int group) const { return total * group / groups; }
+    __device__ __forceinline__ int group_of(long long step) const { return (int)(((step + 1) * groups + total - 1) / total) - 1; }
+};
+// Of a request of the line: its steps of a KV head, before it (of one KV head) and its own.
+struct OnLine {
+    int request, steps;
+    long long before;
+    Kv8Request q;
+};
+__device__ __forceinline__ int line_steps(const AttentionKv8Call& p, const Kv8Request& q, int group, const Share& share) {
+    if (!tiles_of(q, group, share)) return 0;
+    const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
+    return seen.end - seen.begin;
+}
+// The plan for the merge: the line's steps and workgroups, then each request's steps before it.
+__device__ __forceinline__ long long* line_plan(const AttentionKv8Call& p, const Share& share) { return (long long*)(p.partial + share.at); }
+
+// The line, and the request of the first step of the workgroup's piece (request -1: it has none).
+__device__ __forceinline__ OnLine find_piece(const AttentionKv8Call& p, int group, const Share& share, Line& line) {
+    const KvBatchView& b = p.batch;
+    __shared__ long long sums[kWaves];
+    __shared__ OnLine found;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Kv8Request mine{0, 0, 0};
+    int steps = 0;
+    long long before = 0, at = -1;
+    if (threadIdx.x == 0) found.request = -1;
+    // up to a request a thread one round serves both the sum and the search
+    const bool once = b.requests <= kThreads;
+    for (int round = once; round < 2; ++round) {
+        before = 0;
+        for (int base = 0; base < b.requests; base += kThreads) {
+            const int r = base + threadIdx.x;
+            mine = r < b.requests ? kv8_request(b, r) : Kv8Request{0, 0, 0};
+            steps = line_steps(p, mine, group, share);
+            long long s = steps;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const long long below = __shfl_up(s, o, 64);
+                if (lane >= o) s += below;
+            }
+            __syncthreads();
+            if (lane == 63) sums[wave] = s;
+            __syncthreads();
+            long long start = before + s - steps;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if (w < wave) start += sums[w];
+                before += sums[w];
+            }
+            if (round == 1) {
+                if (once) line.total = before * p.cache.kv_heads;
+                if (once || base == 0) {
+                    line.groups = (int)max(1LL, min((long long)gridDim.x, line.total / share.least));
+                    at = (int)blockIdx.x < line.groups && line.total ? line.begin(blockIdx.x) : -1;
+                }
+                const long long from = start * p.cache.kv_heads, to = (start + steps) * p.cache.kv_heads;
+                if (at >= from && at < to) found = OnLine{r, steps, start, mine};
+                if (blockIdx.x == 0 && r < b.requests) line_plan(p, share)[2 + r] = start;
+            }
+        }
+        if (round == 0) line.total = before * p.cache.kv_heads;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        line_plan(p, share)[0] = line.total;
+        line_plan(p, share)[1] = line.groups;
+    }
+    __syncthreads();
+    return found;
+}
+
+template <int CC, bool FULL, bool E4M3>
+__global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
+    const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
+    const int tiles = FULL ? TILES : dim / 16;
+    __shared__ v4f values[kWaves][TILES][64];
+    __shared__ float bases[kWaves][16], sums[kWaves][16];
+    Line line;
+    OnLine on = find_piece(p, group, share, line);
+    if (on.request < 0) return;
+    long long at_step = line.begin(blockIdx.x);
+    const long long piece_end = line.begin(blockIdx.x + 1);
+#pragma unroll 1
+    while (true) {
+    const Kv8Request& q = on.q;
+    const int within = (int)(at_step - on.before * kv_heads), kvh = within / on.steps, skipped = within - kvh * on.steps;
+    const int taken = (int)min((long long)(on.steps - skipped), piece_end - at_step);
+    const int rows = q.rows * group, row = min(li, rows - 1);
+    const int token = q.start + row / group, head = kvh * group + row % group;
+    const int position = q.length - q.rows + row / group;
+    const int low = q.length - q.rows;                             // of the first row
+    const int begin = steps_of(q, group, p.window, share.tile_rows, 0).begin + skipped, end = begin + taken;
+    const Keys keys(p, on.request, kvh, q.length, dim, li, lq);
+
+    // Every load is issued a step ahead, as soon as its registers are free, and none under a condition, after which a
+    // wait for an older one would be for all: past its end a wave loads its last step again.
+    v4u kr[4][CC], vr[TILES];
+    KeyScales scales;
+    auto load_keys = [&](int id, int step) {
+        const uint8_t* codes = keys.key_codes(id, step);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int cc = 0; cc < CC; ++cc) kr[j][cc] = keys.load_key<FULL>(codes, j, cc, lq);
+    };
+    auto load_values = [&](int id, int step) {
+        const uint8_t* codes = keys.value_codes(id, step);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) vr[t] = keys.load_value(codes, FULL ? t : min(t, tiles - 1));
+        scales = keys.scales(id);
+    };
+
+    v8h qh[CC][2], ql[CC][2];
+    float c;
+    int step = begin + wave;
+    const int last = step < end ? step + (end - 1 - step) / kWaves * kWaves : begin;
+    auto after = [&](int s) { return min(s, last); };
+    int ik = keys.key_block(after(step)), iv = keys.value_block(after(step));
+    load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
+    load_keys(ik, after(step));
+    load_values(iv, after(step));
+    ik = keys.key_block(after(step + kWaves));
+    iv = keys.value_block(after(step + kWaves));
+    v4f o[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    Softmax m;
+    for (; step < end; step += kWaves) {
+        v4f acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            v8h k[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j][0] = __builtin_bit_cast(v8h, kr[j][cc]); k[j][1] = k[j][0];
+            // (no product waits for the one before it)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][h], ql[cc][h], acc[j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][h], qh[cc][h], acc[j], 0, 0, 0);
+            }
+        }
+        load_keys(ik, after(step + kWaves));
+        ik = keys.key_block(after(step + 2 * kWaves));
+        v8h hi[2], lo[2];
+        const KeyScales now = scales.checked();
+        const int at = step * kStep + 16 * lq;                     // the lane's first key
+        if (step * kStep + kStep > low + 1 || p.window) {          // the wave's rows see different keys
+            const int from = p.window ? position + 1 - p.window - at : 0;
+            weigh<true>(acc, c, now, m, o, tiles, from, position + 1 - at, hi, lo);
+            // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
+            const int written = now.known ? q.length - at : 0;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+                if (FULL || t < tiles) vr[t] = first_codes(vr[t], written);
+        } else {
+            weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            if (FULL || t < tiles) {
+                v8h v[2];
+                v[0] = __builtin_bit_cast(v8h, vr[t]); v[1] = v[0];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], lo[h], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], hi[h], o[t], 0, 0, 0);
+                }
+            }
+        load_values(iv, after(step + kWaves));
+        iv = keys.value_block(after(step + 2 * kWaves));
+    }
+
+    // ---- the four waves' states together; wave w then has the tiles t % 4 = w
+    m.sum = add_xor32(add_xor16(m.sum));
+    if (lq == 0) {
+        bases[wave][li] = m.base;
+        sums[wave][li] = m.sum;
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+        if (FULL || t < tiles) values[wave][t][lane] = o[t];
+    lds_barrier();
+    float base = kNoBase, sum = 0.0f, alpha[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) base = fmaxf(base, bases[w][li]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        alpha[w] = __builtin_amdgcn_exp2f(bases[w][li] - base);
+        sum = fmaf(sums[w][li], alpha[w], sum);
+    }
+    if (li < rows) {
+        float* to = p.out + ((size_t)token * p.heads + head) * dim;
+        float scale = 1.0f / sum;
+        if (taken < on.steps) {
+            const size_t slot = (size_t)blockIdx.x + (size_t)on.request * kv_heads + kvh;
+            to = partial_values(p, share, slot) + (size_t)li * dim;
+            scale = 1.0f;
+            if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = v2f{base, sum};
+        }
+        for (int t = wave; t < tiles; t += kWaves) {
+            v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const v4f v = values[w][t][lane];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha[w], x[r]);
+            }
+            *(v4f*)(to + 16 * t + 4 * lq) = x * scale;
+        }
+    }
+    at_step += taken;
+    if (at_step >= piece_end) return;
+    if (skipped + taken == on.steps && kvh == kv_heads - 1) {
+        // the next request on the line (there is one: the piece goes on)
+        on.before += on.steps;
+        do {
+            on.q = kv8_request(p.batch, ++on.request);
+            on.steps = line_steps(p, on.q, group, share);
+        } while (!on.steps && on.request + 1 < p.batch.requests);
+        if (!on.steps) return;
+    }
+    lds_barrier();                                                 // the states are read
+    }
+}
+
+// ---- more rows of a KV head: tiles of 128 or 256, K and V widened once for all of them through LDS
+// The softmax of a step's scores takes the vector pipes about as long as its products the matrix cores, so the waves
+// take turns: two groups of four waves, one of each on every SIMD, are half a step apart, and in each phase one group
+// has products only (those of the step's values before, then of its keys) and the other its softmax and its share of
+// the widening.  Barriers between the phases keep them so.
+constexpr int kRowsThreads = 256;
+template <int CC, int QT, bool FULL, bool E4M3>
+__global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC, ROWS = 16 * QT * kWaves;
+    constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
+    constexpr int kKeyBytes = 4 * CC * 2 * kOperand, kBuffer = 2 * kKeyBytes;
+    extern __shared__ __align__(16) uint8_t lds[];                 // two of [tile of keys][cc][half][lane], [tile of dims][half][lane]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
+    const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
+    const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
+    int per;
+    const Item item = find_item<kThreads>(p, group, share, blockIdx.x / kv_heads, per);
+    if (item.request < 0) return;
+    const Kv8Request& q = item.q;
+    const int rows = q.rows * group, r0 = item.tile * ROWS, w0 = r0 + 16 * QT * wave;
+    const int before = q.length - q.rows;                          // position of the first row
+    const Steps seen = steps_of(q, group, p.window, ROWS, item.tile);
+    const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
+    if (item.part >= parts) return;
+    const int begin = seen.begin + (int)((long long)item.part * steps / parts);
+    const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
+    const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
+    int position[QT], token[QT], head[QT];
+    v8h qh[QT][CC][2], ql[QT][CC][2];
+    float c[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const int row = min(w0 + 16 * i + li, rows - 1);
+        token[i] = q.start + row / group;
+        head[i] = kvh * group + row % group;
+        position[i] = before + row / group;
+        load_query<CC, FULL>(p.q_heads + ((size_t)head[i] * p.batch.tokens + token[i]) * dim, dim, lq, p.scale, qh[i], ql[i], c[i]);
+    }
+    // of the wave's rows: the first sees every key up to `low`, the last none after `high`
+    const int low = before + min(w0, rows - 1) / group;
+    const int high = w0 < rows ? before + min(w0 + 16 * QT - 1, rows - 1) / group : -1;
+
+    // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
+    v4u kr[CC], vr[CC];
+    bool known = true;
+    auto load = [&](int step, int ik, int iv) {
+        const uint8_t *kc = keys.key_codes(ik, step), *vc = keys.value_codes(iv, step);
+        known = keys.known(iv);
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            kr[cc] = keys.load_key<FULL>(kc, wave, cc, lq);
+            const int t = wave + 4 * cc;
+            vr[cc] = keys.load_value(vc, FULL ? t : min(t, tiles - 1));
+        }
+    };
+    auto store = [&](int step) {
+        uint8_t* buffer = lds + (step & 1) * kBuffer;
+        const int at = step * kStep + 16 * lq;
+        const bool clear = E4M3 && (step * kStep + kStep > q.length || !__all(known));
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            v8h a, b;
+            widen<E4M3>(kr[cc], a, b);
+            v8h* to = (v8h*)(buffer + ((wave * CC + cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+            if (clear) vr[cc] = first_codes(vr[cc], known ? q.length - at : 0);
+            widen<E4M3>(vr[cc], a, b);
+            to = (v8h*)(buffer + kKeyBytes + ((wave + 4 * cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+        }
+    };
+
+    v4f o[QT][TILES];
+    Softmax m[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) o[i][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    load(begin, keys.key_block(begin), keys.value_block(begin));
+    store(begin);
+    load(begin + 1, keys.key_block(begin + 1), keys.value_block(begin + 1));
+    KeyScales scales = keys.scales(keys.value_block(begin));
+    int ik = keys.key_block(begin + 2), iv = keys.value_block(begin + 2), is = keys.value_block(begin + 1);
+    lds_barrier();
+    for (int step = begin; step < end; ++step) {
+        const uint8_t* buffer = lds + (step & 1) * kBuffer;
+        store(step + 1);
+        load(step + 2, ik, iv);
+        ik = keys.key_block(step + 3);
+        iv = keys.value_block(step + 3);
+        const KeyScales now = scales.checked();
+        const bool idle = step * kStep > high || (p.window && step * kStep + kStep <= low + 1 - p.window);
+        if (!idle) {
+            v4f acc[QT][4];
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            // (no product waits for the one before it)
+#pragma unroll
+            for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8h k[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) k[j] = *((const v8h*)(buffer + ((j * CC + cc) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], ql[i][cc][h], acc[i][j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], qh[i][cc][h], acc[i][j], 0, 0, 0);
+                }
+            v8h hi[QT][2], lo[QT][2];
+            const int at = step * kStep + 16 * lq;
+            const bool masked = step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window);
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                if (masked) {
+                    const int from = p.window ? position[i] + 1 - p.window - at : 0;
+                    weigh<true>(acc[i], c[i], now, m[i], o[i], tiles, from, position[i] + 1 - at, hi[i], lo[i]);
+                } else {
+                    weigh<false>(acc[i], c[i], now, m[i], o[i], tiles, 0, 16, hi[i], lo[i]);
+                }
+            }
+#pragma unroll
+            for (int t0 = 0; t0 < TILES; t0 += 4) {
+                if (!FULL && t0 >= tiles) continue;                // (tiles past the last: of zeros)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8h v[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) v[t] = *((const v8h*)(buffer + kKeyBytes + ((t0 + t) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], lo[i][h], o[i][t0 + t], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) o[i][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], hi[i][h], o[i][t0 + t], 0, 0, 0);
+                }
+            }
+        }
+        scales = keys.scales(is);
+        is = keys.value_block(step + 2);
+        lds_barrier();                                             // (the next loads stay in flight)
+    }
+
+    const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const float sum = add_xor32(add_xor16(m[i].sum));
+        const int row = w0 + 16 * i + li;
+        if (row >= rows) continue;
+        float* to = p.out + ((size_t)token[i] * p.heads + head[i]) * dim;
+        float scale = 1.0f / sum;
+        if (parts > 1) {
+            to = partial_values(p, share, slot) + (size_t)(row - r0) * dim;
+            scale = 1.0f;
+            if (lq == 0) partial_sums(p, share, slot)[row - r0] = v2f{m[i].base, sum};
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[i][t] * scale;
+    }
+}
+
+// ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
+// values of one part at a time
+__global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(AttentionKv8Call p, Share share) {
+    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
+    const int request = blockIdx.x, kvh = blockIdx.y;
+    const Kv8Request q = kv8_request(p.batch, request);
+    const int steps = line_steps(p, q, group, share);
+    if (!steps) return;
+    const long long* plan = line_plan(p, share);
+    const size_t kv_heads = p.cache.kv_heads;
+    const Line line{plan[0], (int)plan[1]};
+    const long long from = plan[2 + request] * (long long)kv_heads + (long long)kvh * steps;
+    const int group_from = line.group_of(from), parts = line.group_of(from + steps - 1) - group_from + 1;
+    if (parts == 1) return;
+    const size_t slot = (size_t)group_from + (size_t)request * kv_heads + kvh;
+    const size_t sum_stride = share.tile_rows, stride = sum_stride * dim;
+    // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
+    const int quads = dim / 4, abreast = 64 / quads, quad = lane % quads, own = lane / quads;
+    for (int row = threadIdx.x >> 6; row < q.rows * group; row += blockDim.x >> 6) {
+        const v2f* sums = partial_sums(p, share, slot) + row;
+        const float* values = partial_values(p, share, slot) + (size_t)row * dim;
+        float base = kNoBase, sum = 0.0f;
+        for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
+        base = wave_max_f32(base);
+        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (own < abreast) {
+#pragma unroll 4
+            for (int i = own; i < parts; i += abreast) {
+                const v2f s = sums[i * sum_stride];
+                const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
+                const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+                sum = fmaf(s.y, alpha, sum);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+            }
+        }
+        // the parts abreast together, in their order
+        v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float total = 0.0f;
+        for (int k = 0; k < abreast; ++k) {
+            total += __shfl(sum, k * quads + quad, 64);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
+        }
+        if (own == 0) {
+            const float scale = 1.0f / total;
+            *(v4f*)(p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim + 4 * quad) = all * scale;
+        }
+    }
+}
+
+// ---- the same of more rows: some workgroups a tile, a thread for four values of a row
+constexpr int kMergeSplit = 4;                      // workgroups of a tile
+__global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(AttentionKv8Call p, Share share) {
+    __shared__ int sums_of[kWaves], found[5];
+    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int kvh = blockIdx.x / kMergeSplit % p.cache.kv_heads, index = blockIdx.x / kMergeSplit / p.cache.kv_heads;
+    // tile `index` of the batch
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    int before = 0;
+    for (int base = 0; base < p.batch.requests; base += kThreads) {
+        const int r = base + threadIdx.x;
+        const Kv8Request mine = r < p.batch.requests ? kv8_request(p.batch, r) : Kv8Request{0, 0, 0};
+        const int tiles = tiles_of(mine, group, share);
+        int s = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(s, o, 64);
+            if (lane >= o) s += below;
+        }
+        if (lane == 63) sums_of[wave] = s;
+        __syncthreads();
+        int start = before + s - tiles;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) start += sums_of[w];
+            before += sums_of[w];
+        }
+        if (index >= start && index < start + tiles) {
+            found[0] = r;
+            found[1] = tiles - 1 - (index - start);
+            found[2] = mine.start;
+            found[3] = mine.rows;
+            found[4] = mine.length;
+        }
+        __syncthreads();
+        if (index < before) break;
+    }
+    if (found[0] < 0) return;
+    const int request = found[0], tile = found[1];
+    const Kv8Request q{found[2], found[3], found[4]};
+    const int* plan = (const int*)p.partial + share.at;
+    const int per = plan[0], first = plan[kHeader + request];
+    const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
+    const int parts = parts_of(seen.end - seen.begin, per);
+    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps(q, group, p.window, share.tile_rows), per);
+    if (parts == 1 || item < 0 || item > share.items - parts) return;
+    const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
+    const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+    const int r0 = tile * share.tile_rows, rows = min(share.tile_rows, q.rows * group - r0), quads = dim / 4;
+    for (int u = blockIdx.x % kMergeSplit * kThreads + threadIdx.x; u < rows * quads; u += kMergeSplit * kThreads) {
+        const int row = u / quads, quad = u % quads;
+        const v2f* sums = partial_sums(p, share, slot) + row;
+        const float* values = partial_values(p, share, slot) + (size_t)row * dim + 4 * quad;
+        float base = kNoBase, sum = 0.0f;
+        v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) base = fmaxf(base, sums[i * sum_stride].x);
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            const v2f s = sums[i * sum_stride];
+            const v4f v = *(const v4f*)(values + i * stride);
+            const float alpha = __builtin_amdgcn_exp2f(s.x - base);
+            sum = fmaf(s.y, alpha, sum);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+        }
+        const float scale = 1.0f / sum;
+        *(v4f*)(p.out + ((size_t)(q.start + (r0 + row) / group) * p.heads + kvh * group + (r0 + row) % group) * dim + 4 * quad) = x * scale;
+    }
+}
+
+// Workgroups that a batch's keys are cut for: those that the GPU holds at once.
+constexpr int few_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; }
+constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; }
+constexpr int row_tiles(int cc) { return 1; }
+constexpr int kManyTokens = 64;
+constexpr int kLeast = 4;                           // steps of a part at least
+
+// At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.
+int most_tiles(const AttentionKv8Call& call, const Share& share) {
+    const size_t group = call.heads / call.cache.kv_heads;
+    size_t tiles = std::min(call.batch.requests, call.batch.tokens);
+    if (share.tile_rows > kFewRows) tiles += (size_t)call.batch.tokens * group / share.tile_rows;
+    return (int)tiles;
+}
+int most_items(const AttentionKv8Call& call, const Share& share) {
+    const size_t kv = call.cache.kv_heads, tiles = most_tiles(call, share);
+    const size_t longest = ((size_t)call.batch.width * call.batch.block + kStep - 1) / kStep + 1;
+    return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
+}
+
+size_t partial_floats(const AttentionKv8Call& call, const Share& share) {
+    return plan_words(call.batch.requests) + share.slots * share.tile_rows * (call.cache.dim + 2);
+}
+
+// Which kernel takes which requests.  Where requests have kManyTokens new tokens on average the kernel of many rows
+// takes those of few too: the other's launch for the odd one is not worth it.
+struct Shares {
+    Share few, many;
+    size_t floats;
+};
+Shares shares_of(const AttentionKv8Call& call) {
+    const int group = call.heads / call.cache.kv_heads;
+    const bool only_many = group > kFewRows || call.batch.tokens / kManyTokens >= call.batch.requests;
+    const bool only_few = (size_t)call.batch.max_rows * group <= kFewRows;
+    const int cc = (call.cache.dim + 63) / 64, kv = call.cache.kv_heads;
+    Shares s{{kFewRows, few_target(cc), kLeast, 1, kFewRows, 0, 0, 0},
+             {16 * kWaves * row_tiles(cc), rows_target(cc), kLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0, 0}, 0};
+    if (only_few || !only_many) {
+        // workgroups of the line: each has least steps at least
+        const size_t longest = ((size_t)call.batch.width * call.batch.block + kStep - 1) / kStep + 1;
+        s.few.items = (int)std::min<size_t>(s.few.target, (longest * call.batch.requests * kv + kLeast - 1) / kLeast);
+        s.few.slots = s.few.items + (size_t)call.batch.requests * kv;
+        s.many.at = (partial_floats(call, s.few) + 3) / 4 * 4;
+        s.floats = s.many.at;
+    }
+    if (!only_few) {
+        s.many.items = most_items(call, s.many);
+        s.many.slots = (size_t)s.many.items * kv;
+        s.floats = s.many.at + partial_floats(call, s.many);
+    }
+    return s;
+}
+
+template <int CC, bool FULL, bool E4M3>
+void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
+    if (share.tile_rows == kFewRows) {
+        attention_kv8_few_kernel<CC, FULL, E4M3><<<share.items, kThreads, 0, stream>>>(call, share);
+        return;
+    }
+    const int grid = share.items * call.cache.kv_heads;
+    constexpr int kLds = 2 * 16 * CC * 1024;
+    constexpr auto kernel = attention_kv8_rows_kernel<CC, row_tiles(CC), FULL, E4M3>;
+    if (kLds >= 65536) {                            // more than the default, with the static arrays
+        static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        (void)allowed;
+    }
+    kernel<<<grid, kRowsThreads, kLds, stream>>>(call, share);
+}
+
+template <int CC, bool FULL>
+void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
+    if (call.cache.e4m3) launch<CC, FULL, true>(call, share, stream);
+    else launch<CC, FULL, false>(call, share, stream);
+}
+
+}  // namespace
+
+size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call) { return 4 * shares_of(call).floats; }
+
+void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
+    const int dim = call.cache.dim, group = call.heads / call.cache.kv_heads;
+    const Shares shares = shares_of(call);
+    for (const Share& share : {shares.few, shares.many}) {
+        if (!share.items) continue;
+        switch ((dim + 63) / 64 * 2 + (dim % 64 == 0)) {
+        case 2: launch<1, false>(call, share, stream); break;
+        case 3: launch<1, true>(call, share, stream); break;
+        case 4: launch<2, false>(call, share, stream); break;
+        case 5: launch<2, true>(call, share, stream); break;
+        case 6: launch<3, false>(call, share, stream); break;
+        case 7: launch<3, true>(call, share, stream); break;
+        case 8: launch<4, false>(call, share, stream); break;
+        default: launch<4, true>(call, share, stream); break;
+        }
+    }
+    if (shares.few.items > 1)
+        attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
+                                         64 * std::min(kFewRows, group * call.batch.max_rows), 0, stream>>>(call, shares.few);
+    const bool parted = ((size_t)call.batch.width << call.batch.block_shift) > (size_t)kLeast * kStep;
+    if (shares.many.items && parted)
+        attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
+            call, shares.many);
+}
+
+}  // namespace leafhip
