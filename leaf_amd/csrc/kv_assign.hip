@@ -27,24 +27,29 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kPerThread = 4;                       // requests a thread sums: LH_KV_MAX_REQUESTS <= 4 * 1024
 constexpr int kGroupTokens = 2048;                  // tokens a workgroup writes before a second one pays
+constexpr int kSmallRows = 4;
 
 // Exclusive prefix sums over the workgroup of each thread's value, and their total.
-__device__ __forceinline__ long long scan_block(long long v, long long* waves, long long& total) {
+template <typename T>
+__device__ __forceinline__ T scan_block(T v, long long* scratch, T& total) {
+    T* waves = (T*)scratch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    long long s = v;
+    T s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const long long below = __shfl_up(s, o, 64);
+        const T below = __shfl_up(s, o, 64);
         if (lane >= o) s += below;
     }
     __syncthreads();
     if (lane == 63) waves[wave] = s;
     __syncthreads();
-    long long before = 0;
+    T before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < kThreads / 64; ++w) {
-        if (w < wave) before += waves[w];
-        total += waves[w];
+        const T one = waves[w];
+        if (w < wave) before += one;
+        total += one;
     }
     return before + s - v;
 }
@@ -62,7 +67,9 @@ __device__ __forceinline__ int find_last(const int* values, int n, int what) {
 
 // DIRECT: the only workgroup, which writes the lengths and the free count too.
 // FINAL: the second launch of several, which writes only those.
-template <bool DIRECT, bool FINAL>
+// SMALL: no request has more than kSmallRows new tokens, so it needs one block at most, and the thread that sums a
+// request writes its tokens and its block too: no bisection, which is a dozen dependent reads.
+template <bool DIRECT, bool FINAL, bool SMALL>
 __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
     extern __shared__ int lds[];
     __shared__ long long waves[kThreads / 64];
@@ -75,7 +82,8 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
     const long long room = (long long)b.width << b.block_shift;
 
     int c[kPerThread], f[kPerThread], held[kPerThread];
-    long long mine_rows = 0, mine_given = 0;
+    long long mine_rows = 0;
+    int mine_given = 0;                             // (blocks: at most the table's entries, which an int counts)
     const int first = threadIdx.x * kPerThread;
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
@@ -86,13 +94,15 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
         mine_rows += max(f[j], 0);
         mine_given += f[j] < 0 ? held[j] : 0;
     }
-    long long all_rows, all_given, all_needed;
+    long long all_rows;
+    int all_given, all_needed;
     long long at_row = scan_block(mine_rows, waves, all_rows);
-    long long at_given = scan_block(mine_given, waves, all_given);
-    const int returned = (int)min(all_given, (long long)(b.blocks - count));
+    int at_given = scan_block(mine_given, waves, all_given);
+    const int returned = min(all_given, b.blocks - count);
     const int free_blocks = count + returned;
     int need[kPerThread];
-    long long mine_needed = 0, row = at_row;
+    int mine_needed = 0;
+    long long row = at_row;
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
         const long long after = (long long)c[j] + max(f[j], 0);
@@ -101,19 +111,22 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
         need[j] = fits ? (int)((after + b.block - 1) >> b.block_shift) - held[j] : -1;
         mine_needed += max(need[j], 0);
     }
-    long long at_needed = scan_block(mine_needed, waves, all_needed);
+    int at_needed = scan_block(mine_needed, waves, all_needed);
+    const int first_row = (int)min(at_row, (long long)b.tokens), first_needed = at_needed;
+    int takes_of = 0;                               // a bit for each of the thread's requests
     int used = 0;                                   // inclusive sum of the last request taken in
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
         const int r = first + j;
-        const long long upto = at_needed + max(need[j], 0);
+        const int upto = at_needed + max(need[j], 0);
         const bool takes = need[j] >= 0 && (need[j] == 0 || upto <= free_blocks);
-        if (takes && need[j] > 0) used = (int)upto;
+        if (takes && need[j] > 0) used = upto;
+        takes_of |= takes << j;
         if (r < n) {
             const int start = (int)min(at_row, (long long)b.tokens);
             starts[r] = start;
-            needed[r] = (int)min(at_needed, 0x7fffffffLL);
-            given[r] = (int)at_given;
+            needed[r] = at_needed;
+            given[r] = at_given;
             cached[r] = takes ? c[j] : -1;
             if (DIRECT || FINAL) {
                 b.starts[r] = start;
@@ -153,27 +166,65 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
 
     const long long thread = blockIdx.x * kThreads + threadIdx.x, threads = gridDim.x * kThreads;
     const int rows = (int)min(all_rows, (long long)b.tokens);
-    for (long long at = thread; at < b.tokens; at += threads) {
-        const int t = (int)at;
-        int position = -1, slot = -1;
-        if (t < rows) {
-            const int r = find_last(starts, n, t);
-            if (cached[r] >= 0) {
-                position = cached[r] + (t - starts[r]);
-                const int entry = position >> b.block_shift, held = held_of(r);
-                const int id = entry < held ? b.table[(size_t)r * b.width + entry] : taken_block(needed[r] + entry - held);
-                if ((unsigned)id < (unsigned)b.blocks) slot = (id << b.block_shift) + (position & (b.block - 1));
+    if (SMALL) {
+        int t = first_row, u = first_needed;
+        // (the blocks of all four requests first, then what depends on them)
+        int held_id[kPerThread], new_id[kPerThread];
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            const bool takes = takes_of >> j & 1;
+            const int before = (c[j] - 1) >> b.block_shift;        // the block of its last token
+            held_id[j] = takes && c[j] > 0 && f[j] > 0 ? b.table[(size_t)(first + j) * b.width + before] : -1;
+            new_id[j] = takes && need[j] > 0 ? taken_block(u) : -1;
+            u += max(need[j], 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            const bool takes = takes_of >> j & 1;
+            if (takes && need[j] > 0) b.table[(size_t)(first + j) * b.width + held[j]] = new_id[j];
+            for (int i = 0; i < f[j]; ++i, ++t) {
+                if (t >= b.tokens) break;
+                const int position = c[j] + i, id = position >> b.block_shift < held[j] ? held_id[j] : new_id[j];
+                const bool known = takes && (unsigned)id < (unsigned)b.blocks;
+                b.positions[t] = takes ? position : -1;
+                b.slots[t] = known ? (id << b.block_shift) + (position & (b.block - 1)) : -1;
             }
         }
-        b.positions[t] = position;
-        b.slots[t] = slot;
+        for (int t = rows + threadIdx.x; t < b.tokens; t += kThreads) b.positions[t] = b.slots[t] = -1;
+    } else {
+        for (long long at = thread; at < b.tokens; at += threads) {
+            const int t = (int)at;
+            int position = -1, slot = -1;
+            if (t < rows) {
+                const int r = find_last(starts, n, t);
+                if (cached[r] >= 0) {
+                    position = cached[r] + (t - starts[r]);
+                    const int entry = position >> b.block_shift, held = held_of(r);
+                    const int id = entry < held ? b.table[(size_t)r * b.width + entry] : taken_block(needed[r] + entry - held);
+                    if ((unsigned)id < (unsigned)b.blocks) slot = (id << b.block_shift) + (position & (b.block - 1));
+                }
+            }
+            b.positions[t] = position;
+            b.slots[t] = slot;
+        }
+        for (long long at = thread; at < used; at += threads) {
+            const int u = (int)at;
+            const int r = find_last(needed, n, u);
+            b.table[(size_t)r * b.width + held_of(r) + (u - needed[r])] = taken_block(u);
+        }
     }
-    for (long long at = thread; at < used; at += threads) {
-        const int u = (int)at;
-        const int r = find_last(needed, n, u);
-        b.table[(size_t)r * b.width + held_of(r) + (u - needed[r])] = taken_block(u);
+    // returned blocks: a wave looks at 64 requests and copies the rows of those that have ended
+    const int lane = threadIdx.x & 63;
+    for (int base = (int)(thread >> 6) * 64; base < n; base += (int)threads) {
+        const int r = base + lane, end = r + 1 < n ? given[r + 1] : all_given, blocks = r < n ? end - given[r] : 0;
+        for (uint64_t ended = __ballot(blocks > 0); ended; ended &= ended - 1) {
+            const int from = __builtin_ctzll(ended), first_block = given[base + from];
+            const int here = min(__shfl(blocks, from, 64), returned - first_block);
+            const int* row = b.table + (size_t)(base + from) * b.width;
+#pragma unroll 4
+            for (int j = lane; j < here; j += 64) b.free_blocks[count + first_block + j] = row[j];
+        }
     }
-    for (long long at = thread; at < returned; at += threads) b.free_blocks[count + at] = returned_block((int)at);
 }
 
 }  // namespace
@@ -181,12 +232,13 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(KvBatchView b) {
 void launch_kv_assign(const KvBatchView& b, hipStream_t stream) {
     const size_t lds = (size_t)4 * b.requests * sizeof(int);
     if (b.tokens <= kGroupTokens) {
-        kv_assign_kernel<true, false><<<1, kThreads, lds, stream>>>(b);
+        if (b.max_rows <= kSmallRows) kv_assign_kernel<true, false, true><<<1, kThreads, lds, stream>>>(b);
+        else kv_assign_kernel<true, false, false><<<1, kThreads, lds, stream>>>(b);
         return;
     }
     const int groups = std::min((b.tokens + kGroupTokens - 1) / kGroupTokens, 256);
-    kv_assign_kernel<false, false><<<groups, kThreads, lds, stream>>>(b);
-    kv_assign_kernel<false, true><<<1, kThreads, lds, stream>>>(b);
+    kv_assign_kernel<false, false, false><<<groups, kThreads, lds, stream>>>(b);
+    kv_assign_kernel<false, true, false><<<1, kThreads, lds, stream>>>(b);
 }
 
 }  // namespace leafhip
