@@ -333,11 +333,11 @@ lh_status lh_argmax(const float* logits, size_t rows, size_t width, uint32_t* ou
  * the last request's are padding and stay as they were. */
 typedef struct lh_kv_batch {
     uint32_t requests;      /* 1..LH_KV_MAX_REQUESTS */
-    uint32_t tokens;        /* rows of the step's arrays */
+    uint32_t tokens;        /* rows of the step's arrays; times the heads at most 2^27 where there are heads */
     uint32_t max_rows;      /* no request has more new tokens than this; a request that has is turned away */
     uint32_t block;         /* tokens a block holds: 16, 32, 64 or 128 */
     uint32_t blocks;        /* blocks of the pool */
-    uint32_t width;         /* table entries of a request */
+    uint32_t width;         /* table entries of a request: width * block is at most 2^30 */
     /* read by lh_kv_assign: */
     const int32_t* cached;      /* [requests] tokens a request has in the cache */
     const int32_t* fresh;       /* [requests] its new tokens; negative: it has ended, its blocks go back */
@@ -362,7 +362,7 @@ typedef struct lh_kv8 {
     void* values;           /* [blocks][kv_heads][dim][block] codes (a dim's tokens are consecutive), 16-byte aligned */
     float* key_scales;      /* [blocks][kv_heads] */
     float* value_scales;    /* [blocks][kv_heads] */
-    uint32_t kv_heads;      /* at most 1024 */
+    uint32_t kv_heads;      /* at most 256 */
     uint32_t dim;           /* a multiple of 16, at most 256 */
     uint32_t format;        /* LH_KV8_* */
 } lh_kv8;

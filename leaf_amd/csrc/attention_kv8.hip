@@ -25,6 +25,7 @@
 // dim's tokens together), and a lane's 16 keys lie in one block, with one scale.
 // Both K and V come as 16-byte loads; a key's dims are permuted alike in Q.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "kv8.h"
@@ -204,7 +205,7 @@ struct Softmax {
 template <bool MASKED, int TILES>
 __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int tiles, int from, int to,
                                       v8h (&hi)[2], v8h (&lo)[2]) {
-    const int exponent = min(max((int)(__float_as_uint(s.value) >> 23) - 127, -64), 64);
+    const int exponent = min(max((int)(__float_as_uint(s.value) >> 23) - 127, -64), 126);
     const float e = (float)exponent, down = __uint_as_float((uint32_t)(127 - exponent) << 23), f = s.value * down;
     c *= s.key;
     c = c < 1e-37f ? 1e-37f : c;                    // (a masked key is minus infinity times it)
@@ -262,7 +263,7 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
 struct Share {
     int tile_rows, target, least;                   // least: steps a part has at least
     int from, to;                                   // takes the requests of from..to rows of a KV head
-    int items;                                      // of a KV head, that there are workgroups and partial results for
+    int items, slots;                               // of a KV head, that there are workgroups, and partial results, for
     size_t at;                                      // where its partial results begin: in floats
 };
 __device__ __forceinline__ int tiles_of(const Kv8Request& q, int group, const Share& share) {
@@ -286,17 +287,17 @@ __device__ __forceinline__ int most_steps(const Kv8Request& q, int group, int wi
 __device__ __forceinline__ int parts_of(int steps, int per) { return (steps + per - 1) / per; }
 
 struct Item {
-    int request, tile, part, index;                 // index: of the tile's first part among the KV head's items
+    int request, tile, part, slot;                  // slot: of the tile's first part among the KV head's partial results
     Kv8Request q;
 };
 
 // Which part of which tile of which request is item `index` (of one KV head);
 // request -1: none.  Every workgroup sums the whole batch, a request a thread.
-// The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first item.
+// The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first slot.
 __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
     const KvBatchView& b = p.batch;
     const int window = p.window;
-    __shared__ int sums[kWaves];
+    __shared__ uint64_t sums[kWaves];
     __shared__ Item found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto steps = [&](const Kv8Request& q) {
@@ -317,37 +318,40 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all += totals[w];
     per = max(share.least, (int)fminf(all * (float)p.cache.kv_heads / (float)share.target * 1.0001f + 1.0f, 1e9f));
-    int before = 0;
+    // items, and of these the partial results (kept for tiles of several parts), before each request: two sums in one
+    uint64_t before = 0;
     for (int base = 0; base < b.requests; base += kThreads) {
         const int r = base + threadIdx.x;
         if (b.requests > kThreads) mine = r < b.requests ? kv8_request(b, r) : Kv8Request{0, 0, 0};
         const int tiles = tiles_of(mine, group, share), parts = parts_of(most_steps(mine, group, window, share.tile_rows), per);
-        const int items = tiles ? tiles * parts : 0;
-        int s = items;
+        // (what a batch's rows allow is far below the limits; requests that claim the same rows may not reach into the other sum)
+        const uint64_t items = tiles ? min((long long)tiles * parts, 1LL << 27) : 0;
+        const uint64_t own = items << 24 | (parts > 1 ? min((uint32_t)items, 4095u) : 0);
+        uint64_t s = own;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int below = __shfl_up(s, o, 64);
+            const uint64_t below = __shfl_up((unsigned long long)s, o, 64);
             if (lane >= o) s += below;
         }
         if (lane == 63) sums[wave] = s;
         __syncthreads();
-        int start = before + s - items, all_items = 0;
+        uint64_t start = before + s - own;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             if (w < wave) start += sums[w];
-            all_items += sums[w];
+            before += sums[w];
         }
-        if (index >= start && index < start + items) {
-            const int i = index - start;
+        const long long i = (long long)index - (long long)(start >> 24);
+        const int slot = (int)(start & 0xFFFFFF);
+        if (i >= 0 && i < (long long)items) {
             // the longest tiles (the last) first
-            found = Item{r, tiles - 1 - i / parts, i % parts, start + i / parts * parts, mine};
+            found = Item{r, tiles - 1 - (int)i / parts, (int)i % parts, slot + (int)i / parts * parts, mine};
         }
         // the first workgroup leaves the plan for the merge
-        if (blockIdx.x == 0 && r < b.requests) ((int*)p.partial)[share.at + kHeader + r] = start;
+        if (blockIdx.x == 0 && r < b.requests) ((int*)p.partial)[share.at + kHeader + r] = slot;
         if (blockIdx.x == 0 && r == 0) ((int*)p.partial)[share.at] = per;
-        before += all_items;
         __syncthreads();
-        if (index < before && blockIdx.x) break;
+        if ((long long)index < (long long)(before >> 24) && blockIdx.x) break;
     }
     return found;
 }
@@ -357,7 +361,7 @@ __device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, cons
     return p.partial + share.at + (kHeader + p.batch.requests + 3) / 4 * 4 + item * share.tile_rows * p.cache.dim;
 }
 __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Share& share, size_t item) {
-    return (v2f*)partial_values(p, share, (size_t)share.items * p.cache.kv_heads) + item * share.tile_rows;
+    return (v2f*)partial_values(p, share, (size_t)share.slots * p.cache.kv_heads) + item * share.tile_rows;
 }
 
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
     const int low = q.length - q.rows;                             // of the first row
     const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
-    if (item.part >= parts) return;
+    if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
@@ -485,7 +489,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
         sum = fmaf(sums[w][li], alpha[w], sum);
     }
     if (li >= rows) return;
-    const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+    const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
     float scale = 1.0f / sum;
     if (parts > 1) {
@@ -525,7 +529,7 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const int before = q.length - q.rows;                          // position of the first row
     const Steps seen = steps_of(q, group, p.window, kTileRows, item.tile);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
-    if (item.part >= parts) return;
+    if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
@@ -639,7 +643,7 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
     float scale = 1.0f / sum;
     if (parts > 1) {
-        const size_t slot = (size_t)(item.index + item.part) * kv_heads + kvh;
+        const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
         to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
         scale = 1.0f;
         if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = v2f{m.base, sum};
@@ -659,9 +663,8 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
     const int* plan = (const int*)p.partial + share.at;
     const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
     const int parts = parts_of(seen.end - seen.begin, plan[0]), item = plan[kHeader + request];
-    if (parts == 1) return;
-    // (requests that claim the same rows can have more parts than there are workgroups for: such rows stay undefined)
-    if (item < 0 || item > share.items - parts) return;
+    // (requests that claim the same rows can have more parts than there is room for: such rows stay undefined)
+    if (parts == 1 || item < 0 || item > share.slots - parts) return;
     const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
     const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
     // lanes: (part i0 + lane / quads, quad lane % quads) of rows of up to 64 quads
@@ -744,7 +747,7 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
     const int parts = parts_of(seen.end - seen.begin, per);
     const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps(q, group, p.window, share.tile_rows), per);
-    if (parts == 1 || item < 0 || item > share.items - parts) return;
+    if (parts == 1 || item < 0 || item > share.slots - parts) return;
     const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
     const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
     const int r0 = tile * share.tile_rows, rows = min(share.tile_rows, q.rows * group - r0), quads = dim / 4;
@@ -789,8 +792,13 @@ int most_items(const AttentionKv8Call& call, const Share& share) {
     return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
 }
 
+// Partial results: a tile of several parts has more steps than `per`, so at most twice its steps / per.
+int most_slots(const AttentionKv8Call& call, const Share& share) {
+    return std::min(share.items, 2 * ((share.target + call.cache.kv_heads - 1) / call.cache.kv_heads) + 1);
+}
+
 size_t partial_floats(const AttentionKv8Call& call, const Share& share) {
-    return (kHeader + call.batch.requests + 3) / 4 * 4 + (size_t)share.items * call.cache.kv_heads * share.tile_rows * (call.cache.dim + 2);
+    return (kHeader + call.batch.requests + 3) / 4 * 4 + (size_t)share.slots * call.cache.kv_heads * share.tile_rows * (call.cache.dim + 2);
 }
 
 // Which kernel takes which requests.  Where requests have kManyTokens new tokens on average the kernel of many rows
@@ -804,15 +812,17 @@ Shares shares_of(const AttentionKv8Call& call) {
     const bool only_many = group > kFewRows || call.batch.tokens / kManyTokens >= call.batch.requests;
     const bool only_few = (size_t)call.batch.max_rows * group <= kFewRows;
     const int cc = (call.cache.dim + 63) / 64;
-    Shares s{{kFewRows, few_target(cc), kFewLeast, 1, kFewRows, 0, 0},
-             {kTileRows, rows_target(cc), kRowsLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0}, 0};
+    Shares s{{kFewRows, few_target(cc), kFewLeast, 1, kFewRows, 0, 0, 0},
+             {kTileRows, rows_target(cc), kRowsLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0, 0}, 0};
     if (only_few || !only_many) {
         s.few.items = most_items(call, s.few);
+        s.few.slots = most_slots(call, s.few);
         s.many.at = (partial_floats(call, s.few) + 3) / 4 * 4;
         s.floats = s.many.at;
     }
     if (!only_few) {
         s.many.items = most_items(call, s.many);
+        s.many.slots = most_slots(call, s.many);
         s.floats = s.many.at + partial_floats(call, s.many);
     }
     return s;
@@ -827,10 +837,13 @@ void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream
     }
     constexpr int kLds = 2 * 16 * CC * 1024;
     constexpr auto kernel = attention_kv8_rows_kernel<CC, FULL, E4M3>;
-    if (kLds >= 65536) {                            // more than the default, with the static arrays
-        static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-        (void)allowed;
+    if (kLds >= 65536) {                            // more than the default, with the static arrays: allowed once a device
+        static std::atomic<uint64_t> allowed{0};
+        int device = 0;
+        (void)hipGetDevice(&device);
+        if (!(allowed >> (device & 63) & 1) &&
+            hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
+            allowed |= 1ull << (device & 63);
     }
     kernel<<<grid, kThreads, kLds, stream>>>(call, share);
 }
@@ -865,7 +878,7 @@ void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
     const size_t steps = ((size_t)call.batch.width << call.batch.block_shift) / kStep + 1;
     if (shares.few.items && steps > (size_t)kFewLeast)
         attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
-                                         64 * std::min(kFewRows, group * call.batch.max_rows), 0, stream>>>(call, shares.few);
+                                         64 * (int)std::min<int64_t>(kFewRows, (int64_t)group * call.batch.max_rows), 0, stream>>>(call, shares.few);
     if (shares.many.items && steps > (size_t)kRowsLeast)
         attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
             call, shares.many);

@@ -230,7 +230,8 @@ leafhip::KvBatchView view_of(const lh_kv_batch* b) {
     require_arg(b->block == 16 || b->block == 32 || b->block == 64 || b->block == 128,
                 "KV block must hold 16, 32, 64 or 128 tokens");
     require_arg(b->blocks >= 1 && uint64_t(b->blocks) * b->block <= 0x7fffffff, "KV pool has no blocks or too many");
-    require_arg(b->width >= 1 && uint64_t(b->requests) * b->width <= 0x7fffffff, "KV table is empty or too large");
+    require_arg(b->width >= 1 && uint64_t(b->requests) * b->width <= 0x7fffffff &&
+                    uint64_t(b->width) * b->block <= 1 << 30, "KV table is empty or too large");
     require_arg(b->tokens >= 1 && b->tokens <= 0x7fffffff && b->max_rows >= 1, "KV batch has no rows or too many");
     leafhip::KvBatchView v;
     v.requests = int(b->requests);
@@ -252,7 +253,7 @@ leafhip::Kv8View view_of(const lh_kv8* c, bool pointers = true) {
     require_arg(c != nullptr, "KV cache is null");
     require_arg(!pointers || (c->keys && c->values && c->key_scales && c->value_scales), "KV cache is empty");
     require_arg(aligned16(c->keys) && aligned16(c->values), "KV cache codes must be 16-byte aligned");
-    require_arg(c->kv_heads >= 1 && c->kv_heads <= 1024, "KV heads must be 1..1024");
+    require_arg(c->kv_heads >= 1 && c->kv_heads <= 256, "KV heads of an 8-bit cache must be 1..256");
     require_arg(c->dim >= 16 && c->dim <= 256 && c->dim % 16 == 0, "head dim of an 8-bit cache must be a multiple of 16 up to 256");
     require_arg(c->format == LH_KV8_INT8 || c->format == LH_KV8_E4M3, "unknown 8-bit KV format");
     leafhip::Kv8View v;
@@ -272,7 +273,7 @@ leafhip::AttentionKv8Call attention_kv8_call(const lh_kv_batch* batch, const lh_
     a.batch = view_of(batch);
     a.cache = view_of(cache, pointers);
     require_arg(heads >= 1 && heads <= 65535 && heads % cache->kv_heads == 0, "heads must be a multiple of the KV heads, at most 65535");
-    require_arg(uint64_t(batch->tokens) * heads <= 1 << 29, "too many rows of attention");
+    require_arg(uint64_t(batch->tokens) * heads <= 1 << 27, "too many rows of attention");
     a.heads = int(heads);
     return a;
 }
@@ -895,7 +896,7 @@ lh_status lh_rope_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float
         require_arg(rotary_dim <= cache->dim && rotary_dim % 2 == 0 && (!rotary_dim || (cosines && sines)), "invalid rotary dim");
         require_arg(table_positions >= 1 && table_positions <= 0x7fffffff, "RoPE tables are empty or too long");
         require_arg((uint64_t(heads) + 2 * uint64_t(cache->kv_heads)) * cache->dim <= 0x7fffffff &&
-                        uint64_t(batch->tokens) * heads <= 1 << 29, "too many heads");
+                        uint64_t(batch->tokens) * heads <= 1 << 27, "too many heads");
         require_arg(aligned16(qkv) && aligned16(q_heads) && aligned16(cosines) && aligned16(sines),
                     "rope arrays must be 16-byte aligned");
         r.qkv = qkv; r.cosines = cosines; r.sines = sines; r.heads = int(heads); r.rotary = int(rotary_dim);

@@ -350,6 +350,27 @@ def test_attention_of_many_requests(rt, requests):
     check_attention(rt, attention_case(rng, batch, 4, 1, 64, 16, ref.INT8), 16, ref.INT8, workspace="own")
 
 
+@pytest.mark.parametrize("requests,heads,kv", [([(900, 1)], 4, 2), ([(70, 3), (40, 1)], 4, 2), ([(300, 1), (64, 1), (2000, 1), (5, 1)], 20, 1),
+                                               ([(1 + i % 90, 1 + i % 7) for i in range(600)], 6, 1)])
+@pytest.mark.parametrize("padding", [0, 1000])
+def test_attention_in_tiles_of_few_rows(rt, requests, heads, kv, padding):
+    # the kernel of many rows with few of them: many padding rows, groups of more than 16, hundreds of requests
+    requests = [(max(n, r), r) for n, r in requests]
+    rng = np.random.default_rng(len(requests))
+    check_attention(rt, attention_case(rng, requests, heads, kv, 64, 16, ref.INT8, padding=padding), 16, ref.INT8, workspace="own")
+
+
+@pytest.mark.parametrize("batch", ["ragged", "mixed"])
+def test_attention_of_huge_values(rt, batch):
+    # value scales of 2^100, scores of ordinary size from tiny keys and large queries
+    rng = np.random.default_rng(8)
+    c = attention_case(rng, BATCHES[batch], 4, 2, 64, 16, ref.INT8)
+    c["value_scales"] *= np.float32(2.0 ** 100)
+    c["key_scales"] *= np.float32(2.0 ** -70)
+    c["q"] *= np.float32(2.0 ** 70)
+    check_attention(rt, c, 16, ref.INT8)
+
+
 @pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
 @pytest.mark.parametrize("batch", ["ragged", "mixed"])
 def test_attention_scales_far_apart(rt, form, batch):
@@ -602,3 +623,44 @@ def test_first_call_in_a_capture_needs_a_workspace(rt):
         assert np.array_equal(out.numpy(), want)
     graph.close()
     stream.close()
+
+
+def test_two_streams_and_two_graphs(rt):
+    # calls and graphs that may run at the same time: scratch of their streams, workspaces of their own
+    rng = np.random.default_rng(19)
+    cases = [attention_case(rng, b, 8, 2, 64, 32, ref.INT8) for b in ([(3000, 1)] * 6, [(2500, 1), (800, 1), (4000, 1)])]
+    want = [attend_on_gpu(rt, c, 32, ref.INT8) for c in cases]
+    streams, calls, outs, graphs, kept = [rt.Stream(), rt.Stream()], [], [], [], []
+    for c in cases:
+        heads, tokens, dim = c["q"].shape
+        d = {k: ints(rt, c[k]) for k in ("table", "lengths", "starts", "rows")}
+        data = [rt.DeviceArray.of(c[k]) for k in ("keys", "values", "key_scales", "value_scales")]
+        batch = rt.KvBatch(requests=len(c["rows"]), tokens=tokens, max_rows=1, block=32, blocks=len(c["keys"]), width=c["table"].shape[1],
+                           **{k: v.ptr for k, v in d.items()})
+        cache = rt.Kv8(*(a.ptr for a in data), 2, dim, ref.INT8)
+        q, out = rt.DeviceArray.of(c["q"]), rt.DeviceArray((tokens, heads, dim), np.float32)
+        workspace = rt.DeviceArray((rt.attention_kv8_workspace(batch, cache, heads),), np.uint8)
+        kept.append((d, data, q, workspace))
+        outs.append(out)
+        calls.append(lambda stream, workspace=None, a=(batch, cache, q, heads, out): rt.attention_kv8(*a, 0, workspace, stream))
+    for _ in range(3):
+        for out in outs:
+            out.zero()
+        rt.synchronize()
+        for _ in range(4):
+            for call, stream in zip(calls, streams):
+                call(stream.handle)
+        rt.synchronize()
+        assert all(np.array_equal(o.numpy(), w) for o, w in zip(outs, want))
+    for call, k in zip(calls, kept):
+        graphs.append(rt.Graph(streams[0], lambda: call(streams[0].handle, k[3])))
+    for _ in range(3):
+        for out in outs:
+            out.zero()
+        rt.synchronize()
+        for graph, stream in zip(graphs, streams):
+            rt.check(rt.library().lh_graph_launch(graph.handle, stream.handle))
+        rt.synchronize()
+        assert all(np.array_equal(o.numpy(), w) for o, w in zip(outs, want))
+    for g in graphs + streams:
+        g.close()

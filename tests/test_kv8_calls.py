@@ -36,9 +36,9 @@ def refused(fake_hip, calls):
         assert code == 1 and message.startswith("Leaf decoder: ") and launched == 0, (call, code, message)
 
 
-BATCHES = ["requests=0", "requests=4001", "tokens=0", "tokens=2**31", "max_rows=0", "block=0", "block=8", "block=48",
+BATCHES = ["width=2**20, block=128, blocks=4, requests=1, tokens=2**31", "width=2**24, block=128, blocks=4, requests=1", "requests=0", "requests=4001", "tokens=0", "tokens=2**31", "max_rows=0", "block=0", "block=8", "block=48",
            "block=256", "blocks=0", "blocks=2**28", "width=0", "width=2**31"]
-CACHES = ["kv_heads=0", "kv_heads=65536", "dim=0", "dim=8", "dim=72", "dim=272", "format=2", "keys=None", "values=None",
+CACHES = ["kv_heads=0", "kv_heads=257", "kv_heads=65536", "dim=0", "dim=8", "dim=72", "dim=272", "format=2", "keys=None", "values=None",
           "key_scales=None", "value_scales=None", "keys=buffer.ptr + 8", "values=buffer.ptr + 4"]
 
 
@@ -54,7 +54,7 @@ def test_refused_arguments(fake_hip):  # noqa: F811
             [f"attend(batch({n}=None))" for n in ("table", "lengths", "starts", "rows")] +
             [f"rope(batch({n}=None), cos=1, sin=1)" for n in ("positions", "slots")] +
             ["attend(heads=0)", "attend(heads=3)", "attend(q=4)", "attend(out=8)", "attend(q=-buffer.ptr)", "attend(out=-buffer.ptr)",
-             "attend(batch(tokens=2**20), heads=4096)", "attend(workspace=buffer.ptr + 8, bytes=1 << 20)",
+             "attend(batch(tokens=2**20), heads=4096)", "attend(batch(tokens=2**20), heads=130)", "rope(batch(tokens=2**20), heads=130, cos=1, sin=1)", "attend(workspace=buffer.ptr + 8, bytes=1 << 20)",
              "rope(heads=0, cos=1, sin=1)", "rope(heads=5, cos=1, sin=1)", "rope(cos=1)", "rope(sin=1)", "rope(rotary=3, cos=1, sin=1)",
              "rope(rotary=66, cos=1, sin=1)", "rope(positions=0, cos=1, sin=1)", "rope(positions=2**31, cos=1, sin=1)",
              "rope(qkv=4, cos=1, sin=1)", "rope(q=4, cos=1, sin=1)", "rope(cos=5, sin=1)", "rope(cos=1, sin=9)",
@@ -67,6 +67,47 @@ result = [assign(batch()), rope(cos=1, sin=1), rope(rotary=0), attend(), attend(
           assign(batch(requests=4000, tokens=2**31 - 1)), attend(batch(requests=4000, tokens=2**20))]
 ''')
     assert all(code == 0 and launched >= 1 for code, _, launched in results), results
+
+
+@pytest.mark.parametrize("sizes,heads,kernels", [
+    ("requests=64, tokens=64, max_rows=1, width=64", 4, ["few_kernel", "few_merge"]),          # a decode step
+    ("requests=64, tokens=64, max_rows=1, width=8", 4, ["few_kernel"]),                        # too short to be parted
+    ("requests=1, tokens=300, max_rows=300, width=64", 4, ["rows_kernel", "rows_merge"]),      # a prompt
+    ("requests=1, tokens=300, max_rows=300, width=20", 4, ["rows_kernel"]),
+    ("requests=30, tokens=300, max_rows=200, width=64", 4, ["few_kernel", "rows_kernel", "few_merge", "rows_merge"]),
+    ("requests=5, tokens=20, max_rows=8, width=64", 4, ["few_kernel", "few_merge"]),           # 16 rows of a KV head
+    ("requests=5, tokens=20, max_rows=9, width=64", 4, ["few_kernel", "rows_kernel", "few_merge", "rows_merge"]),
+    ("requests=64, tokens=64, max_rows=1, width=64", 34, ["rows_kernel", "rows_merge"])])      # groups of 17
+def test_attention_routes(fake_hip, sizes, heads, kernels):  # noqa: F811
+    launched = fake_hip(CALLS + f"""
+code = lib.lh_attention_kv8(C.byref(batch({sizes})), C.byref(cache()), buffer.ptr, {heads}, 0, buffer.ptr, None, 0, None)
+result = [code, kernels()]
+""")
+    assert launched[0] == 0 and len(launched[1]) == len(kernels)
+    assert all(f"attention_kv8_{name}" in k for name, k in zip(kernels, launched[1])), launched
+
+
+def test_assign_routes(fake_hip):  # noqa: F811
+    small, large, many = fake_hip(CALLS + """
+result = []
+for changed in (dict(max_rows=4), dict(max_rows=5), dict(tokens=2049, max_rows=1)):
+    assert lib.lh_kv_assign(C.byref(batch(**changed)), None) == 0
+    result.append(kernels())
+""")
+    assert [len(k) for k in (small, large, many)] == [1, 1, 2]
+    assert "ILb1ELb0ELb1E" in small[0] and "ILb1ELb0ELb0E" in large[0] and "ILb0ELb1ELb0E" in many[1]
+
+
+def test_workspace_does_not_depend_on_lengths(fake_hip):  # noqa: F811
+    # a decode step's parts are bounded by the GPU's size, not by the table's width
+    sizes, error = fake_hip(CALLS + """
+n, result = C.c_size_t(), []
+for width in (64, 4096, 2**20):
+    assert lib.lh_attention_kv8_workspace(C.byref(batch(requests=64, tokens=64, max_rows=1, width=width)), C.byref(cache(keys=None, values=None)), 8, C.byref(n)) == 0
+    result.append(n.value)
+result = [result, lib.lh_attention_kv8_workspace(C.byref(batch()), C.byref(cache()), 8, None)]
+""")
+    assert sizes[1] == sizes[2] <= 16 << 20 and sizes[0] <= sizes[1] and error == 1
 
 
 # ---- the plain forms themselves
