@@ -776,7 +776,7 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
 // Workgroups that a batch's keys are cut for: those that the GPU holds at once.
 constexpr int few_target(int cc) { return cc <= 2 ? 512 : 256; }
 constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; }
-constexpr int kManyTokens = 64;
+constexpr int kManyTokens = 6;
 constexpr int kFewLeast = 4, kRowsLeast = 8;        // steps of a part at least
 
 // At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.

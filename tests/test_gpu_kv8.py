@@ -360,6 +360,16 @@ def test_attention_in_tiles_of_few_rows(rt, requests, heads, kv, padding):
     check_attention(rt, attention_case(rng, requests, heads, kv, 64, 16, ref.INT8, padding=padding), 16, ref.INT8, workspace="own")
 
 
+@pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("heads,kv,dim,block", [(8, 2, 64, 16), (4, 1, 128, 64), (6, 2, 80, 32)])
+def test_attention_decoding_beside_a_prompt(rt, form, window, heads, kv, dim, block):
+    # both kernels in one call
+    rng = np.random.default_rng(dim)
+    batch = [(int(rng.integers(1, 700)), 1) for _ in range(30)] + [(170, 60), (2500, 1), (61, 3)]
+    check_attention(rt, attention_case(rng, batch, heads, kv, dim, block, form, padding=5), block, form, window)
+
+
 @pytest.mark.parametrize("batch", ["ragged", "mixed"])
 def test_attention_of_huge_values(rt, batch):
     # value scales of 2^100, scores of ordinary size from tiny keys and large queries

@@ -74,7 +74,8 @@ result = [assign(batch()), rope(cos=1, sin=1), rope(rotary=0), attend(), attend(
     ("requests=64, tokens=64, max_rows=1, width=8", 4, ["few_kernel"]),                        # too short to be parted
     ("requests=1, tokens=300, max_rows=300, width=64", 4, ["rows_kernel", "rows_merge"]),      # a prompt
     ("requests=1, tokens=300, max_rows=300, width=20", 4, ["rows_kernel"]),
-    ("requests=30, tokens=300, max_rows=200, width=64", 4, ["few_kernel", "rows_kernel", "few_merge", "rows_merge"]),
+    ("requests=51, tokens=300, max_rows=200, width=64", 4, ["few_kernel", "rows_kernel", "few_merge", "rows_merge"]),
+    ("requests=50, tokens=300, max_rows=200, width=64", 4, ["rows_kernel", "rows_merge"]),     # six new tokens a request
     ("requests=5, tokens=20, max_rows=8, width=64", 4, ["few_kernel", "few_merge"]),           # 16 rows of a KV head
     ("requests=5, tokens=20, max_rows=9, width=64", 4, ["few_kernel", "rows_kernel", "few_merge", "rows_merge"]),
     ("requests=64, tokens=64, max_rows=1, width=64", 34, ["rows_kernel", "rows_merge"])])      # groups of 17
