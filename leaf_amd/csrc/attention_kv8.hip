@@ -24,6 +24,13 @@
 // leaving its registers, V's lanes read 16 codes of one dim (the cache keeps a
 // dim's tokens together), and a lane's 16 keys lie in one block, with one scale.
 // Both K and V come as 16-byte loads; a key's dims are permuted alike in Q.
+//
+// Two kernels: requests of at most 16 rows of a KV head (attention_kv8_few_kernel)
+// read the cache straight into registers, others (attention_kv8_rows_kernel)
+// share what they widen through LDS.  The keys of a tile of rows are cut into
+// parts where a batch has too few tiles for the GPU, and a second launch joins
+// the parts.  Lengths are known on the device only: every workgroup sums the
+// batch and finds its own part (1 to 2 us, of the 7 that the smallest call takes).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -365,6 +372,12 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 }
 
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
+// 64 requests of 200 to 4096 tokens, 32 heads of 128 over 8: 69 us and 5 for the
+// join, 281 MB at 4.1 TB/s (without any arithmetic 65 in all: what bounds it is the
+// latency of its parts, some eight steps a wave behind 8 us of finding the part, the
+// query, the first table entries and the first codes).  8 requests of 16000 tokens
+// take 57 us, 4.6 TB/s.  Vector instructions issue for 39% of a busy CU's time, 320 of
+// 680 a step of 64 keys widening codes (INT8, heads of 128).
 template <int CC, bool FULL, bool E4M3>
 __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
@@ -510,6 +523,13 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 }
 
 // ---- more rows of a KV head: tiles of 64, 16 for a wave, K and V widened once for all of them through LDS
+// 512 tokens behind 7001 keys, 32 heads of 128 over 8 (E4M3): 131 us and 10 for the
+// join; 2048 tokens of 14 heads of 64 over 2 (INT8): 39 and 7.  What bounds it is issue:
+// vector instructions take 42% of a busy CU's cycles (a score's softmax and splitting
+// about ten, the widening of a step 80) and MFMAs 41%, and they hardly overlap.  Two row tiles
+// a wave (54 us for the prompt, 138 for the chunk, with spills), three or four waves a
+// SIMD in fewer registers (47 and 169), and eight waves in two groups half a step apart, one
+// in its products while the other is in its softmax (62 and 143), gave nothing.
 constexpr int kTileRows = 16 * kWaves;
 
 template <int CC, bool FULL, bool E4M3>
@@ -703,7 +723,7 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
 }
 
 // ---- the same of more rows: some workgroups a tile, a thread for four values of a row
-constexpr int kMergeSplit = 4;                      // workgroups of a tile
+constexpr int kMergeSplit = 4;                      // workgroups of a tile (2 / 4 / 8: a chunk beside decoding requests 45 / 44 / 48 us)
 __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(AttentionKv8Call p, Share share) {
     __shared__ int sums_of[kWaves], found[5];
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -773,11 +793,19 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     }
 }
 
-// Workgroups that a batch's keys are cut for: those that the GPU holds at once.
+// Workgroups that a batch's keys are cut for, about those that the GPU holds at once: more are more partial results and
+// more starts, fewer leave CUs idle.  Of few rows, with 512 / 768 / 1024: heads of 64, 100 requests 23 / 26 / 27 us, heads
+// of 128, 64 ragged requests 73 / 68 / 74 and 8 long ones 57 / 67 / 62; of many rows, heads of 64, a prompt of 2048
+// tokens 54 / 46 / 47, heads of 128, a chunk of 512 138 / 152 / 150.
 constexpr int few_target(int cc) { return cc <= 2 ? 512 : 256; }
 constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; }
+// Steps of a part at least, with 4 / 8: one request of 4095 tokens 10.9 / 12.5 us (a part's wave has one or two steps);
+// eight prompts of 300 tokens 37 / 27 (none is parted with 8; 16 costs a chunk beside decoding requests 47 for 44).
+constexpr int kFewLeast = 4, kRowsLeast = 8;
+// New tokens of a request, on average, from which the kernel of many rows takes every request: one launch in place of
+// two, one after the other, although it has a request of one token in a tile of 64.  At 13 a request it takes 75 us for 73
+// (heads of 128) and at 8 30 for 40 (heads of 64), at 3.5 203 for 151 and 39 for 45.
 constexpr int kManyTokens = 6;
-constexpr int kFewLeast = 4, kRowsLeast = 8;        // steps of a part at least
 
 // At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.
 int most_tiles(const AttentionKv8Call& call, const Share& share) {
@@ -801,8 +829,7 @@ size_t partial_floats(const AttentionKv8Call& call, const Share& share) {
     return (kHeader + call.batch.requests + 3) / 4 * 4 + (size_t)share.slots * call.cache.kv_heads * share.tile_rows * (call.cache.dim + 2);
 }
 
-// Which kernel takes which requests.  Where requests have kManyTokens new tokens on average the kernel of many rows
-// takes those of few too: the other's launch for the odd one is not worth it.
+// Which kernel takes which requests, and where in the workspace.
 struct Shares {
     Share few, many;
     size_t floats;

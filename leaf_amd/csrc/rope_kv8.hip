@@ -7,6 +7,18 @@
 // magnitude gives the scale; a scale that grows moves the codes of the block's
 // earlier tokens.  Where a skipped token parts a block's tokens, they are
 // several runs, one after the other.
+//
+// Keys are stored row by row, values with a dim's tokens together, as attention
+// reads them.  A thread takes four dims of four slots: a word of four codes for
+// each, stored along the dims for keys and along the slots for values.
+//
+// What bounds it: the latency of dependent loads (slots and positions, the rows
+// beside them, the values, their scale, and, past one group of slots a thread,
+// the values again), some 8 us behind the launch, and cold code: with loops unrolled
+// over 16 slots, 100 KB of it, the same calls took two to three times as long.  64 single tokens of
+// 32 heads of 64 over 4 take 7.5 us, 2048 tokens of 14 heads over 2 15 (18 MB, of which
+// the queries 14.7), a chunk of 500 beside 47 single tokens, 32 heads of 128 over 8, 21;
+// 4096 tokens of those 73 (235 MB at 3.2 TB/s, 46 of them the queries').
 #include <algorithm>
 
 #include "kv8.h"
@@ -80,7 +92,9 @@ __device__ __forceinline__ v4f rotated4(const float* row, int d, const float* c,
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kGroup = 4;                           // slots of a unit, by four dims: what a thread takes at a time
-constexpr int kWaveUnits = 128;                     // (groups of slots by quads of dims) that one wave takes at most of a block
+// Groups of slots by quads of dims of a block that one wave takes; more are the workgroup's.  With 32 / 128 / 512: 64 tokens
+// in a block of 64 (heads of 64) 8.9 / 11.5 / 15.2 us, 4096 tokens in blocks of 16 (heads of 128) 67 / 56 / 42, of 64 39 / 39 / 123.
+constexpr int kWaveUnits = 128;
 
 // A token that is the first of its block in this step.
 struct Leader {
@@ -350,7 +364,9 @@ __global__ __launch_bounds__(kThreads, 4) void rope_kv8_kernel(RopeKv8Call p, La
     }
 }
 
-constexpr int kMostGroups = 512;                    // of the cache's, before a wave looks at several tokens
+// Workgroups for the cache's part before a wave looks at several tokens (up to eight), about those that the GPU holds at once.
+// With 256 / 512 / 1024: 2048 tokens of 2 heads of 64 22 / 13 / 18 us, a chunk of 500 beside 47 single tokens 35 / 21 / 21.
+constexpr int kMostGroups = 512;
 
 }  // namespace
 
