@@ -30,7 +30,7 @@
 // share what they widen through LDS.  The keys of a tile of rows are cut into
 // parts where a batch has too few tiles for the GPU, and a second launch joins
 // the parts.  Lengths are known on the device only: every workgroup sums the
-// batch and finds its own part (1 to 2 us, of the 7 that the smallest call takes).
+// batch and finds its own part (dependent loads, part of the 7 us that the smallest call takes).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -373,9 +373,10 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
 // 64 requests of 200 to 4096 tokens, 32 heads of 128 over 8: 69 us and 5 for the
-// join, 281 MB at 4.1 TB/s (without any arithmetic 65 in all: what bounds it is the
-// latency of its parts, some eight steps a wave behind 8 us of finding the part, the
-// query, the first table entries and the first codes).  8 requests of 16000 tokens
+// join, 281 MB at 4.1 TB/s.  What bounds it is latency: without its arithmetic an
+// earlier state took 65 of 77 us in all.  A part is some eight steps a wave behind four
+// dependent loads (its place, the query, the first table entries, the first codes); that
+// these starts are what is left is not shown.  8 requests of 16000 tokens
 // take 57 us, 4.6 TB/s.  Vector instructions issue for 39% of a busy CU's time, 320 of
 // 680 a step of 64 keys widening codes (INT8, heads of 128).
 template <int CC, bool FULL, bool E4M3>
@@ -523,10 +524,11 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 }
 
 // ---- more rows of a KV head: tiles of 64, 16 for a wave, K and V widened once for all of them through LDS
-// 512 tokens behind 7001 keys, 32 heads of 128 over 8 (E4M3): 131 us and 10 for the
-// join; 2048 tokens of 14 heads of 64 over 2 (INT8): 39 and 7.  What bounds it is issue:
-// vector instructions take 42% of a busy CU's cycles (a score's softmax and splitting
-// about ten, the widening of a step 80) and MFMAs 41%, and they hardly overlap.  Two row tiles
+// 512 tokens behind 7001 keys, 32 heads of 128 over 8 (E4M3): 141 to 147 us, about
+// 10 of them the join's; 2048 tokens of 14 heads of 64 over 2 (INT8): 44 to 46, 7 the join's.
+// What bounds it is issue: other vector instructions (257 a step of 16 scores a lane, some 80
+// of them widening codes) take 42% of the chunk's busy cycles and MFMAs 41%, of the
+// prompt's 57% and 22%.  Two row tiles
 // a wave (54 us for the prompt, 138 for the chunk, with spills), three or four waves a
 // SIMD in fewer registers (47 and 169), and eight waves in two groups half a step apart, one
 // in its products while the other is in its softmax (62 and 143), gave nothing.

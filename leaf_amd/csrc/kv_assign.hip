@@ -17,7 +17,7 @@
 // written by the only workgroup, or by a second launch.
 //
 // What bounds it: the latency of a launch (5 us) and of some dependent loads and
-// sums: 24 requests of one token take 6.5 us, 2000 9, 1000 of which 50 return 6,250 blocks
+// sums: 24 requests of one token take 6.5 us, 2000 9, 1000 of which 50 return some 6,250 blocks
 // 13, 40 prompts of 15,600 tokens together 7.7 and 5 for the second launch.
 #include <algorithm>
 

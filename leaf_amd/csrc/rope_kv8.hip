@@ -14,10 +14,10 @@
 //
 // What bounds it: the latency of dependent loads (slots and positions, the rows
 // beside them, the values, their scale, and, past one group of slots a thread,
-// the values again), some 8 us behind the launch, and cold code: with loops unrolled
+// the values again) and cold code: with loops unrolled
 // over 16 slots, 100 KB of it, the same calls took two to three times as long.  64 single tokens of
-// 32 heads of 64 over 4 take 7.5 us, 2048 tokens of 14 heads over 2 15 (18 MB, of which
-// the queries 14.7), a chunk of 500 beside 47 single tokens, 32 heads of 128 over 8, 21;
+// 32 heads of 64 over 4 take 7.7 us, 2048 tokens of 14 heads over 2 15.6 (18 MB, of which
+// the queries 14.7), a chunk of 500 beside 47 single tokens, 32 heads of 128 over 8, 22;
 // 4096 tokens of those 73 (235 MB at 3.2 TB/s, 46 of them the queries').
 #include <algorithm>
 
