@@ -56,7 +56,7 @@ struct BlockBits {
     __device__ __forceinline__ int run(int i) const {
         const uint64_t gaps = ~from(i);
         if (gaps) return __builtin_ctzll(gaps);
-        const uint64_t later = i ? 0 : high;             // (64 from i > 0 on are the last)
+        const uint64_t later = i < 64 ? high >> i : 0;   // those from i + 64 on
         return 64 + (~later ? __builtin_ctzll(~later) : 64);
     }
     // The first set bit from i on; 128 where there is none.

@@ -187,6 +187,16 @@ def test_append(rt, form, runs, heads, kv, dim, rotary, block):
 
 
 @pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
+def test_append_more_than_64_behind_a_start(rt, form):
+    # blocks of 128 that take 64 tokens and more from a slot inside them, the largest value last: one run, one rounding
+    rng = np.random.default_rng(11)
+    runs = [(1, 127), (37, 91), (63, 65), (64, 64), (5, 64)]
+    case = append_case(rng, runs, 4, 2, 64, 64, 128, form)
+    case[6][np.cumsum([n for _, n in runs]) - 1] *= np.float32(37.0)
+    check_append(rt, case, 4, 64, 128, form)
+
+
+@pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
 def test_append_extremes(rt, form):
     # zeros, tiny and huge values beside each other; a scale that doubles makes ties of odd codes
     rng = np.random.default_rng(3)
