@@ -406,11 +406,13 @@ class BlockPool:
 
     ``step`` takes each request's new tokens (negative: it has ended) to the device and assigns their blocks;
     ``batch`` is what ``rope_kv8`` and ``attention_kv8`` take then.  Lengths and free blocks are kept on the device.
+    A step waits on the host for what its stream has to do already, which may still read the last step's new tokens; a
+    step that is captured writes ``fresh`` itself and calls ``kv_assign``.
     """
 
     def __init__(self, requests: int, tokens: int, block: int, blocks: int, width: int, max_rows: int = 0):
-        def ints(*shape):
-            return DeviceArray(shape, np.int32).zero()
+        def ints(*shape):                           # (copied: no stream's call may run before a fill that is not waited for)
+            return DeviceArray.of(np.zeros(shape, np.int32))
         self.fresh, self.lengths, self.rows = ints(requests), ints(requests), ints(requests)
         self.starts, self.positions, self.slots = ints(requests + 1), ints(tokens), ints(tokens)
         self.table = DeviceArray.of(np.full((requests, width), -1, np.int32))
@@ -424,6 +426,8 @@ class BlockPool:
         fresh = np.ascontiguousarray(fresh, np.int32)
         if fresh.shape != self.fresh.shape:
             raise ValueError(f"new tokens of {self.fresh.shape[0]} requests are needed, got {fresh.shape}")
+        if stream is not None:                      # the library's streams do not order the copy behind their work
+            check(library().lh_stream_synchronize(stream))
         check(library().lh_copy_to_device(self.fresh.ptr, _ptr(fresh), fresh.nbytes))
         kv_assign(self.batch, stream)
 

@@ -684,3 +684,25 @@ def test_two_streams_and_two_graphs(rt):
         assert all(np.array_equal(o.numpy(), w) for o, w in zip(outs, want))
     for g in graphs + streams:
         g.close()
+
+
+@pytest.mark.parametrize("on_stream", [False, True])
+def test_pool_steps_without_waits(rt, on_stream):
+    # each step's new tokens are the ones given with it, on the default stream and on one of the library's
+    requests, tokens, block, blocks, width = 5, 120, 16, 40, 9
+    pool, stream = rt.BlockPool(requests, tokens, block, blocks, width), rt.Stream() if on_stream else None
+    rng = np.random.default_rng(20)
+    want = {"table": np.full((requests, width), -1), "free_blocks": np.arange(blocks)[::-1].copy(), "free_left": blocks,
+            "lengths": np.zeros(requests, np.int64)}
+    for i in range(20):
+        fresh = rng.integers(0, 24, requests)
+        if i % 3 == 2:
+            fresh[i % requests] = -1
+        pool.step(fresh, stream.handle if on_stream else None)
+        want = ref.assign(want["lengths"], fresh, want["table"], want["free_blocks"], int(np.ravel(want["free_left"])[0]), block, width,
+                          blocks, tokens, tokens)
+    rt.synchronize()
+    for name in ("lengths", "rows", "starts", "positions", "slots", "table"):
+        assert np.array_equal(getattr(pool, name).numpy(), want[name]), name
+    if on_stream:
+        stream.close()

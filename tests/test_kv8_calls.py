@@ -156,3 +156,25 @@ def test_attention_form_sees_a_planted_mistake(form):
     for o, scales in zip(out, (ks, ks[[1, 0, 2]])):
         ref.attention(q, keys, values, scales, vs, table, [40], [0, 1], [1], 16, form, 0, o)
     assert np.abs(out[0] - out[1]).max() > 1e-2
+
+
+def test_pool_waits_for_its_stream(fake_hip):
+    # a step's new tokens are not overwritten before the last step's kernels have read them; none fills on another stream
+    assert fake_hip("""
+calls = []
+class Spy:
+    def __getattr__(self, name):
+        if name.startswith("lh_") and name not in ("lh_device_alloc", "lh_device_free"): calls.append(name)
+        return getattr(lib, name)
+spy = Spy()
+rt.library = lambda: spy
+pool, stream = rt.BlockPool(3, 8, 16, 10, 4), rt.Stream()
+made = sorted(set(calls))
+del calls[:]
+pool.step([1, 1, 1], stream.handle)
+on_stream = calls[:]
+del calls[:]
+pool.step([1, -1, 1])
+result = [made, on_stream, calls[:]]
+""") == [["lh_copy_to_device", "lh_stream_create"], ["lh_stream_synchronize", "lh_copy_to_device", "lh_kv_assign"],
+        ["lh_copy_to_device", "lh_kv_assign"]]
