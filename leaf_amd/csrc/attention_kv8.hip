@@ -9,13 +9,14 @@
 // would need three).
 //
 // Scales.  The score of a key is (q . code) c with c = query scale * key scale *
-// log2(e) / sqrt(dim).  A value's scale is 2^e f with 1 <= f < 2: weights are
-// formed as t = 2^(score + e - b + 8), relative to the largest weight times value
-// scale rather than the largest weight, so that w = t f, which is what meets the
-// value codes, keeps its 22 bits wherever it counts however far the scales of
-// blocks are apart, and the sum of weights adds t 2^-e.  b is a whole number per
-// row, at most 6 below the largest score + e so far (w < 2^15), so most steps
-// rescale nothing and a rescale is exact.
+// log2(e) / sqrt(dim); its weight is u = 2^(score - a + 8).  What meets the value
+// codes is w = u v 2^(a - b) of a value scale v = 2^e f, 1 <= f < 2: relative to the
+// largest weight times value scale, so that it keeps its 22 bits wherever it counts
+// however far the scales of blocks are apart, while the sum is of u, in which a key
+// counts whatever its value's scale is.  a and b are whole numbers per row, at most 6
+// below the largest score and the largest score + e so far (u < 2^14, w < 2^15), so
+// most steps rescale nothing and a rescale is exact.  A row's output is its sum of
+// w times codes, times 2^(b - a), over its sum of u.
 //
 // Layout.  A step is 64 keys.  S^T = K Q^T by v_mfma_f32_16x16x32_f16 with lane
 // l = 16 lq + li: row li of its tile j of keys is key 16 (li / 4) + 4 j + li % 4
@@ -50,6 +51,7 @@ constexpr int kFewRows = 16;                        // rows of a KV head in one 
 constexpr int kHeader = 4;                          // integers before a plan's requests
 constexpr float kNoBase = -1e30f;
 constexpr float kSlack = 6.0f, kLift = 8.0f;
+constexpr float kJoinDrop = 11.0f;                  // a tile has fewer than 2^11 parts: see most_slots
 
 // 16 codes as two operands.
 template <bool E4M3>
@@ -202,18 +204,26 @@ __device__ __forceinline__ v4u first_codes(v4u codes, int keys) {
     return codes;
 }
 
-// A row's online softmax: its base and its sum (this lane's keys).
+// A row's online softmax: the bases of its weights and of its outputs (a and b above), and its sum (this lane's keys).
 struct Softmax {
-    float base = kNoBase, sum = 0.0f;
+    float base = kNoBase, out = kNoBase, sum = 0.0f;
 };
 
+// What a row's outputs are multiplied by.  A row that sees no key of a part has none.
+__device__ __forceinline__ float output_scale(float base, float out, float sum) {
+    return sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / sum, (int)(out - base));
+}
+// A part's sum of weights for the join: 2^x y with y < 1, or no key.
+__device__ __forceinline__ v2f part_weight(float base, float sum) {
+    return v2f{base + (float)__builtin_amdgcn_frexp_expf(sum), __builtin_amdgcn_frexp_mantf(sum)};
+}
+
 // A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
-// MASKED: of these only keys [from, to) are visible.  Rescales o where the base moves.
+// MASKED: of these only keys [from, to) are visible.  Rescales sum and o where their bases move.
 template <bool MASKED, int TILES>
 __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int tiles, int from, int to,
                                       v8h (&hi)[2], v8h (&lo)[2]) {
-    const int exponent = min(max((int)(__float_as_uint(s.value) >> 23) - 127, -64), 126);
-    const float e = (float)exponent, down = __uint_as_float((uint32_t)(127 - exponent) << 23), f = s.value * down;
+    const float e = (float)((int)(__float_as_uint(s.value) >> 23) - 127);
     c *= s.key;
     c = c < 1e-37f ? 1e-37f : c;                    // (a masked key is minus infinity times it)
     if (MASKED) {
@@ -228,28 +238,34 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[j][r]);
-    top = fmaf(top, c, e);
-    top = max_xor32(max_xor16(top));
-    if (__any(top > m.base + kSlack)) {
+    top *= c;
+    float most = top + e;
+    if (__any(top > m.base + kSlack || most > m.out + kSlack)) {   // (a row's four lanes have the same bases)
+        top = max_xor32(max_xor16(top));
+        most = max_xor32(max_xor16(most));
         const float base = top > m.base + kSlack ? __builtin_ceilf(top) : m.base;
-        const float alpha = __builtin_amdgcn_exp2f(m.base - base);
+        const float out = most > m.out + kSlack ? __builtin_ceilf(most) : m.out;
+        const float alpha = __builtin_amdgcn_exp2f(m.out - out);
+        m.sum *= __builtin_amdgcn_exp2f(m.base - base);
         m.base = base;
-        m.sum *= alpha;
+        m.out = out;
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
             if (t < tiles) o[t] = o[t] * alpha;
     }
-    const float shift = e + (kLift - m.base);
+    const float shift = kLift - m.base;
+    float f = __builtin_amdgcn_ldexpf(s.value, (int)(m.base - m.out));
+    f = f > 0x1p127f ? 0x1p127f : f;                // (only where every u is below 2^-112; zero times infinity it may not be)
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float t = __builtin_amdgcn_exp2f(fmaf(acc[j][r], c, shift));
-            w[r] = t * f;
-            if (MASKED && (4 * j + r < from || 4 * j + r >= to)) t = w[r] = 0.0f;
-            sum += t;
+            float u = __builtin_amdgcn_exp2f(fmaf(acc[j][r], c, shift));
+            w[r] = u * f;
+            if (MASKED && (4 * j + r < from || 4 * j + r >= to)) u = w[r] = 0.0f;
+            sum += u;
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -260,7 +276,7 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
             lo[j >> 1][at] = l.x; lo[j >> 1][at + 1] = l.y;
         }
     }
-    m.sum = fmaf(sum, down, m.sum);
+    m.sum += sum;
 }
 
 // How a batch's work is shared out.  A request's rows of a KV head make tiles of
@@ -363,7 +379,7 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
     return found;
 }
 
-// Partial results: of each item its rows by dim floats; behind all of them each row's base and sum.
+// Partial results: of each item its rows' outputs, rows by dim floats; behind all of them each row's weight (part_weight).
 __device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, const Share& share, size_t item) {
     return p.partial + share.at + (kHeader + p.batch.requests + 3) / 4 * 4 + item * share.tile_rows * p.cache.dim;
 }
@@ -484,32 +500,35 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 
     // ---- the four waves' states together; wave w then has the tiles t % 4 = w
     __shared__ v4f values[kWaves][TILES][64];
-    __shared__ float bases[kWaves][16], sums[kWaves][16];
+    __shared__ float bases[kWaves][16], outs[kWaves][16], sums[kWaves][16];
     m.sum = add_xor32(add_xor16(m.sum));
     if (lq == 0) {
         bases[wave][li] = m.base;
+        outs[wave][li] = m.out;
         sums[wave][li] = m.sum;
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
         if (FULL || t < tiles) values[wave][t][lane] = o[t];
     __syncthreads();
-    float base = kNoBase, sum = 0.0f, alpha[kWaves];
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) base = fmaxf(base, bases[w][li]);
+    float base = kNoBase, out = kNoBase, sum = 0.0f, alpha[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        alpha[w] = __builtin_amdgcn_exp2f(bases[w][li] - base);
-        sum = fmaf(sums[w][li], alpha[w], sum);
+        base = fmaxf(base, bases[w][li]);
+        out = fmaxf(out, outs[w][li]);
+    }
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        alpha[w] = __builtin_amdgcn_exp2f(outs[w][li] - out);
+        sum = fmaf(sums[w][li], __builtin_amdgcn_exp2f(bases[w][li] - base), sum);
     }
     if (li >= rows) return;
     const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    float scale = 1.0f / sum;
+    const float scale = output_scale(base, out, sum);
     if (parts > 1) {
         to = partial_values(p, share, slot) + (size_t)li * dim;
-        scale = 1.0f;
-        if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = v2f{base, sum};
+        if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = part_weight(base, sum);
     }
     for (int t = wave; t < tiles; t += kWaves) {
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -663,12 +682,11 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const float sum = add_xor32(add_xor16(m.sum));
     if (w0 + li >= rows) return;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    float scale = 1.0f / sum;
+    const float scale = output_scale(m.base, m.out, sum);
     if (parts > 1) {
         const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
         to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
-        scale = 1.0f;
-        if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = v2f{m.base, sum};
+        if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = part_weight(m.base, sum);
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
@@ -696,15 +714,15 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
         const float* values = partial_values(p, share, slot) + (size_t)row * dim;
         float base = kNoBase, sum = 0.0f;
         for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
-        base = wave_max_f32(base);
+        base = wave_max_f32(base) + kJoinDrop;                     // weights of parts that together are at most one
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (own < abreast) {
 #pragma unroll 4
             for (int i = own; i < parts; i += abreast) {
                 const v2f s = sums[i * sum_stride];
                 const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
-                const float alpha = __builtin_amdgcn_exp2f(s.x - base);
-                sum = fmaf(s.y, alpha, sum);
+                const float alpha = s.y * __builtin_amdgcn_exp2f(s.x - base);
+                sum += alpha;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
             }
@@ -781,12 +799,13 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) base = fmaxf(base, sums[i * sum_stride].x);
+        base += kJoinDrop;                                         // weights of parts that together are at most one
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) {
             const v2f s = sums[i * sum_stride];
             const v4f v = *(const v4f*)(values + i * stride);
-            const float alpha = __builtin_amdgcn_exp2f(s.x - base);
-            sum = fmaf(s.y, alpha, sum);
+            const float alpha = s.y * __builtin_amdgcn_exp2f(s.x - base);
+            sum += alpha;
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
         }
@@ -822,7 +841,8 @@ int most_items(const AttentionKv8Call& call, const Share& share) {
     return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
 }
 
-// Partial results: a tile of several parts has more steps than `per`, so at most twice its steps / per.
+// Partial results: a tile of several parts has more steps than `per`, so at most twice its steps / per: at most
+// 2 * 768 + 1 in all.
 int most_slots(const AttentionKv8Call& call, const Share& share) {
     return std::min(share.items, 2 * ((share.target + call.cache.kv_heads - 1) / call.cache.kv_heads) + 1);
 }
