@@ -16,6 +16,7 @@ namespace leafhip {
 
 void hip_check(hipError_t status, const char* what) {
     if (status != hipSuccess) {
+        (void)hipGetLastError();   // reported here: not the next call's launch error
         const lh_status code = status == hipErrorOutOfMemory ? LH_ERROR_OUT_OF_MEMORY : LH_ERROR_DEVICE;
         throw Error(code, std::string("Leaf decoder: HIP error in ") + what + ": " + hipGetErrorString(status));
     }
