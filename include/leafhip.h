@@ -189,7 +189,9 @@ lh_status lh_synchronize(void);
  * the stream and frees that scratch; the scratch of a stream that was ever
  * captured stays allocated until the process ends, since a graph captured
  * from it may still be launched.  Threads may call them on one stream at a time
- * as they like: a call holds the stream's scratch until its last launch.  A graph
+ * as they like: a call holds the stream's scratch until its last launch.  On the
+ * per-thread default stream (hipStreamPerThread) scratch is kept for each thread, and
+ * taken over by a later thread after a thread's end.  A graph
  * with integer linears or one-token attention uses the scratch of the stream it
  * was captured from: launch it in order with that stream's own calls.
  * Attention of several tokens takes none while a stream captures (it then does

@@ -2,6 +2,7 @@
 // converts exceptions into a status code plus a thread-local message; nothing
 // throws across the ABI.
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cstdio>
 #include <cmath>
@@ -11,6 +12,7 @@
 #include <mutex>
 #include <optional>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -69,6 +71,10 @@ hipStream_t as_stream(lh_stream s) { return static_cast<hipStream_t>(s); }
 // later on another stream, so such a set is kept until the process ends.  Nothing
 // is freed by static destructors, which run after the HIP runtime and a profiler
 // may have shut down.
+//
+// The per-thread default stream is one handle for a stream of each thread, whose
+// calls run side by side: there a set is a thread's own.  When the thread ends its
+// sets wait for the next thread that needs one, unless a graph may hold them.
 struct StreamScratch {
     std::mutex in_use;                            // held by the call that uses the buffers
     leafhip::DeviceBuffer* work = nullptr;       // grown on demand
@@ -76,14 +82,49 @@ struct StreamScratch {
     std::vector<leafhip::DeviceBuffer*> retired;  // outgrown work buffers
     bool captured = false;                        // a graph may hold these buffers
 };
-std::mutex g_scratch_lock;                        // the map, and `captured`
-auto* g_scratch = new std::map<std::pair<int, hipStream_t>, std::shared_ptr<StreamScratch>>();
+// Of which thread: 0 unless the stream is the per-thread default stream.
+struct ScratchKey {
+    int device;
+    hipStream_t stream;
+    uint64_t thread;
+    bool operator<(const ScratchKey& o) const {
+        return std::tie(device, stream, thread) < std::tie(o.device, o.stream, o.thread);
+    }
+};
+std::mutex g_scratch_lock;                        // the maps, and `captured`
+auto* g_scratch = new std::map<ScratchKey, std::shared_ptr<StreamScratch>>();
+auto* g_idle_scratch = new std::multimap<int, std::shared_ptr<StreamScratch>>();   // of ended threads, by device
+
+// This thread's number, from 1.  Its end makes no HIP call: the runtime may be gone.
+struct ScratchThread {
+    uint64_t number = 0;
+    uint64_t get() {
+        static std::atomic<uint64_t> threads{0};
+        if (!number) number = ++threads;
+        return number;
+    }
+    ~ScratchThread() {
+        if (!number) return;
+        std::lock_guard<std::mutex> guard(g_scratch_lock);
+        for (auto it = g_scratch->begin(); it != g_scratch->end();) {
+            if (it->first.thread != number) {
+                ++it;
+                continue;
+            }
+            if (!it->second->captured) g_idle_scratch->emplace(it->first.device, it->second);
+            it = g_scratch->erase(it);
+        }
+    }
+};
+thread_local ScratchThread t_scratch_thread;
+
+uint64_t scratch_thread(hipStream_t stream) { return stream == hipStreamPerThread ? t_scratch_thread.get() : 0; }
 
 // Called with the stream idle and about to be destroyed.
 void release_stream_scratch(hipStream_t stream) {
     std::lock_guard<std::mutex> guard(g_scratch_lock);
     for (auto it = g_scratch->begin(); it != g_scratch->end();) {
-        if (it->first.second != stream) {
+        if (it->first.stream != stream) {
             ++it;
             continue;
         }
@@ -100,7 +141,7 @@ void release_stream_scratch(hipStream_t stream) {
 void mark_stream_captured(hipStream_t stream) {
     std::lock_guard<std::mutex> guard(g_scratch_lock);
     for (auto& [key, sc] : *g_scratch)
-        if (key.second == stream) sc->captured = true;
+        if (key.stream == stream && key.thread == scratch_thread(stream)) sc->captured = true;
 }
 
 bool capturing(hipStream_t stream) {
@@ -115,16 +156,27 @@ public:
     explicit ScratchUse(hipStream_t stream) : stream_(stream) {
         int dev = 0;
         leafhip::hip_check(hipGetDevice(&dev), "hipGetDevice");
+        const ScratchKey key{dev, stream, scratch_thread(stream)};
         {
             std::lock_guard<std::mutex> guard(g_scratch_lock);
-            auto& sc = (*g_scratch)[{dev, stream}];
-            if (!sc) sc = std::make_shared<StreamScratch>();
-            set_ = sc;
+            const auto found = g_scratch->find(key);
+            if (found != g_scratch->end()) set_ = found->second;
+        }
+        if (!set_) {
+            auto made = key.thread ? of_ended_thread(dev) : nullptr;
+            if (!made) made = std::make_shared<StreamScratch>();
+            std::lock_guard<std::mutex> guard(g_scratch_lock);
+            set_ = g_scratch->emplace(key, made).first->second;   // (another thread's, where it was first)
         }
         held_ = std::unique_lock<std::mutex>(set_->in_use);
     }
 
     void* work(size_t bytes) {
+        // (the library's own captures are marked where they begin; a thread's set outlives it only unmarked)
+        if (stream_ == hipStreamPerThread && capturing(stream_)) {
+            std::lock_guard<std::mutex> guard(g_scratch_lock);
+            set_->captured = true;
+        }
         if (!set_->work || set_->work->bytes < bytes) {
             if (capturing(stream_))
                 throw leafhip::Error(LH_ERROR_STATE, "Leaf decoder: kernel scratch must grow outside stream capture "
@@ -138,8 +190,8 @@ public:
 
     // For work that can also run without: null while the stream captures (a
     // graph that held the buffer would race, launched on another stream, with
-    // this one's calls), on the per-thread default stream, whose one handle
-    // stands for a stream of each thread, and where the device has no memory left.
+    // this one's calls), on the per-thread default stream, where it would be
+    // memory for each thread, and where the device has no memory left.
     void* work_if_own(size_t bytes) {
         try {
             if (stream_ == hipStreamPerThread || capturing(stream_)) return nullptr;
@@ -171,6 +223,24 @@ public:
     }
 
 private:
+    // A set that an ended thread has left, once all work that may use it is done; null: none.
+    std::shared_ptr<StreamScratch> of_ended_thread(int dev) {
+        if (capturing(stream_)) return nullptr;
+        std::shared_ptr<StreamScratch> set;
+        {
+            std::lock_guard<std::mutex> guard(g_scratch_lock);
+            const auto it = g_idle_scratch->find(dev);
+            if (it == g_idle_scratch->end()) return nullptr;
+            set = it->second;
+            g_idle_scratch->erase(it);
+        }
+        if (hipDeviceSynchronize() == hipSuccess) return set;
+        (void)hipGetLastError();                  // another thread captures: for a later call
+        std::lock_guard<std::mutex> guard(g_scratch_lock);
+        g_idle_scratch->emplace(dev, set);
+        return nullptr;
+    }
+
     hipStream_t stream_;
     std::shared_ptr<StreamScratch> set_;   // released after held_
     std::unique_lock<std::mutex> held_;
@@ -615,7 +685,7 @@ lh_status lh_stream_create(lh_stream* out) {
 }
 lh_status lh_stream_destroy(lh_stream stream) {
     return guarded([&] {
-        require_arg(stream, "only a created stream can be destroyed");
+        require_arg(stream && as_stream(stream) != hipStreamPerThread, "only a created stream can be destroyed");
         leafhip::hip_check(hipStreamSynchronize(as_stream(stream)), "hipStreamSynchronize");
         release_stream_scratch(as_stream(stream));
         leafhip::hip_check(hipStreamDestroy(as_stream(stream)), "hipStreamDestroy");
