@@ -409,7 +409,8 @@ lh_status lh_rope_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const float
  * and rows (of any source: a request whose rows or length do not fit the batch is
  * passed over, its rows of out left as they were, as are padding rows).  A query
  * that is not finite, a block whose scale is negative or not finite and a table entry
- * that is no block give NaN in the rows that see them, and only there.  The codes of
+ * that is no block give NaN in the rows that see them, and only there; so does a row's
+ * largest score (times log2 e) where f32 has no number for it.  The codes of
  * written places are those lh_rope_kv8 writes (E4M3's NaN is not among them).
  *
  * Long contexts are split over the GPU; the parts' results pass through a workspace

@@ -10,13 +10,15 @@
 //
 // Scales.  The score of a key is (q . code) c with c = query scale * key scale *
 // log2(e) / sqrt(dim); its weight is u = 2^(score - a + 8).  What meets the value
-// codes is w = u v 2^(a - b) of a value scale v = 2^e f, 1 <= f < 2: relative to the
+// codes is w = u v 2^-d of a value scale v = 2^e f, 1 <= f < 2: relative to the
 // largest weight times value scale, so that it keeps its 22 bits wherever it counts
 // however far the scales of blocks are apart, while the sum is of u, in which a key
-// counts whatever its value's scale is.  a and b are whole numbers per row, at most 6
-// below the largest score and the largest score + e so far (u < 2^14, w < 2^15), so
-// most steps rescale nothing and a rescale is exact.  A row's output is its sum of
-// w times codes, times 2^(b - a), over its sum of u.
+// counts whatever its value's scale is.  a and d are whole numbers per row, a at most 6
+// below the largest score and d at most 6 below the largest score - a + e so far
+// (u < 2^14, w < 2^15), so most steps rescale nothing and a rescale is exact.  A row's
+// output is its sum of w times codes, times 2^d, over its sum of u.  Scores past 2^22
+// are rounded before a is taken from them, as a was (score - a + 8 in one rounding is
+// off by the product's, which is then half and more).
 //
 // Layout.  A step is 64 keys.  S^T = K Q^T by v_mfma_f32_16x16x32_f16 with lane
 // l = 16 lq + li: row li of its tile j of keys is key 16 (li / 4) + 4 j + li % 4
@@ -49,9 +51,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kFewRows = 16;                        // rows of a KV head in one tile
 constexpr int kHeader = 4;                          // integers before a plan's requests
-constexpr float kNoBase = -1e30f;
+constexpr float kNoBase = -3e38f;
 constexpr float kSlack = 6.0f, kLift = 8.0f;
-constexpr float kJoinDrop = 11.0f;                  // a tile has fewer than 2^11 parts: see most_slots
+constexpr float kFar = 4194304.0f;
 
 // 16 codes as two operands.
 template <bool E4M3>
@@ -204,19 +206,16 @@ __device__ __forceinline__ v4u first_codes(v4u codes, int keys) {
     return codes;
 }
 
-// A row's online softmax: the bases of its weights and of its outputs (a and b above), and its sum (this lane's keys).
+// A row's online softmax: the bases of its weights and of its outputs (a and d above), and its sum (this lane's keys).
 struct Softmax {
-    float base = kNoBase, out = kNoBase, sum = 0.0f;
+    float base = kNoBase, lift = 0.0f, sum = 0.0f;
+    bool far = false;                               // of the wave: whether a base is past kFar
 };
 
-// What a row's outputs are multiplied by.  A row that sees no key of a part has none.
-__device__ __forceinline__ float output_scale(float base, float out, float sum) {
-    return sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / sum, (int)(out - base));
-}
-// A part's sum of weights for the join: 2^x y with y < 1, or no key.
-__device__ __forceinline__ v2f part_weight(float base, float sum) {
-    return v2f{base + (float)__builtin_amdgcn_frexp_expf(sum), __builtin_amdgcn_frexp_mantf(sum)};
-}
+// What a row's outputs are multiplied by.
+__device__ __forceinline__ float output_scale(float lift, float sum) { return __builtin_amdgcn_ldexpf(1.0f / sum, (int)lift); }
+// The same of a part, of which a row may see no key.
+__device__ __forceinline__ float part_scale(float lift, float sum) { return sum == 0.0f ? 0.0f : output_scale(lift, sum); }
 
 // A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
 // MASKED: of these only keys [from, to) are visible.  Rescales sum and o where their bases move.
@@ -239,30 +238,42 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[j][r]);
     top *= c;
-    float most = top + e;
-    if (__any(top > m.base + kSlack || most > m.out + kSlack)) {   // (a row's four lanes have the same bases)
-        top = max_xor32(max_xor16(top));
-        most = max_xor32(max_xor16(most));
-        const float base = top > m.base + kSlack ? __builtin_ceilf(top) : m.base;
-        const float out = most > m.out + kSlack ? __builtin_ceilf(most) : m.out;
-        const float alpha = __builtin_amdgcn_exp2f(m.out - out);
-        m.sum *= __builtin_amdgcn_exp2f(m.base - base);
+    if (__any(top - m.base > kSlack || (top - m.base) + e > m.lift + kSlack)) {   // (a row's four lanes have the same bases)
+        const float row_top = max_xor32(max_xor16(top));
+        const float base = row_top - m.base > kSlack ? __builtin_ceilf(row_top) : m.base, moved = m.base - base;
+        const float most = max_xor32(max_xor16((top - base) + e));
+        // (the outputs' own base, base + lift, moves only where it has to)
+        const float kept = m.lift + moved, lift = most > kept + kSlack ? __builtin_ceilf(most) : kept;
+        const float alpha = __builtin_amdgcn_exp2f(kept - lift);
+        m.sum *= __builtin_amdgcn_exp2f(moved);
         m.base = base;
-        m.out = out;
+        m.lift = lift;
+        m.far = __any(__builtin_fabsf(base) > kFar && base != kNoBase);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-            if (t < tiles) o[t] = o[t] * alpha;
+        for (int t = 0; t < TILES; ++t) o[t] = o[t] * alpha;
     }
-    const float shift = kLift - m.base;
-    float f = __builtin_amdgcn_ldexpf(s.value, (int)(m.base - m.out));
+    float f = __builtin_amdgcn_ldexpf(s.value, -(int)m.lift);
     f = f > 0x1p127f ? 0x1p127f : f;                // (only where every u is below 2^-112; zero times infinity it may not be)
+    const float shift = kLift - m.base;
+    if (m.far) {
+        const bool far = __builtin_fabsf(m.base) > kFar;           // a row's own: all of its waves weigh a score alike
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][r] = far ? (acc[j][r] * c - m.base) + kLift : fmaf(acc[j][r], c, shift);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(acc[j][r], c, shift);
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float u = __builtin_amdgcn_exp2f(fmaf(acc[j][r], c, shift));
+            float u = __builtin_amdgcn_exp2f(acc[j][r]);
             w[r] = u * f;
             if (MASKED && (4 * j + r < from || 4 * j + r >= to)) u = w[r] = 0.0f;
             sum += u;
@@ -379,7 +390,7 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
     return found;
 }
 
-// Partial results: of each item its rows' outputs, rows by dim floats; behind all of them each row's weight (part_weight).
+// Partial results: of each item its rows' outputs, rows by dim floats; behind all of them each row's base and sum.
 __device__ __forceinline__ float* partial_values(const AttentionKv8Call& p, const Share& share, size_t item) {
     return p.partial + share.at + (kHeader + p.batch.requests + 3) / 4 * 4 + item * share.tile_rows * p.cache.dim;
 }
@@ -478,14 +489,13 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
             // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
             const int written = now.known ? q.length - at : 0;
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
-                if (FULL || t < tiles) vr[t] = first_codes(vr[t], written);
+            for (int t = 0; t < TILES; ++t) vr[t] = first_codes(vr[t], written);
         } else {
             weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
-            if (FULL || t < tiles) {
+            if (FULL || t <= 4 * CC - 4 || t < tiles) {            // (a head has more than 64 (CC - 1) dims)
                 v8h v[2];
                 widen<E4M3>(vr[t], v[0], v[1]);
 #pragma unroll
@@ -500,35 +510,37 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 
     // ---- the four waves' states together; wave w then has the tiles t % 4 = w
     __shared__ v4f values[kWaves][TILES][64];
-    __shared__ float bases[kWaves][16], outs[kWaves][16], sums[kWaves][16];
+    __shared__ float bases[kWaves][16], lifts[kWaves][16], sums[kWaves][16];
     m.sum = add_xor32(add_xor16(m.sum));
     if (lq == 0) {
         bases[wave][li] = m.base;
-        outs[wave][li] = m.out;
+        lifts[wave][li] = m.lift;
         sums[wave][li] = m.sum;
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
         if (FULL || t < tiles) values[wave][t][lane] = o[t];
     __syncthreads();
-    float base = kNoBase, out = kNoBase, sum = 0.0f, alpha[kWaves];
+    float base = kNoBase, lift = -INFINITY, sum = 0.0f, alpha[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) base = fmaxf(base, bases[w][li]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        base = fmaxf(base, bases[w][li]);
-        out = fmaxf(out, outs[w][li]);
+        const float below = bases[w][li] - base;
+        sum = fmaf(sums[w][li], __builtin_amdgcn_exp2f(below), sum);
+        alpha[w] = below + lifts[w][li];
+        lift = fmaxf(lift, alpha[w]);
     }
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        alpha[w] = __builtin_amdgcn_exp2f(outs[w][li] - out);
-        sum = fmaf(sums[w][li], __builtin_amdgcn_exp2f(bases[w][li] - base), sum);
-    }
+    for (int w = 0; w < kWaves; ++w) alpha[w] = __builtin_amdgcn_exp2f(alpha[w] - lift);
     if (li >= rows) return;
     const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    const float scale = output_scale(base, out, sum);
+    float scale = output_scale(lift, sum);
     if (parts > 1) {
         to = partial_values(p, share, slot) + (size_t)li * dim;
-        if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = part_weight(base, sum);
+        scale = part_scale(lift, sum);
+        if (wave == 0 && lq == 0) partial_sums(p, share, slot)[li] = v2f{base, sum};
     }
     for (int t = wave; t < tiles; t += kWaves) {
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -682,15 +694,27 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const float sum = add_xor32(add_xor16(m.sum));
     if (w0 + li >= rows) return;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    const float scale = output_scale(m.base, m.out, sum);
+    float scale = output_scale(m.lift, sum);
     if (parts > 1) {
         const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
         to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
-        if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = part_weight(m.base, sum);
+        scale = part_scale(m.lift, sum);
+        if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = v2f{m.base, sum};
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
         if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[t] * scale;
+}
+
+// A row's parts together: its base, and its sum relative to that.
+__device__ __forceinline__ void add_part(v2f part, float& base, float& total) {
+    const float most = fmaxf(base, part.x);
+    total = fmaf(total, __builtin_amdgcn_exp2f(base - most), part.y * __builtin_amdgcn_exp2f(part.x - most));
+    base = most;
+}
+// What a part's outputs count for: at most one, so that no output is too large or too small for the sum.
+__device__ __forceinline__ float part_share(v2f part, float base, float inverse) {
+    return part.y * __builtin_amdgcn_exp2f(part.x - base) * inverse;
 }
 
 // ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
@@ -712,33 +736,27 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
     for (int row = threadIdx.x >> 6; row < q.rows * group; row += blockDim.x >> 6) {
         const v2f* sums = partial_sums(p, share, slot) + row;
         const float* values = partial_values(p, share, slot) + (size_t)row * dim;
-        float base = kNoBase, sum = 0.0f;
-        for (int i = lane; i < parts; i += 64) base = fmaxf(base, sums[i * sum_stride].x);
-        base = wave_max_f32(base) + kJoinDrop;                     // weights of parts that together are at most one
+        float base = kNoBase, total = 0.0f;
+        for (int i = lane; i < parts; i += 64) add_part(sums[i * sum_stride], base, total);
+        const float own_base = base;
+        base = wave_max_f32(base);
+        const float inverse = 1.0f / wave_sum_f32(total * __builtin_amdgcn_exp2f(own_base - base));
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (own < abreast) {
 #pragma unroll 4
             for (int i = own; i < parts; i += abreast) {
-                const v2f s = sums[i * sum_stride];
+                const float share_of = part_share(sums[i * sum_stride], base, inverse);
                 const v4f v = *(const v4f*)(values + i * stride + 4 * quad);
-                const float alpha = s.y * __builtin_amdgcn_exp2f(s.x - base);
-                sum += alpha;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], share_of, x[r]);
             }
         }
         // the parts abreast together, in their order
         v4f all = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        float total = 0.0f;
-        for (int k = 0; k < abreast; ++k) {
-            total += __shfl(sum, k * quads + quad, 64);
+        for (int k = 0; k < abreast; ++k)
 #pragma unroll
             for (int r = 0; r < 4; ++r) all[r] += __shfl(x[r], k * quads + quad, 64);
-        }
-        if (own == 0) {
-            const float scale = 1.0f / total;
-            *(v4f*)(p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim + 4 * quad) = all * scale;
-        }
+        if (own == 0) *(v4f*)(p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim + 4 * quad) = all;
     }
 }
 
@@ -795,22 +813,19 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
         const int row = u / quads, quad = u % quads;
         const v2f* sums = partial_sums(p, share, slot) + row;
         const float* values = partial_values(p, share, slot) + (size_t)row * dim + 4 * quad;
-        float base = kNoBase, sum = 0.0f;
+        float base = kNoBase, total = 0.0f;
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-        for (int i = 0; i < parts; ++i) base = fmaxf(base, sums[i * sum_stride].x);
-        base += kJoinDrop;                                         // weights of parts that together are at most one
+        for (int i = 0; i < parts; ++i) add_part(sums[i * sum_stride], base, total);
+        const float inverse = 1.0f / total;
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) {
-            const v2f s = sums[i * sum_stride];
+            const float share_of = part_share(sums[i * sum_stride], base, inverse);
             const v4f v = *(const v4f*)(values + i * stride);
-            const float alpha = s.y * __builtin_amdgcn_exp2f(s.x - base);
-            sum += alpha;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], alpha, x[r]);
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], share_of, x[r]);
         }
-        const float scale = 1.0f / sum;
-        *(v4f*)(p.out + ((size_t)(q.start + (r0 + row) / group) * p.heads + kvh * group + (r0 + row) % group) * dim + 4 * quad) = x * scale;
+        *(v4f*)(p.out + ((size_t)(q.start + (r0 + row) / group) * p.heads + kvh * group + (r0 + row) % group) * dim + 4 * quad) = x;
     }
 }
 
@@ -841,8 +856,7 @@ int most_items(const AttentionKv8Call& call, const Share& share) {
     return (int)std::min<size_t>((share.target + kv - 1) / kv + tiles, tiles * ((longest + share.least - 1) / share.least));
 }
 
-// Partial results: a tile of several parts has more steps than `per`, so at most twice its steps / per: at most
-// 2 * 768 + 1 in all.
+// Partial results: a tile of several parts has more steps than `per`, so at most twice its steps / per.
 int most_slots(const AttentionKv8Call& call, const Share& share) {
     return std::min(share.items, 2 * ((share.target + call.cache.kv_heads - 1) / call.cache.kv_heads) + 1);
 }
