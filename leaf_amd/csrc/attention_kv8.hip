@@ -16,9 +16,9 @@
 // counts whatever its value's scale is.  a and d are whole numbers per row, a at most 6
 // below the largest score and d at most 6 below the largest score - a + e so far
 // (u < 2^14, w < 2^15), so most steps rescale nothing and a rescale is exact.  A row's
-// output is its sum of w times codes, times 2^d, over its sum of u.  Scores past 2^22
-// are rounded before a is taken from them, as a was (score - a + 8 in one rounding is
-// off by the product's, which is then half and more).
+// output is its sum of w times codes, times 2^d, over its sum of u.  score - a + 8 is one
+// fused operation where what the rounding of a's own score left out is little; past
+// 2^22, where it grows to more than w has room for, scores are rounded before a is taken.
 //
 // Layout.  A step is 64 keys.  S^T = K Q^T by v_mfma_f32_16x16x32_f16 with lane
 // l = 16 lq + li: row li of its tile j of keys is key 16 (li / 4) + 4 j + li % 4
@@ -28,9 +28,10 @@
 // dim's tokens together), and a lane's 16 keys lie in one block, with one scale.
 // Both K and V come as 16-byte loads; a key's dims are permuted alike in Q.
 //
-// Two kernels: requests of at most 16 rows of a KV head (attention_kv8_few_kernel)
-// read the cache straight into registers, others (attention_kv8_rows_kernel)
-// share what they widen through LDS.  The keys of a tile of rows are cut into
+// Two kernels: attention_kv8_few_kernel takes requests of at most 16 rows of a KV
+// head and reads the cache straight into registers; attention_kv8_rows_kernel takes
+// the others, or every request (see kManyTokens), and shares what it widens through
+// LDS.  The keys of a tile of rows are cut into
 // parts where a batch has too few tiles for the GPU, and a second launch joins
 // the parts.  Lengths are known on the device only: every workgroup sums the
 // batch and finds its own part (dependent loads, part of the 7 us that the smallest call takes).
@@ -53,7 +54,7 @@ constexpr int kFewRows = 16;                        // rows of a KV head in one 
 constexpr int kHeader = 4;                          // integers before a plan's requests
 constexpr float kNoBase = -3e38f;
 constexpr float kSlack = 6.0f, kLift = 8.0f;
-constexpr float kFar = 4194304.0f;
+constexpr float kFar = 4194304.0f;                  // 2^22: a score's rounding is an eighth below it (w has room for one)
 
 // 16 codes as two operands.
 template <bool E4M3>
@@ -220,7 +221,7 @@ __device__ __forceinline__ float part_scale(float lift, float sum) { return sum 
 // A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
 // MASKED: of these only keys [from, to) are visible.  Rescales sum and o where their bases move.
 template <bool MASKED, int TILES>
-__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int tiles, int from, int to,
+__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int from, int to,
                                       v8h (&hi)[2], v8h (&lo)[2]) {
     const float e = (float)((int)(__float_as_uint(s.value) >> 23) - 127);
     c *= s.key;
@@ -401,11 +402,12 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 // ---- at most 16 rows of a KV head (single tokens): each wave takes every fourth step, straight from memory
 // 64 requests of 200 to 4096 tokens, 32 heads of 128 over 8: 69 us and 5 for the
 // join, 281 MB at 4.1 TB/s.  What bounds it is latency: without its arithmetic an
-// earlier state took 65 of 77 us in all.  A part is some eight steps a wave behind four
-// dependent loads (its place, the query, the first table entries, the first codes); that
-// these starts are what is left is not shown.  8 requests of 16000 tokens
-// take 57 us, 4.6 TB/s.  Vector instructions issue for 39% of a busy CU's time, 320 of
-// 680 a step of 64 keys widening codes (INT8, heads of 128).
+// earlier state took 65 of 77 us in all.  A CU has waves for 66% of the kernel's cycles,
+// and issues vector instructions for 41% of those, 320 of some 680 a step of 64 keys
+// widening codes (INT8, heads of 128).  A part is some eight steps a wave behind four
+// dependent loads (its place, the query, the first table entries, the first codes); how
+// much of the rest is these starts and how much parts that end unevenly is not shown.
+// 8 requests of 16000 tokens take 57 us, 4.6 TB/s.
 template <int CC, bool FULL, bool E4M3>
 __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
@@ -485,13 +487,13 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
         const int at = step * kStep + 16 * lq;                     // the lane's first key
         if (step * kStep + kStep > low + 1 || p.window) {          // the wave's rows see different keys
             const int from = p.window ? position + 1 - p.window - at : 0;
-            weigh<true>(acc, c, now, m, o, tiles, from, position + 1 - at, hi, lo);
+            weigh<true>(acc, c, now, m, o, from, position + 1 - at, hi, lo);
             // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
             const int written = now.known ? q.length - at : 0;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) vr[t] = first_codes(vr[t], written);
         } else {
-            weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
+            weigh<false>(acc, c, now, m, o, 0, 16, hi, lo);
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -555,11 +557,13 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 }
 
 // ---- more rows of a KV head: tiles of 64, 16 for a wave, K and V widened once for all of them through LDS
-// 512 tokens behind 7001 keys, 32 heads of 128 over 8 (E4M3): 141 to 147 us, about
+// 512 tokens behind 7001 keys, 32 heads of 128 over 8 (E4M3): 137 to 147 us, about
 // 10 of them the join's; 2048 tokens of 14 heads of 64 over 2 (INT8): 44 to 46, 7 the join's.
-// What bounds it is issue: other vector instructions (257 a step of 16 scores a lane, some 80
-// of them widening codes) take 42% of the chunk's busy cycles and MFMAs 41%, of the
-// prompt's 57% and 22%.  Two row tiles
+// What bounds the chunk is issue: a CU has waves for 87% of the kernel's cycles, and of those
+// other vector instructions (252 a step of 16 scores a lane, some 80 of them widening codes)
+// take 41% and MFMAs 42%.  The prompt leaves CUs idle first: they have waves for 59% of the
+// cycles, of which vector instructions take 57% and MFMAs 22%.  Its tiles see from one step
+// to all, while parts are cut, and workgroups launched, for tiles as long as the last.  Two row tiles
 // a wave (54 us for the prompt, 138 for the chunk, with spills), three or four waves a
 // SIMD in fewer registers (47 and 169), and eight waves in two groups half a step apart, one
 // in its products while the other is in its softmax (62 and 143), gave nothing.
@@ -667,9 +671,9 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
             const int at = step * kStep + 16 * lq;
             if (step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window)) {
                 const int from = p.window ? position + 1 - p.window - at : 0;
-                weigh<true>(acc, c, now, m, o, tiles, from, position + 1 - at, hi, lo);
+                weigh<true>(acc, c, now, m, o, from, position + 1 - at, hi, lo);
             } else {
-                weigh<false>(acc, c, now, m, o, tiles, 0, 16, hi, lo);
+                weigh<false>(acc, c, now, m, o, 0, 16, hi, lo);
             }
 #pragma unroll
             for (int t0 = 0; t0 < TILES; t0 += 4) {
@@ -838,9 +842,11 @@ constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; 
 // Steps of a part at least, with 4 / 8: one request of 4095 tokens 10.9 / 12.5 us (a part's wave has one or two steps);
 // eight prompts of 300 tokens 37 / 27 (none is parted with 8; 16 costs a chunk beside decoding requests 47 for 44).
 constexpr int kFewLeast = 4, kRowsLeast = 8;
-// New tokens of a request, on average, from which the kernel of many rows takes every request: one launch in place of
+// Rows of the step for each request from which the kernel of many rows takes every request: one launch in place of
 // two, one after the other, although it has a request of one token in a tile of 64.  At 13 a request it takes 75 us for 73
-// (heads of 128) and at 8 30 for 40 (heads of 64), at 3.5 203 for 151 and 39 for 45.
+// (heads of 128) and at 8 30 for 40 (heads of 64), at 3.5 203 for 151 and 39 for 45; between 3.5 and 8 nothing was
+// measured.  The host knows the batch's sizes alone, so padding rows count: 64 single tokens in 512 rows take 110 us for
+// 74 (heads of 128) and 43 for 24 (heads of 64) where max_rows lets the rows be one request's.
 constexpr int kManyTokens = 6;
 
 // At most this many tiles, and items, of a KV head: a tile's parts are at most its steps / per + 1.

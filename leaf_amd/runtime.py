@@ -406,6 +406,8 @@ class BlockPool:
 
     ``step`` takes each request's new tokens (negative: it has ended) to the device and assigns their blocks;
     ``batch`` is what ``rope_kv8`` and ``attention_kv8`` take then.  Lengths and free blocks are kept on the device.
+    ``tokens`` and ``max_rows`` are the most that a step has; kernels are chosen by ``batch.tokens`` and ``batch.max_rows``,
+    so set these to a step's own rows and its longest request's before it (q_heads and out have ``batch.tokens`` rows then).
     A step waits on the host for what its stream has to do already, which may still read the last step's new tokens; a
     step that is captured writes ``fresh`` itself and calls ``kv_assign``.
     """
