@@ -429,6 +429,95 @@ lh_status lh_attention_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const 
 /* Bytes that any call of the batch's sizes needs, whatever the lengths. */
 lh_status lh_attention_kv8_workspace(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads, size_t* bytes);
 
+/* ------------------------------------------------- drafted trees over that cache
+ * A step that checks drafted tokens: a request's new rows are a tree, its first row
+ * the last token that stands (not in the cache yet), each other row a drafted token
+ * behind its parent.  After lh_kv_assign,
+ *   lh_kv_tree             positions and ancestor masks of the rows,
+ *   lh_rope_kv8            as ever, with these positions,
+ *   lh_attention_kv8_tree  attention of each row over the cached keys and its ancestors,
+ *   lh_verify_drafts       which rows stand, and the token behind the last of them,
+ *   lh_kv8_compact         the rows that stand moved together, in all layers' caches,
+ *   lh_kv_keep             lengths and free blocks as if only these had been taken in.
+ * A row that is not drafted (of a prompt, or a single token) is a tree of one path.  No
+ * call reads lengths or results on the host, so the step can be captured and replayed. */
+#define LH_KV_TREE_ROWS 512 /* of a request: the batch's max_rows is at most this */
+
+/* parents [tokens] (device): for row i of a request its parent, an earlier row of the request; -1 (or
+ * what is no earlier row) for one whose parent is the last cached token.  Writes for the
+ * rows of requests that were taken in
+ *   positions[t]   length - rows + (number of ancestors in the step), and
+ *   masks [tokens][words], words = (max_rows + 63) / 64: bit j % 64 of word j / 64 is
+ *                  set where row j of the request is the row itself or an ancestor;
+ * other rows' entries stay as they were.  Reads the batch's lengths, starts and rows. */
+lh_status lh_kv_tree(const lh_kv_batch* batch, const int32_t* parents, uint64_t* masks, lh_stream stream);
+
+/* lh_attention_kv8 of trees: a row sees the keys of its request before the step's rows,
+ * length - rows of them, and of these rows those whose bit is set in its mask, whatever their order (the
+ * masks may be others than lh_kv_tree's; bits of rows that the request does not have count for nothing).  With a window, keys at
+ * positions up to the row's own less window are hidden, where a step's row stands at positions[t] (at
+ * least length - rows; read only then).  A row that sees no key gets zeros.  Otherwise as
+ * lh_attention_kv8: the same batch arrays, NaN rules, accuracy and workspace. */
+lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,
+                                uint32_t window, const uint64_t* masks, float* out, void* workspace, size_t workspace_bytes,
+                                lh_stream stream);
+
+/* What verification reads and writes: device pointers. */
+typedef struct lh_drafts {
+    uint32_t vocab;
+    const float* logits;         /* [tokens][vocab] the model's, of every row */
+    const float* draft_logits;   /* [tokens][vocab] the draft's at the rows whose children were drawn from it; NULL: drafts come without probabilities */
+    const int32_t* ids;          /* [tokens] the rows' tokens */
+    const int32_t* parents;      /* [tokens] as for lh_kv_tree */
+    const float* temperatures;   /* [requests] T; 0: greedy */
+    const float* accept;         /* [tokens] a random number of [0, 1) for each row; negative: the row stands without a test */
+    const float* sample;         /* [requests] a random number of [0, 1) for the token behind */
+    int32_t* path;               /* [tokens] from starts[r] on: the request's rows that stand, in order from row 0; behind them -1 */
+    int32_t* kept;               /* [requests] how many */
+    int32_t* next;               /* [requests] the token behind the last of them */
+} lh_drafts;
+
+/* Which drafted tokens stand.  Row 0 does.  From the last row that stands, its children
+ * are tried in the order of their rows, until one is taken (which stands then) or none is left:
+ *   greedy    a child is taken if its token is the first largest of its parent's logits;
+ *             the token behind is that of the last row;
+ *   sampling  with p = softmax(logits / T) and q = softmax(draft_logits / T) of the parent,
+ *             C = 0 and r = p at first, and S the sum of r: a child with token x and
+ *             random number u is taken if u S q(x) < r(x).  If not, C becomes C + S and r
+ *             max(p - C q, 0), which keeps the tokens that stand distributed as p says.  Without
+ *             draft_logits (tokens that were not drawn, as the draft's best) x is taken if u S < r(x); if
+ *             not, r(x) becomes 0.  The token behind is the first whose sum of r in the tokens' order
+ *             passes sample times S (where nothing is left, S = 0, the same of p).
+ * All in 64 bits: a random number within 1e-12 of a border may fall to either side.
+ * A token outside the vocabulary is not taken.  Where a test or the token behind needs logits of
+ * which one is NaN or plus infinity or all are minus infinity, or a T that is negative or
+ * not finite, the walk ends, with next -1.  A request without rows has kept 0 and next -1.
+ * Reads the batch's starts and rows; the rows' entries of requests that have none, and padding's, stay as they were.
+ * The workspace is lh_attention_kv8's: the caller's, 16-byte aligned, of lh_verify_drafts_workspace
+ * bytes, or with NULL (and 0) the scratch of the stream. */
+lh_status lh_verify_drafts(const lh_kv_batch* batch, const lh_drafts* drafts, void* workspace, size_t workspace_bytes,
+                           lh_stream stream);
+/* Bytes that any call of the batch's sizes and the vocabulary needs (draft_logits NULL or not as in the call). */
+lh_status lh_verify_drafts_workspace(const lh_kv_batch* batch, const lh_drafts* drafts, size_t* bytes);
+
+/* The rows that stand, moved together in `layers` caches (caches is a host array; all of the same
+ * heads, dim and format): of each request row path[starts[r] + k] goes to the place of row k, for k
+ * < kept[r].  A block that takes in a moved row gets, for keys and for values of each KV head, the largest scale of the blocks that
+ * its tokens (cached ones, and rows that stand) come from, and their codes become code * old
+ * scale / scale as in lh_rope_kv8; other blocks, and the places behind the rows that stand, stay
+ * as they were.  A scale among these that is negative or not finite makes the block's NaN.  Reads the batch's table, lengths
+ * (with all of the step's rows: before lh_kv_keep), starts and rows.  A request whose path does not ascend
+ * within its rows or whose kept is not 1..rows is passed over, and so is a row whose block, on either side, is none of the pool. */
+lh_status lh_kv8_compact(const lh_kv_batch* batch, const lh_kv8* caches, uint32_t layers, const int32_t* path,
+                         const int32_t* kept, lh_stream stream);
+
+/* Lengths and blocks after a step of which kept[r] of a request's rows stand: lengths [requests]
+ * (may be the batch's own) becomes length - rows + kept, and the blocks behind that go on
+ * the free stack, in the requests' order, behind its *free_count entries; *free_left is the count then (it may be
+ * free_count itself, which says the free blocks that lh_kv_assign left).  A request without rows, or whose kept is
+ * not 0..rows, keeps its length.  Reads the batch's table, lengths and rows. */
+lh_status lh_kv_keep(const lh_kv_batch* batch, const int32_t* kept, int32_t* lengths, lh_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

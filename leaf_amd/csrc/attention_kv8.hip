@@ -218,11 +218,28 @@ __device__ __forceinline__ float output_scale(float lift, float sum) { return __
 // The same of a part, of which a row may see no key.
 __device__ __forceinline__ float part_scale(float lift, float sum) { return sum == 0.0f ? 0.0f : output_scale(lift, sum); }
 
+// Which of a lane's 16 keys of a step its row sees: all, those of [from, to), or those with a bit.
+struct EveryKey {
+    static constexpr bool kAll = true;
+    __device__ __forceinline__ bool operator()(int) const { return true; }
+};
+struct KeyRange {
+    static constexpr bool kAll = false;
+    int from, to;
+    __device__ __forceinline__ bool operator()(int k) const { return k >= from && k < to; }
+};
+struct KeyBits {
+    static constexpr bool kAll = false;
+    uint32_t bits;
+    __device__ __forceinline__ bool operator()(int k) const { return bits >> k & 1; }
+};
+
 // A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
-// MASKED: of these only keys [from, to) are visible.  Rescales sum and o where their bases move.
-template <bool MASKED, int TILES>
-__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], int from, int to,
+// Rescales sum and o where their bases move.
+template <typename Seen, int TILES>
+__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], Seen seen,
                                       v8h (&hi)[2], v8h (&lo)[2]) {
+    constexpr bool MASKED = !Seen::kAll;
     const float e = (float)((int)(__float_as_uint(s.value) >> 23) - 127);
     c *= s.key;
     c = c < 1e-37f ? 1e-37f : c;                    // (a masked key is minus infinity times it)
@@ -231,7 +248,7 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (4 * j + r < from || 4 * j + r >= to) acc[j][r] = -INFINITY;
+                if (!seen(4 * j + r)) acc[j][r] = -INFINITY;
     }
     float top = acc[0][0];
 #pragma unroll
@@ -276,7 +293,7 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
         for (int r = 0; r < 4; ++r) {
             float u = __builtin_amdgcn_exp2f(acc[j][r]);
             w[r] = u * f;
-            if (MASKED && (4 * j + r < from || 4 * j + r >= to)) u = w[r] = 0.0f;
+            if (MASKED && !seen(4 * j + r)) u = w[r] = 0.0f;
             sum += u;
         }
 #pragma unroll
@@ -290,6 +307,56 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
     }
     m.sum += sum;
 }
+
+// A row of a tree: the keys before the step's own, and of these the rows whose bits its mask has.  ONE: the request
+// has no more rows than bits of a word, which is loaded once.
+template <int ONE>
+struct TreeRow {
+    uint64_t word = 0;
+    const uint64_t* mask = nullptr;
+    const int* positions = nullptr;                 // of the request's rows; null without a window
+    int rows = 0, before = 0, position = 0, words = 0, window = 0;
+
+    __device__ __forceinline__ TreeRow() {}
+    __device__ __forceinline__ TreeRow(const AttentionKv8Call& p, const Kv8Request& q, int row) {
+        mask = p.masks + (size_t)(q.start + row) * p.words;
+        words = p.words;
+        rows = q.rows;
+        before = position = q.length - q.rows;
+        window = p.window;
+        if (ONE) word = *mask;
+        if (window) {
+            positions = p.batch.positions + q.start;
+            position = min(max(position, positions[row]), 1 << 30);
+        }
+    }
+    // A bit for each of the 16 keys from `at` on, of which those before the step's rows count from key at + `from`.
+    __device__ __forceinline__ uint32_t seen(int at, int from) const {
+        const int j = at - before;                  // the first as a row
+        uint32_t bits = 0xFFFF;
+        if (j > -16) {
+            uint64_t w;
+            if (ONE) {
+                w = j < 0 ? word << -j : j < 64 ? word >> j : 0;
+            } else if (j < 0) {
+                w = *mask << -j;
+            } else {
+                const int i = j >> 6, s = j & 63;
+                w = i < words ? mask[i] >> s : 0;
+                if (s > 48 && i + 1 < words) w |= mask[i + 1] << (64 - s);
+            }
+            if (j < 0) w |= (1u << -j) - 1;
+            const int left = rows - j;
+            bits = (uint32_t)w & (left >= 16 ? 0xFFFFu : left > 0 ? (1u << left) - 1 : 0u);
+            if (window)                             // (of a row its position counts, not its place)
+#pragma unroll 4
+                for (int k = max(-j, 0); k < min(16, left); ++k)
+                    if (positions[j + k] <= position - window) bits &= ~(1u << k);
+        }
+        const int hidden = min(from, -j);
+        return hidden <= 0 ? bits : hidden >= 16 ? 0 : bits >> hidden << hidden;
+    }
+};
 
 // How a batch's work is shared out.  A request's rows of a KV head make tiles of
 // `tile_rows`; a tile's steps are cut into equal parts of at most `per`, per
@@ -310,12 +377,20 @@ __device__ __forceinline__ int tiles_of(const Kv8Request& q, int group, const Sh
 struct Steps {
     int begin, end;
 };
+template <bool TREE>
 __device__ __forceinline__ Steps steps_of(const Kv8Request& q, int group, int window, int tile_rows, int tile) {
+    // (no row of a tree stands before its first, and a row may see any)
+    if (TREE) return Steps{window ? max(0, q.length - q.rows + 1 - window) / kStep : 0, (q.length - 1) / kStep + 1};
     const int r0 = tile * tile_rows, last = min(r0 + tile_rows, q.rows * group) - 1, before = q.length - q.rows;
     return Steps{window ? max(0, before + r0 / group + 1 - window) / kStep : 0, (before + last / group) / kStep + 1};
 }
 // No tile of a request has more.
+template <bool TREE>
 __device__ __forceinline__ int most_steps(const Kv8Request& q, int group, int window, int tile_rows) {
+    if (TREE) {
+        const Steps every = steps_of<true>(q, group, window, tile_rows, 0);
+        return every.end - every.begin;
+    }
     const int all = (q.length - 1) / kStep + 1;
     return window ? (int)min((long long)all, ((long long)window + tile_rows / group) / kStep + 3) : all;
 }
@@ -329,6 +404,7 @@ struct Item {
 // Which part of which tile of which request is item `index` (of one KV head);
 // request -1: none.  Every workgroup sums the whole batch, a request a thread.
 // The plan of a batch, for the merge, stands before the partial results: `per`, then each request's first slot.
+template <bool TREE>
 __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, const Share& share, int index, int& per) {
     const KvBatchView& b = p.batch;
     const int window = p.window;
@@ -336,7 +412,7 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
     __shared__ Item found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto steps = [&](const Kv8Request& q) {
-        return (float)tiles_of(q, group, share) * (float)most_steps(q, group, window, share.tile_rows);
+        return (float)tiles_of(q, group, share) * (float)most_steps<TREE>(q, group, window, share.tile_rows);
     };
     Kv8Request mine{0, 0, 0};
     float all = 0.0f;
@@ -358,7 +434,7 @@ __device__ __forceinline__ Item find_item(const AttentionKv8Call& p, int group, 
     for (int base = 0; base < b.requests; base += kThreads) {
         const int r = base + threadIdx.x;
         if (b.requests > kThreads) mine = r < b.requests ? kv8_request(b, r) : Kv8Request{0, 0, 0};
-        const int tiles = tiles_of(mine, group, share), parts = parts_of(most_steps(mine, group, window, share.tile_rows), per);
+        const int tiles = tiles_of(mine, group, share), parts = parts_of(most_steps<TREE>(mine, group, window, share.tile_rows), per);
         // (what a batch's rows allow is far below the limits; requests that claim the same rows may not reach into the other sum)
         const uint64_t items = tiles ? min((long long)tiles * parts, 1LL << 27) : 0;
         const uint64_t own = items << 24 | (parts > 1 ? min((uint32_t)items, 4095u) : 0);
@@ -408,21 +484,22 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 // dependent loads (its place, the query, the first table entries, the first codes); how
 // much of the rest is these starts and how much parts that end unevenly is not shown.
 // 8 requests of 16000 tokens take 57 us, 4.6 TB/s.
-template <int CC, bool FULL, bool E4M3>
+template <int CC, bool FULL, bool E4M3, bool TREE>
 __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item<TREE>(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, row = min(li, rows - 1);
     const int token = q.start + row / group, head = kvh * group + row % group;
-    const int position = q.length - q.rows + row / group;
-    const int low = q.length - q.rows;                             // of the first row
-    const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
+    const int low = q.length - q.rows;                             // position of the first row
+    const TreeRow<1> tree = TREE ? TreeRow<1>(p, q, row / group) : TreeRow<1>();
+    const int position = TREE ? tree.position : low + row / group;
+    const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, 0);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
     if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
@@ -485,15 +562,16 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
         v8h hi[2], lo[2];
         const KeyScales now = scales.checked();
         const int at = step * kStep + 16 * lq;                     // the lane's first key
-        if (step * kStep + kStep > low + 1 || p.window) {          // the wave's rows see different keys
+        if (step * kStep + kStep > low + !TREE || p.window) {      // the wave's rows see different keys
             const int from = p.window ? position + 1 - p.window - at : 0;
-            weigh<true>(acc, c, now, m, o, from, position + 1 - at, hi, lo);
+            if (TREE) weigh(acc, c, now, m, o, KeyBits{tree.seen(at, from)}, hi, lo);
+            else weigh(acc, c, now, m, o, KeyRange{from, position + 1 - at}, hi, lo);
             // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
             const int written = now.known ? q.length - at : 0;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) vr[t] = first_codes(vr[t], written);
         } else {
-            weigh<false>(acc, c, now, m, o, 0, 16, hi, lo);
+            weigh(acc, c, now, m, o, EveryKey{}, hi, lo);
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -538,7 +616,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
     if (li >= rows) return;
     const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    float scale = output_scale(lift, sum);
+    float scale = TREE ? part_scale(lift, sum) : output_scale(lift, sum);   // (a tree's row may see no key)
     if (parts > 1) {
         to = partial_values(p, share, slot) + (size_t)li * dim;
         scale = part_scale(lift, sum);
@@ -569,7 +647,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 // in its products while the other is in its softmax (62 and 143), gave nothing.
 constexpr int kTileRows = 16 * kWaves;
 
-template <int CC, bool FULL, bool E4M3>
+template <int CC, bool FULL, bool E4M3, bool TREE>
 __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
     constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
@@ -579,25 +657,27 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item<TREE>(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, w0 = item.tile * kTileRows + 16 * wave;   // the wave's first row
     const int before = q.length - q.rows;                          // position of the first row
-    const Steps seen = steps_of(q, group, p.window, kTileRows, item.tile);
+    const Steps seen = steps_of<TREE>(q, group, p.window, kTileRows, item.tile);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
     if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
     const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
-    const int position = before + row / group;
+    const TreeRow<0> tree = TREE ? TreeRow<0>(p, q, row / group) : TreeRow<0>();
+    const int position = TREE ? tree.position : before + row / group;
     v8h qh[CC][2], ql[CC][2];
     float c;
     load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
     // of the wave's rows: the first sees every key up to `low`, the last none after `high`
-    const int low = before + min(w0, rows - 1) / group;
-    const int high = w0 < rows ? before + min(w0 + 15, rows - 1) / group : -1;
+    // (of a tree's rows: any sees every key before the first's position, none one at or after the length)
+    const int low = TREE ? before : before + min(w0, rows - 1) / group;
+    const int high = w0 >= rows ? -1 : TREE ? q.length - 1 : before + min(w0 + 15, rows - 1) / group;
 
     // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
     v4u kr[CC], vr[CC];
@@ -669,11 +749,12 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
                 }
             v8h hi[2], lo[2];
             const int at = step * kStep + 16 * lq;
-            if (step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window)) {
+            if (step * kStep + kStep > low + !TREE || (p.window && step * kStep <= high - p.window)) {
                 const int from = p.window ? position + 1 - p.window - at : 0;
-                weigh<true>(acc, c, now, m, o, from, position + 1 - at, hi, lo);
+                if (TREE) weigh(acc, c, now, m, o, KeyBits{tree.seen(at, from)}, hi, lo);
+                else weigh(acc, c, now, m, o, KeyRange{from, position + 1 - at}, hi, lo);
             } else {
-                weigh<false>(acc, c, now, m, o, 0, 16, hi, lo);
+                weigh(acc, c, now, m, o, EveryKey{}, hi, lo);
             }
 #pragma unroll
             for (int t0 = 0; t0 < TILES; t0 += 4) {
@@ -698,7 +779,7 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const float sum = add_xor32(add_xor16(m.sum));
     if (w0 + li >= rows) return;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    float scale = output_scale(m.lift, sum);
+    float scale = TREE ? part_scale(m.lift, sum) : output_scale(m.lift, sum);
     if (parts > 1) {
         const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
         to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
@@ -723,13 +804,14 @@ __device__ __forceinline__ float part_share(v2f part, float base, float inverse)
 
 // ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
 // values of one part at a time
+template <bool TREE>
 __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(AttentionKv8Call p, Share share) {
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
     const int request = blockIdx.x, kvh = blockIdx.y;
     const Kv8Request q = kv8_request(p.batch, request);
     if (!tiles_of(q, group, share)) return;
     const int* plan = (const int*)p.partial + share.at;
-    const Steps seen = steps_of(q, group, p.window, share.tile_rows, 0);
+    const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, 0);
     const int parts = parts_of(seen.end - seen.begin, plan[0]), item = plan[kHeader + request];
     // (requests that claim the same rows can have more parts than there is room for: such rows stay undefined)
     if (parts == 1 || item < 0 || item > share.slots - parts) return;
@@ -744,7 +826,8 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
         for (int i = lane; i < parts; i += 64) add_part(sums[i * sum_stride], base, total);
         const float own_base = base;
         base = wave_max_f32(base);
-        const float inverse = 1.0f / wave_sum_f32(total * __builtin_amdgcn_exp2f(own_base - base));
+        total = wave_sum_f32(total * __builtin_amdgcn_exp2f(own_base - base));
+        const float inverse = TREE && total == 0.0f ? 0.0f : 1.0f / total;
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (own < abreast) {
 #pragma unroll 4
@@ -766,6 +849,7 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
 
 // ---- the same of more rows: some workgroups a tile, a thread for four values of a row
 constexpr int kMergeSplit = 4;                      // workgroups of a tile (2 / 4 / 8: a chunk beside decoding requests 45 / 44 / 48 us)
+template <bool TREE>
 __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(AttentionKv8Call p, Share share) {
     __shared__ int sums_of[kWaves], found[5];
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -806,9 +890,9 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     const Kv8Request q{found[2], found[3], found[4]};
     const int* plan = (const int*)p.partial + share.at;
     const int per = plan[0], first = plan[kHeader + request];
-    const Steps seen = steps_of(q, group, p.window, share.tile_rows, tile);
+    const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, tile);
     const int parts = parts_of(seen.end - seen.begin, per);
-    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps(q, group, p.window, share.tile_rows), per);
+    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps<TREE>(q, group, p.window, share.tile_rows), per);
     if (parts == 1 || item < 0 || item > share.slots - parts) return;
     const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
     const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
@@ -821,7 +905,7 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) add_part(sums[i * sum_stride], base, total);
-        const float inverse = 1.0f / total;
+        const float inverse = TREE && total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) {
             const float share_of = part_share(sums[i * sum_stride], base, inverse);
@@ -897,15 +981,15 @@ Shares shares_of(const AttentionKv8Call& call) {
     return s;
 }
 
-template <int CC, bool FULL, bool E4M3>
+template <int CC, bool FULL, bool E4M3, bool TREE>
 void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
     const int grid = share.items * call.cache.kv_heads;
     if (share.tile_rows == kFewRows) {
-        attention_kv8_few_kernel<CC, FULL, E4M3><<<grid, kThreads, 0, stream>>>(call, share);
+        attention_kv8_few_kernel<CC, FULL, E4M3, TREE><<<grid, kThreads, 0, stream>>>(call, share);
         return;
     }
     constexpr int kLds = 2 * 16 * CC * 1024;
-    constexpr auto kernel = attention_kv8_rows_kernel<CC, FULL, E4M3>;
+    constexpr auto kernel = attention_kv8_rows_kernel<CC, FULL, E4M3, TREE>;
     if (kLds >= 65536) {                            // more than the default, with the static arrays: allowed once a device
         static std::atomic<uint64_t> allowed{0};
         int device = 0;
@@ -917,40 +1001,46 @@ void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream
     kernel<<<grid, kThreads, kLds, stream>>>(call, share);
 }
 
-template <int CC, bool FULL>
+template <int CC, bool FULL, bool TREE>
 void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream) {
-    if (call.cache.e4m3) launch<CC, FULL, true>(call, share, stream);
-    else launch<CC, FULL, false>(call, share, stream);
+    if (call.cache.e4m3) launch<CC, FULL, true, TREE>(call, share, stream);
+    else launch<CC, FULL, false, TREE>(call, share, stream);
 }
 
 }  // namespace
 
 size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call) { return 4 * shares_of(call).floats; }
 
-void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
+template <bool TREE>
+static void launch_attention(const AttentionKv8Call& call, hipStream_t stream) {
     const int dim = call.cache.dim, group = call.heads / call.cache.kv_heads;
     const Shares shares = shares_of(call);
     for (const Share& share : {shares.few, shares.many}) {
         if (!share.items) continue;
         switch ((dim + 63) / 64 * 2 + (dim % 64 == 0)) {
-        case 2: launch<1, false>(call, share, stream); break;
-        case 3: launch<1, true>(call, share, stream); break;
-        case 4: launch<2, false>(call, share, stream); break;
-        case 5: launch<2, true>(call, share, stream); break;
-        case 6: launch<3, false>(call, share, stream); break;
-        case 7: launch<3, true>(call, share, stream); break;
-        case 8: launch<4, false>(call, share, stream); break;
-        default: launch<4, true>(call, share, stream); break;
+        case 2: launch<1, false, TREE>(call, share, stream); break;
+        case 3: launch<1, true, TREE>(call, share, stream); break;
+        case 4: launch<2, false, TREE>(call, share, stream); break;
+        case 5: launch<2, true, TREE>(call, share, stream); break;
+        case 6: launch<3, false, TREE>(call, share, stream); break;
+        case 7: launch<3, true, TREE>(call, share, stream); break;
+        case 8: launch<4, false, TREE>(call, share, stream); break;
+        default: launch<4, true, TREE>(call, share, stream); break;
         }
     }
     // (no tile is parted that has no more steps than a part at least)
     const size_t steps = ((size_t)call.batch.width << call.batch.block_shift) / kStep + 1;
     if (shares.few.items && steps > (size_t)kFewLeast)
-        attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
+        attention_kv8_few_merge_kernel<TREE><<<dim3(call.batch.requests, call.cache.kv_heads),
                                          64 * (int)std::min<int64_t>(kFewRows, (int64_t)group * call.batch.max_rows), 0, stream>>>(call, shares.few);
     if (shares.many.items && steps > (size_t)kRowsLeast)
-        attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
+        attention_kv8_rows_merge_kernel<TREE><<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
             call, shares.many);
+}
+
+void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
+    if (call.masks) launch_attention<true>(call, stream);
+    else launch_attention<false>(call, stream);
 }
 
 }  // namespace leafhip

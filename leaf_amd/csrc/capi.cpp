@@ -348,6 +348,53 @@ leafhip::AttentionKv8Call attention_kv8_call(const lh_kv_batch* batch, const lh_
     return a;
 }
 
+// A batch whose requests have at most LH_KV_TREE_ROWS rows each.
+leafhip::KvBatchView tree_view_of(const lh_kv_batch* b) {
+    const leafhip::KvBatchView v = view_of(b);
+    require_arg(b->max_rows <= LH_KV_TREE_ROWS, "max_rows of a step of trees must be 1..512");
+    return v;
+}
+static_assert(leafhip::kTreeRows == LH_KV_TREE_ROWS, "rows of a tree");
+int mask_words(const lh_kv_batch* b) { return int((b->max_rows + 63) / 64); }
+
+// Attention of a batch, causal or (with masks) of trees.
+void run_attention_kv8(leafhip::AttentionKv8Call a, const lh_kv8* cache, const float* q_heads, float* out, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream) {
+    require_arg(a.batch.table && a.batch.lengths && a.batch.starts && a.batch.rows && q_heads && out,
+                "invalid attention call");
+    require_arg(aligned16(q_heads) && aligned16(out) && aligned16(workspace),
+                "attention arrays and workspace must be 16-byte aligned");
+    a.q_heads = q_heads;
+    a.out = out;
+    a.scale = 1.0f / std::sqrt(static_cast<float>(cache->dim));
+    const size_t bytes = leafhip::attention_kv8_workspace_bytes(a);
+    std::optional<ScratchUse> scratch;
+    if (workspace) {
+        require_arg(workspace_bytes >= bytes, "attention workspace is too small (lh_attention_kv8_workspace)");
+        a.partial = static_cast<float*>(workspace);
+    } else if (bytes) {
+        scratch.emplace(stream);
+        a.partial = static_cast<float*>(scratch->work(bytes));
+    }
+    leafhip::launch_attention_kv8(a, stream);
+    leafhip::hip_check(hipGetLastError(), "attention launch");
+}
+
+leafhip::VerifyCall verify_call(const lh_kv_batch* batch, const lh_drafts* drafts, bool pointers) {
+    leafhip::VerifyCall v;
+    v.batch = tree_view_of(batch);
+    require_arg(drafts != nullptr, "drafts are null");
+    require_arg(drafts->vocab >= 1 && drafts->vocab <= 0x7fffffff - 65536, "vocabulary is empty or too large");
+    require_arg(!pointers || (drafts->logits && drafts->ids && drafts->parents && drafts->temperatures && drafts->accept &&
+                              drafts->sample && drafts->path && drafts->kept && drafts->next),
+                "verification needs all arrays but the draft's logits");
+    v.vocab = int(drafts->vocab);
+    v.logits = drafts->logits; v.draft = drafts->draft_logits; v.temperatures = drafts->temperatures;
+    v.accept = drafts->accept; v.sample = drafts->sample; v.ids = drafts->ids; v.parents = drafts->parents;
+    v.path = drafts->path; v.kept = drafts->kept; v.next = drafts->next;
+    return v;
+}
+
 lh_status linear_impl(const lh_weight* weight, const float* x, const int8_t* q, const float* qs, size_t tokens,
                       uint32_t activation_bits, float* y, int32_t* acc, lh_stream stream, int force_path,
                       unsigned required_bits, bool no_alloc = false) {
@@ -985,25 +1032,97 @@ lh_status lh_attention_kv8(const lh_kv_batch* batch, const lh_kv8* cache, const 
                            uint32_t window, float* out, void* workspace, size_t workspace_bytes, lh_stream stream) {
     return guarded([&] {
         leafhip::AttentionKv8Call a = attention_kv8_call(batch, cache, heads, true);
-        require_arg(a.batch.table && a.batch.lengths && a.batch.starts && a.batch.rows && q_heads && out,
-                    "invalid attention call");
-        require_arg(aligned16(q_heads) && aligned16(out) && aligned16(workspace),
-                    "attention arrays and workspace must be 16-byte aligned");
-        a.q_heads = q_heads;
-        a.out = out;
         a.window = int(std::min<uint32_t>(window, 0x7fffffff));
-        a.scale = 1.0f / std::sqrt(static_cast<float>(cache->dim));
-        const size_t bytes = leafhip::attention_kv8_workspace_bytes(a);
+        run_attention_kv8(a, cache, q_heads, out, workspace, workspace_bytes, as_stream(stream));
+    });
+}
+
+lh_status lh_kv_tree(const lh_kv_batch* batch, const int32_t* parents, uint64_t* masks, lh_stream stream) {
+    return guarded([&] {
+        leafhip::KvTreeCall t;
+        t.batch = tree_view_of(batch);
+        require_arg(t.batch.lengths && t.batch.starts && t.batch.rows && t.batch.positions && parents && masks, "invalid tree call");
+        t.parents = parents;
+        t.masks = masks;
+        t.words = mask_words(batch);
+        leafhip::launch_kv_tree(t, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "tree launch");
+    });
+}
+lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,
+                                uint32_t window, const uint64_t* masks, float* out, void* workspace, size_t workspace_bytes,
+                                lh_stream stream) {
+    return guarded([&] {
+        leafhip::AttentionKv8Call a = attention_kv8_call(batch, cache, heads, true);
+        tree_view_of(batch);
+        require_arg(masks && (!window || a.batch.positions), "attention of trees needs masks, and with a window positions");
+        a.masks = masks;
+        a.words = mask_words(batch);
+        a.window = int(std::min<uint32_t>(window, 1u << 30));      // (a request has no more keys)
+        run_attention_kv8(a, cache, q_heads, out, workspace, workspace_bytes, as_stream(stream));
+    });
+}
+lh_status lh_verify_drafts_workspace(const lh_kv_batch* batch, const lh_drafts* drafts, size_t* bytes) {
+    return guarded([&] {
+        require_arg(bytes != nullptr, "output pointer is null");
+        *bytes = leafhip::verify_workspace_bytes(verify_call(batch, drafts, false));
+    });
+}
+lh_status lh_verify_drafts(const lh_kv_batch* batch, const lh_drafts* drafts, void* workspace, size_t workspace_bytes,
+                           lh_stream stream) {
+    return guarded([&] {
+        leafhip::VerifyCall v = verify_call(batch, drafts, true);
+        require_arg(v.batch.starts && v.batch.rows, "verification needs the batch's starts and rows");
+        require_arg(aligned16(workspace), "verification workspace must be 16-byte aligned");
+        const size_t bytes = leafhip::verify_workspace_bytes(v);
         std::optional<ScratchUse> scratch;
         if (workspace) {
-            require_arg(workspace_bytes >= bytes, "attention workspace is too small (lh_attention_kv8_workspace)");
-            a.partial = static_cast<float*>(workspace);
+            require_arg(workspace_bytes >= bytes, "verification workspace is too small (lh_verify_drafts_workspace)");
+            v.workspace = workspace;
         } else if (bytes) {
             scratch.emplace(as_stream(stream));
-            a.partial = static_cast<float*>(scratch->work(bytes));
+            v.workspace = scratch->work(bytes);
         }
-        leafhip::launch_attention_kv8(a, as_stream(stream));
-        leafhip::hip_check(hipGetLastError(), "attention launch");
+        leafhip::launch_verify(v, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "verification launch");
+    });
+}
+lh_status lh_kv8_compact(const lh_kv_batch* batch, const lh_kv8* caches, uint32_t layers, const int32_t* path,
+                         const int32_t* kept, lh_stream stream) {
+    return guarded([&] {
+        leafhip::Kv8CompactCall c;
+        c.batch = tree_view_of(batch);
+        require_arg(c.batch.table && c.batch.lengths && c.batch.starts && c.batch.rows && path && kept, "invalid compaction call");
+        require_arg(caches && layers >= 1 && layers <= 65535, "compaction needs the caches of 1..65535 layers");
+        c.path = path;
+        c.kept = kept;
+        for (uint32_t i = 0; i < layers; ++i) {
+            view_of(&caches[i]);
+            require_arg(caches[i].kv_heads == caches[0].kv_heads && caches[i].dim == caches[0].dim &&
+                            caches[i].format == caches[0].format, "layers of a compaction must have the same heads, dim and format");
+        }
+        for (uint32_t first = 0; first < layers; first += leafhip::kCompactLayers) {
+            const uint32_t count = std::min<uint32_t>(layers - first, leafhip::kCompactLayers);
+            for (uint32_t i = 0; i < count; ++i) {
+                const leafhip::Kv8View v = view_of(&caches[first + i]);
+                c.kv_heads = v.kv_heads; c.dim = v.dim; c.e4m3 = v.e4m3;
+                c.layers[i] = leafhip::Kv8Layer{v.keys, v.values, v.key_scales, v.value_scales};
+            }
+            leafhip::launch_kv8_compact(c, int(count), as_stream(stream));
+            leafhip::hip_check(hipGetLastError(), "compaction launch");
+        }
+    });
+}
+lh_status lh_kv_keep(const lh_kv_batch* batch, const int32_t* kept, int32_t* lengths, lh_stream stream) {
+    return guarded([&] {
+        leafhip::KvKeepCall k;
+        k.batch = view_of(batch);
+        require_arg(k.batch.table && k.batch.lengths && k.batch.rows && k.batch.free_blocks && k.batch.free_count &&
+                        k.batch.free_left && kept && lengths, "invalid keep call");
+        k.kept = kept;
+        k.lengths = lengths;
+        leafhip::launch_kv_keep(k, as_stream(stream));
+        leafhip::hip_check(hipGetLastError(), "keep launch");
     });
 }
 

@@ -280,8 +280,48 @@ struct AttentionKv8Call {
     int heads = 0, window = 0;
     float scale = 1.0f;             // of q.k: 1 / sqrt(dim)
     float* partial = nullptr;       // attention_kv8_workspace_bytes(call) bytes
+    const uint64_t* masks = nullptr;   // of a tree's rows (lh_kv_tree): [tokens][words]; null: causal
+    int words = 0;
 };
 size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call);
 void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream);
+
+// ---- drafted trees over that cache (include/leafhip.h: lh_kv_tree to lh_kv_keep)
+constexpr int kTreeRows = 512;      // of a request: LH_KV_TREE_ROWS
+struct KvTreeCall {
+    KvBatchView batch;
+    const int* parents = nullptr;
+    uint64_t* masks = nullptr;      // [tokens][words]
+    int words = 0;
+};
+void launch_kv_tree(const KvTreeCall& call, hipStream_t stream);
+struct VerifyCall {
+    KvBatchView batch;
+    int vocab = 0;
+    const float *logits = nullptr, *draft = nullptr, *temperatures = nullptr, *accept = nullptr, *sample = nullptr;
+    const int *ids = nullptr, *parents = nullptr;
+    int *path = nullptr, *kept = nullptr, *next = nullptr;
+    void* workspace = nullptr;      // verify_workspace_bytes(call) bytes
+};
+size_t verify_workspace_bytes(const VerifyCall& call);
+void launch_verify(const VerifyCall& call, hipStream_t stream);
+struct Kv8Layer {
+    uint8_t *keys, *values;
+    float *key_scales, *value_scales;
+};
+constexpr int kCompactLayers = 32;  // of one launch
+struct Kv8CompactCall {
+    KvBatchView batch;
+    const int *path = nullptr, *kept = nullptr;
+    int kv_heads = 0, dim = 0, e4m3 = 0;
+    Kv8Layer layers[kCompactLayers];
+};
+void launch_kv8_compact(const Kv8CompactCall& call, int layers, hipStream_t stream);
+struct KvKeepCall {
+    KvBatchView batch;
+    const int* kept = nullptr;
+    int* lengths = nullptr;
+};
+void launch_kv_keep(const KvKeepCall& call, hipStream_t stream);
 
 }  // namespace leafhip

@@ -73,6 +73,13 @@ class Kv8(C.Structure):
 
 KV8_FORMATS = {"int8": 0, "e4m3": 1}
 
+
+class Drafts(C.Structure):
+    """lh_drafts: what verification reads and writes (addresses on the device; draft_logits may be None)."""
+    _fields_ = [("vocab", C.c_uint32)] + [(name, C.c_void_p) for name in (
+        "logits", "draft_logits", "ids", "parents", "temperatures", "accept", "sample", "path", "kept", "next")]
+
+
 _lib = None
 _exiting = False
 
@@ -146,6 +153,12 @@ def library(path: Path | None = None) -> C.CDLL:
         "lh_rope_kv8": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, sz, vp, vp], i32),
         "lh_attention_kv8": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, sz, vp], i32),
         "lh_attention_kv8_workspace": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, C.POINTER(sz)], i32),
+        "lh_kv_tree": ([C.POINTER(KvBatch), vp, vp, vp], i32),
+        "lh_attention_kv8_tree": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, vp, sz, vp], i32),
+        "lh_verify_drafts": ([C.POINTER(KvBatch), C.POINTER(Drafts), vp, sz, vp], i32),
+        "lh_verify_drafts_workspace": ([C.POINTER(KvBatch), C.POINTER(Drafts), C.POINTER(sz)], i32),
+        "lh_kv8_compact": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, vp, vp, vp], i32),
+        "lh_kv_keep": ([C.POINTER(KvBatch), vp, vp, vp], i32),
         "lh_silu_gate": ([vp, sz, sz, vp, vp], i32),
         "lh_activation": ([vp, sz, u32, vp, vp], i32),
         "lh_argmax": ([vp, sz, sz, vp, vp], i32),
@@ -470,6 +483,40 @@ def attention_kv8_workspace(batch: KvBatch, cache: Kv8, heads: int) -> int:
     n = C.c_size_t()
     check(library().lh_attention_kv8_workspace(C.byref(batch), C.byref(cache), heads, C.byref(n)))
     return n.value
+
+
+def kv_tree(batch: KvBatch, parents: DeviceArray, masks: DeviceArray, stream=None) -> None:
+    """Positions and ancestor masks [tokens, (max_rows + 63) // 64] (uint64) of a step's trees."""
+    check(library().lh_kv_tree(C.byref(batch), parents.ptr, masks.ptr, stream))
+
+
+def attention_kv8_tree(batch: KvBatch, cache: Kv8, q_heads: DeviceArray, heads: int, masks: DeviceArray, out: DeviceArray,
+                       window: int = 0, workspace: DeviceArray | None = None, stream=None) -> None:
+    check(library().lh_attention_kv8_tree(C.byref(batch), C.byref(cache), q_heads.ptr, heads, window, masks.ptr, out.ptr,
+                                          workspace.ptr if workspace is not None else None,
+                                          workspace.nbytes if workspace is not None else 0, stream))
+
+
+def verify_drafts(batch: KvBatch, drafts: Drafts, workspace: DeviceArray | None = None, stream=None) -> None:
+    check(library().lh_verify_drafts(C.byref(batch), C.byref(drafts), workspace.ptr if workspace is not None else None,
+                                     workspace.nbytes if workspace is not None else 0, stream))
+
+
+def verify_drafts_workspace(batch: KvBatch, drafts: Drafts) -> int:
+    n = C.c_size_t()
+    check(library().lh_verify_drafts_workspace(C.byref(batch), C.byref(drafts), C.byref(n)))
+    return n.value
+
+
+def kv8_compact(batch: KvBatch, caches, path: DeviceArray, kept: DeviceArray, stream=None) -> None:
+    """The rows that stand moved together in every cache of `caches` (Kv8 descriptions of a model's layers)."""
+    array = (Kv8 * len(caches))(*caches)
+    check(library().lh_kv8_compact(C.byref(batch), array, len(caches), path.ptr, kept.ptr, stream))
+
+
+def kv_keep(batch: KvBatch, kept: DeviceArray, lengths: DeviceArray | None = None, stream=None) -> None:
+    """Lengths (default: the batch's own) and free blocks after a step of which kept rows stand."""
+    check(library().lh_kv_keep(C.byref(batch), kept.ptr, lengths.ptr if lengths is not None else batch.lengths, stream))
 
 
 class Stream:
