@@ -384,7 +384,7 @@ leafhip::VerifyCall verify_call(const lh_kv_batch* batch, const lh_drafts* draft
     leafhip::VerifyCall v;
     v.batch = tree_view_of(batch);
     require_arg(drafts != nullptr, "drafts are null");
-    require_arg(drafts->vocab >= 1 && drafts->vocab <= 0x7fffffff - 65536, "vocabulary is empty or too large");
+    require_arg(drafts->vocab >= 1 && drafts->vocab <= 1u << 30, "vocabulary is empty or too large");
     require_arg(!pointers || (drafts->logits && drafts->ids && drafts->parents && drafts->temperatures && drafts->accept &&
                               drafts->sample && drafts->path && drafts->kept && drafts->next),
                 "verification needs all arrays but the draft's logits");

@@ -13,237 +13,502 @@
 // sums in order pass u times all, and among 10^5 tokens an f32 sum would often be
 // on the other side of it.
 //
-// A workgroup walks a request's tree and reads only the rows on its way.  Each
-// wave has a contiguous share of the vocabulary: the shares' sums say where the
-// last token is, and its share alone is read again.
+// Only the rows on a walk's way are read, and a walk's rows come one after the
+// other.  Several workgroups share a request: each has a segment of the
+// vocabulary, and all of them walk.  What a walk needs of the whole vocabulary (a row's largest value and sums, the sum of
+// what a refusal has left) they exchange through slots in memory, one for each
+// segment and exchange of the walk, each word of which tells by itself whether it
+// has been written.  A workgroup that does not find another's words in time (it
+// may not have started) computes them itself: the same operations on the same
+// values give the same words, and no workgroup depends on another's progress.
+#include <algorithm>
+#include <cfloat>
+#include <cstdlib>
+
 #include "kv8.h"
 
 namespace leafhip {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBatch = 16;                          // values that a thread has in flight
-constexpr int kTable = 64;                          // powers of two of a step
+constexpr int kMostSegments = 128;
+constexpr int kWords = 3;                           // of a slot
+constexpr int kBatch = 4;                           // values of a row that a thread has in flight
+constexpr int kTable = 256;                         // powers of two of a step
+constexpr uint64_t kEmpty = ~0ull;                  // a word that is not written: no value's bits (NaN is stored as kNaN)
+constexpr uint32_t kNaN = 0x7fc00000u;
 
-// 2^y for y <= 0 (0 below 2^-1000), to 1e-15: table[j] = 2^(j / 64), 2^f by its series for |f| <= 1/128.
+// 2^y for y <= 0 (0 below 2^-1000), to 1.5e-13: table[j] = 2^(j / 256), 2^f by its series for |f| <= 1/512.
 __device__ __forceinline__ double power(double y, const double* table) {
-    const double shift = 6755399441055744.0 / kTable;              // 1.5 * 2^52 / 64: the sum's last bit is 1/64
-    const double t = fmax(y, -1000.0) + shift, f = fmax(y, -1000.0) - (t - shift);
-    const int n = __double2loint(t);                               // 64 y to the nearest
-    double s = 1.3333558146428443e-3;                              // ln2^k / k!
-    s = fma(s, f, 9.618129107628477e-3);
-    s = fma(s, f, 5.550410866482158e-2);
+    const double shift = 6755399441055744.0 / kTable;              // 1.5 * 2^52 / 256: the sum's last bit is 1/256
+    const double t = y + shift, f = y - (t - shift);
+    const int n = __double2loint(t);                               // 256 y to the nearest
+    double s = 5.550410866482158e-2;                               // ln2^k / k!
     s = fma(s, f, 2.402265069591007e-1);
     s = fma(s, f, 6.931471805599453e-1);
     s = fma(s, f, 1.0);
     s *= table[n & (kTable - 1)];
-    const double p = __hiloint2double(__double2hiint(s) + ((n >> 6) << 20), __double2loint(s));
+    const double p = __hiloint2double(__double2hiint(s) + ((n >> 8) << 20), __double2loint(s));
     return y < -1000.0 ? 0.0 : p;
 }
 
-// A row of logits in weights.
-struct Row {
-    const float* logits;
-    float most;
-    double total;                                   // the sum of its weights
-};
+// Reductions over a wave without the LDS: rotations in rows of 16 lanes, then swaps of rows.  Every lane gets the result.
+template <int N>
+__device__ __forceinline__ uint32_t rotated16(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + N, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float all_max(float x) {
+    x = fmaxf(x, __uint_as_float(rotated16<8>(__float_as_uint(x))));
+    x = fmaxf(x, __uint_as_float(rotated16<4>(__float_as_uint(x))));
+    x = fmaxf(x, __uint_as_float(rotated16<2>(__float_as_uint(x))));
+    x = fmaxf(x, __uint_as_float(rotated16<1>(__float_as_uint(x))));
+    return max_xor32(max_xor16(x));
+}
+__device__ __forceinline__ int all_min(int x) {
+    x = min(x, (int)rotated16<8>((uint32_t)x));
+    x = min(x, (int)rotated16<4>((uint32_t)x));
+    x = min(x, (int)rotated16<2>((uint32_t)x));
+    x = min(x, (int)rotated16<1>((uint32_t)x));
+    auto p = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = min((int)p[0], (int)p[1]);
+    p = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    return min((int)p[0], (int)p[1]);
+}
+template <int N>
+__device__ __forceinline__ double add_rotated16(double x) {
+    return x + __hiloint2double((int)rotated16<N>((uint32_t)__double2hiint(x)), (int)rotated16<N>((uint32_t)__double2loint(x)));
+}
+__device__ __forceinline__ double all_sum(double x) {
+    x = add_rotated16<1>(add_rotated16<2>(add_rotated16<4>(add_rotated16<8>(x))));
+    auto h = __builtin_amdgcn_permlane16_swap((uint32_t)__double2hiint(x), (uint32_t)__double2hiint(x), false, false);
+    auto l = __builtin_amdgcn_permlane16_swap((uint32_t)__double2loint(x), (uint32_t)__double2loint(x), false, false);
+    x = __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
+    h = __builtin_amdgcn_permlane32_swap((uint32_t)__double2hiint(x), (uint32_t)__double2hiint(x), false, false);
+    l = __builtin_amdgcn_permlane32_swap((uint32_t)__double2loint(x), (uint32_t)__double2loint(x), false, false);
+    return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
+}
 
 struct Shared {
     double table[kTable];
-    double sums[kWaves];                            // of each share: of what is left,
-    double whole[kWaves];                           // of the target's weights
-    double scan[kWaves];
-    float tops[kWaves];
+    uint64_t words[kWords][kMostSegments];          // of an exchange
+    double whole[kMostSegments], left[kMostSegments];   // of each segment: the sum of the target's weights, and of what is left
+    double sums[2][kWaves];                         // of each wave's share of the segment in hand
+    float tops[2][kWaves];
     int where[kWaves];
     int parents[kTreeRows], ids[kTreeRows], refused[kTreeRows];
     float accept[kTreeRows];
     int found;
 };
 
-// What the walk is at: the target's row, the draft's, and what refusals have left.
-struct State {
-    Row target, draft;
-    bool bad;                                       // no distribution
-    int best;                                       // greedy: the first largest
-    double scale;                                   // K; 0: nothing refused
-    double used;                                    // C
-    double left;                                    // the sum of r
-    int refusals;                                   // tokens in `refused`
+struct How {
+    int segments, size;                             // of the vocabulary, and values of one: a multiple of kWaves
+    long long wait;                                 // cycles until a workgroup computes what others owe
 };
 
-__device__ __forceinline__ double weight(const Row& row, int x, double c, const double* table) {
-    return power(((double)row.logits[x] - (double)row.most) * c, table);
-}
-
-// The sum of v over the workgroup's waves, each wave's in `sums` too.
-__device__ __forceinline__ double sum_shares(double v, double* sums) {
-    v = wave_sum_f64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double all = 0.0;
-    for (int w = 0; w < kWaves; ++w) all += sums[w];
-    return all;
-}
-
+// One walk, by one of its workgroups.  Every workgroup of a request holds the same values here.
 struct Walk {
     const VerifyCall& p;
     Shared& s;
+    const How& how;
+    uint64_t* slots;                                // the walk's: [exchange][segment][kWords]
+    int own, start;
     double c;                                       // log2(e) / T
-    int share;                                      // values of a wave's share
+    bool greedy;
 
-    __device__ __forceinline__ int begin(int wave) const { return min(wave * share, p.vocab); }
+    int exchange = 0;                               // the next one
+    // of the row that the walk is at
+    const float *target = nullptr, *drafted = nullptr;   // drafted: null where no child is tried against it
+    float most_w = 0.0f, most_v = 0.0f;             // m
+    double total_w = 0.0, total_v = 0.0;            // Z, Y
+    int best = 0;                                   // greedy: the first largest
+    double scale = 0.0, used = 0.0, left = 0.0;     // K, C and the sum of r
+    int refusals = 0;
 
-    // A row's largest value, its first place, and the sum of its weights (each share's in `sums`); false: no distribution.
-    __device__ bool measure(Row& row, int& best, bool greedy, double* sums) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, end = begin(wave + 1);
-        float most = -INFINITY;
-        int at = p.vocab;
-        double sum = 0.0;
-        bool wrong = false;
-        for (int base = begin(wave) + lane; base < end; base += 64 * kBatch) {
-            float l[kBatch], top = -INFINITY;
+    __device__ __forceinline__ Walk(const VerifyCall& p_, Shared& s_, const How& how_, uint64_t* slots_, int own_, int start_, float temperature)
+        : p(p_), s(s_), how(how_), slots(slots_), own(own_), start(start_), c(1.4426950408889634 / (double)temperature),
+          greedy(temperature == 0.0f) {}
+
+    __device__ __forceinline__ double weight(float l, float most) const { return power(((double)l - (double)most) * c, s.table); }
+
+    // A wave's share of a segment.
+    __device__ __forceinline__ int share_begin(int segment, int wave) const { return min(segment * how.size + how.size / kWaves * wave, p.vocab); }
+
+    // A wave's share of a segment, some values at a time, the next ones under way meanwhile: use(values of the row, of
+    // the draft's, the first one's place and the share's end, behind which values are minus infinity).
+    template <bool BOTH, int BATCH, typename Use>
+    __device__ __forceinline__ void stream(int segment, Use use) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, end = share_begin(segment, wave + 1);
+        int base = share_begin(segment, wave) + lane;
+        float l[BATCH], d[BATCH], nl[BATCH], nd[BATCH];
+        auto load = [&](int from, float (&a)[BATCH], float (&b)[BATCH]) {
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) l[i] = base + 64 * i < end ? row.logits[base + 64 * i] : -INFINITY;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                wrong = wrong || !(l[i] < INFINITY);
-                top = fmaxf(top, l[i]);
+            for (int i = 0; i < BATCH; ++i) {
+                const int x = min(from + 64 * i, p.vocab - 1);
+                a[i] = target[x];
+                if (BOTH) b[i] = drafted[x];
             }
-            if (greedy) {
-                if (top > most) {
+        };
+        load(base, l, d);
+        for (; base - lane < end; base += 64 * BATCH) {
+            load(base + 64 * BATCH, nl, nd);
 #pragma unroll
-                    for (int i = kBatch - 1; i >= 0; --i)
-                        if (l[i] == top) at = base + 64 * i;
-                    most = top;
-                }
-                continue;
-            }
-            if (top > most) {
-                if (most > -INFINITY) sum *= power(((double)most - (double)top) * c, s.table);
-                most = top;
-            }
-            if (most == -INFINITY) continue;
+            for (int i = 0; i < BATCH; ++i)
+                if (base + 64 * i >= end) l[i] = d[i] = -INFINITY;
+            use(l, d, base);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) sum += l[i] > -INFINITY ? power(((double)l[i] - (double)most) * c, s.table) : 0.0;
+            for (int i = 0; i < BATCH; ++i) {
+                l[i] = nl[i];
+                d[i] = nd[i];
+            }
         }
-        float top = wave_max_f32(most);
-        int place = most == top ? at : p.vocab;
-        for (int o = 32; o > 0; o >>= 1) place = min(place, __shfl_xor(place, o, 64));
-        if (lane == 0) {
-            s.tops[wave] = top;
-            s.where[wave] = place;
-        }
-        wrong = __syncthreads_or(wrong);
-        top = s.tops[0];
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s.tops[w]);
-        best = p.vocab;
-        for (int w = kWaves - 1; w >= 0; --w)
-            if (s.tops[w] == top) best = s.where[w];
-        row.most = top;
-        if (wrong || top == -INFINITY) return false;
-        if (greedy) {
-            __syncthreads();
-            return true;
-        }
-        if (most > -INFINITY) sum *= power(((double)most - (double)top) * c, s.table);
-        row.total = sum_shares(sum, sums);
-        return true;
     }
 
-    // What is left of value x.
-    __device__ __forceinline__ double left_of(const State& z, int x) const {
-        double r = weight(z.target, x, c, s.table);
-        if (z.scale > 0.0) r = fmax(r - z.scale * weight(z.draft, x, c, s.table), 0.0);
-        for (int i = 0; i < z.refusals; ++i)
+    // A lane's largest value so far, and the sum of its weights relative to that.
+    struct Part {
+        float most = -FLT_MAX;
+        double sum = 0.0;
+        bool wrong = false;
+    };
+    __device__ __forceinline__ void add(const float (&l)[kBatch], Part& part) const {
+        float top = l[0];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            part.wrong = part.wrong || !(l[i] < INFINITY);
+            top = fmaxf(top, l[i]);
+        }
+        if (__any(top > part.most)) {
+            const float higher = fmaxf(top, part.most);
+            part.sum *= weight(part.most, higher);
+            part.most = higher;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) part.sum += weight(l[i], part.most);
+    }
+
+    // The words of a segment's slot: largest values (at least -FLT_MAX), and sums of the weights relative to them (in
+    // `sums` those of each wave's share).
+    __device__ __forceinline__ void measure(int segment, uint64_t (&out)[kWords]) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const bool draft = drafted != nullptr;
+        Part a_w, a_v;
+        int at = p.vocab;
+        float top_w, top_v = -FLT_MAX;
+        double sum_w = 0.0, sum_v = 0.0;
+        if (greedy) {
+            a_w.most = -INFINITY;
+            stream<false, 2 * kBatch>(segment, [&](const float (&l)[2 * kBatch], const float (&)[2 * kBatch], int base) {
+#pragma unroll
+                for (int i = 0; i < 2 * kBatch; ++i) {
+                    a_w.wrong = a_w.wrong || !(l[i] < INFINITY);
+                    if (l[i] > a_w.most) {
+                        a_w.most = l[i];
+                        at = base + 64 * i;
+                    }
+                }
+            });
+            top_w = all_max(a_w.wrong ? INFINITY : a_w.most);      // (plus infinity: no distribution)
+            at = all_min(a_w.most == top_w ? at : p.vocab);
+        } else {
+            if (draft)
+                stream<true, kBatch>(segment, [&](const float (&l)[kBatch], const float (&d)[kBatch], int) {
+                    add(l, a_w);
+                    add(d, a_v);
+                });
+            else
+                stream<false, kBatch>(segment, [&](const float (&l)[kBatch], const float (&)[kBatch], int) { add(l, a_w); });
+            top_w = all_max(a_w.wrong ? INFINITY : a_w.most);
+            sum_w = all_sum(a_w.sum * weight(a_w.most, top_w));
+            if (draft) {
+                top_v = all_max(a_v.wrong ? INFINITY : a_v.most);
+                sum_v = all_sum(a_v.sum * weight(a_v.most, top_v));
+            }
+        }
+        __syncthreads();                            // the last exchange is read
+        if (lane == 0) {
+            s.tops[0][wave] = top_w;
+            s.tops[1][wave] = top_v;
+            s.sums[0][wave] = sum_w;
+            s.sums[1][wave] = sum_v;
+            s.where[wave] = at;
+        }
+        __syncthreads();
+        // the waves' together: a lane a wave
+        const int i = lane & (kWaves - 1);
+        const float a = s.tops[0][i], b = s.tops[1][i];
+        top_w = all_max(a);
+        top_v = all_max(b);
+        out[0] = (uint64_t)(top_v == INFINITY ? kNaN : __float_as_uint(top_v)) << 32 | (top_w == INFINITY ? kNaN : __float_as_uint(top_w));
+        out[2] = 0;
+        if (greedy) {
+            out[1] = (uint64_t)all_min(a == top_w ? s.where[i] : p.vocab);
+            return;
+        }
+        out[1] = __double_as_longlong(all_sum(lane < kWaves ? s.sums[0][i] * weight(a, top_w) : 0.0));
+        if (draft) out[2] = __double_as_longlong(all_sum(lane < kWaves ? s.sums[1][i] * weight(b, top_v) : 0.0));
+    }
+
+    // What is left of value x, of logits l and d.
+    __device__ __forceinline__ double left_of(int x, float l, float d) const {
+        double r = weight(l, most_w);
+        if (scale > 0.0) r = fmax(r - scale * weight(d, most_v), 0.0);
+        for (int i = 0; i < refusals; ++i)
             if (s.refused[i] == x) r = 0.0;
         return r;
     }
+    __device__ __forceinline__ double left_of(int x) const { return left_of(x, target[x], scale > 0.0 ? drafted[x] : 0.0f); }
 
-    // The sum of what is left, of every share.
-    __device__ double measure_left(const State& z) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, end = begin(wave + 1);
+    // The sum of what is left of a segment (in `sums` of each wave's share).
+    __device__ __forceinline__ void measure_left(int segment, uint64_t (&out)[kWords]) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         double sum = 0.0;
-        for (int base = begin(wave) + lane; base < end; base += 64 * kBatch / 2) {
-            float l[kBatch / 2], d[kBatch / 2];
+        if (scale > 0.0)
+            stream<true, kBatch>(segment, [&](const float (&l)[kBatch], const float (&d)[kBatch], int) {
 #pragma unroll
-            for (int i = 0; i < kBatch / 2; ++i) {
-                l[i] = base + 64 * i < end ? z.target.logits[base + 64 * i] : -INFINITY;
-                d[i] = base + 64 * i < end ? z.draft.logits[base + 64 * i] : -INFINITY;
-            }
+                for (int i = 0; i < kBatch; ++i) sum += fmax(weight(l[i], most_w) - scale * weight(d[i], most_v), 0.0);
+            });
+        else
+            stream<false, kBatch>(segment, [&](const float (&l)[kBatch], const float (&)[kBatch], int base) {
 #pragma unroll
-            for (int i = 0; i < kBatch / 2; ++i)
-                sum += fmax(power(((double)l[i] - (double)z.target.most) * c, s.table) -
-                            z.scale * power(((double)d[i] - (double)z.draft.most) * c, s.table), 0.0);
-        }
-        return sum_shares(sum, s.sums);
-    }
-
-    // The share of a refused token anew.
-    __device__ double measure_share(const State& z, int x) const {
-        const int wave = x / share, end = begin(wave + 1);
-        double sum = 0.0;
-        for (int i = begin(wave) + threadIdx.x; i < end; i += kThreads) sum += left_of(z, i);
-        sum = sum_shares(sum, s.scan);
-        if (threadIdx.x == 0) s.sums[wave] = sum;
+                for (int i = 0; i < kBatch; ++i) sum += left_of(base + 64 * i, l[i], 0.0f);
+            });
+        sum = all_sum(sum);
+        __syncthreads();                            // the last exchange is read
+        if (lane == 0) s.sums[0][wave] = sum;
         __syncthreads();
-        double all = 0.0;
-        for (int w = 0; w < kWaves; ++w) all += s.sums[w];
-        return all;
+        out[0] = __double_as_longlong(all_sum(lane < kWaves ? s.sums[0][lane & (kWaves - 1)] : 0.0));
+        out[1] = out[2] = 0;
     }
 
-    // The first token at which the sums in order pass u times all.
-    __device__ int choose(const State& z, float u, const double* sums) const {
+    // Brings the first values of a row's own segment near, while others' words are waited for.
+    __device__ __forceinline__ void touch(int row, bool draft) const {
+        const int x = min(share_begin(own, threadIdx.x >> 6) + (int)(threadIdx.x & 63), p.vocab - 1);
+        const size_t at = (size_t)(start + row) * p.vocab;
+        float near = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const size_t y = at + min(x + 64 * i, p.vocab - 1);
+            near = fmaxf(near, p.logits[y]);
+            if (draft) near = fmaxf(near, p.draft[y]);
+        }
+        asm volatile("" ::"v"(near));
+    }
+
+    // An exchange: of a row's largest values and sums, or (LEFT) of what is left, of every segment or of `only` one.
+    template <bool LEFT>
+    __device__ __forceinline__ void trade(int only, int next = -1) {
+        constexpr int words = LEFT ? 1 : kWords;
+        const int segments = how.segments;
+        uint64_t* const slot = slots + (size_t)exchange * segments * kWords;
+        ++exchange;
+        bool waited = segments == 1;
+        int segment = only < 0 ? own : only;
+        bool computes = segment == own;             // (another's word is waited for first)
+        for (;;) {
+            if (computes) {
+                uint64_t out[kWords];
+                if (LEFT) measure_left(segment, out);
+                else measure(segment, out);
+                if (threadIdx.x < words) {
+                    uint64_t word = out[0];
+                    if (threadIdx.x == 1) word = out[1];
+                    if (threadIdx.x == 2) word = out[2];
+                    s.words[threadIdx.x][segment] = word;
+                    if (segments > 1 && segment == own)
+                        __hip_atomic_store(slot + segment * kWords + threadIdx.x, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            } else {
+                __syncthreads();                    // the last exchange is read
+            }
+            if (!waited) {
+                if (next >= 0) touch(next, drafted != nullptr);
+                for (int i = threadIdx.x; i < segments * words; i += kThreads) {
+                    const int of = i / words, word = i - of * words;
+                    if (of == own || (only >= 0 && of != only)) continue;
+                    const long long begin = clock64();
+                    uint64_t got;
+                    do {
+                        got = __hip_atomic_load(slot + of * kWords + word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    } while (got == kEmpty && clock64() - begin < how.wait);
+                    s.words[word][of] = got;
+                }
+                waited = true;
+            }
+            __syncthreads();
+            // a segment whose words have not come
+            int missing = segments;
+            for (int i = threadIdx.x & 63; i < segments; i += 64)
+                for (int j = 0; j < words; ++j)
+                    if ((only < 0 || i == only) && s.words[j][i] == kEmpty) missing = min(missing, i);
+            missing = all_min(missing);
+            if (missing == segments) return;
+            segment = missing;
+            computes = true;
+        }
+    }
+
+    // The distributions at a row; false: there is none.
+    __device__ __forceinline__ bool look(int row, bool draft, int next) {
+        target = p.logits + (size_t)(start + row) * p.vocab;
+        drafted = draft ? p.draft + (size_t)(start + row) * p.vocab : nullptr;
+        scale = used = 0.0;
+        refusals = 0;
+        trade<false>(-1, next);
+        const int lane = threadIdx.x & 63, segments = how.segments;
+        float a[kMostSegments / 64], b[kMostSegments / 64];
+        most_w = greedy ? -INFINITY : -FLT_MAX;
+        most_v = -FLT_MAX;
+        bool wrong = false;
+#pragma unroll
+        for (int k = 0; k < kMostSegments / 64; ++k) {
+            const bool some = lane + 64 * k < segments;
+            const uint64_t tops = some ? s.words[0][lane + 64 * k] : 0xff800000ff800000ull;
+            a[k] = __uint_as_float((uint32_t)tops);
+            b[k] = __uint_as_float((uint32_t)(tops >> 32));
+            wrong = wrong || a[k] != a[k] || (draft && b[k] != b[k]);
+            most_w = fmaxf(most_w, a[k]);
+            most_v = fmaxf(most_v, b[k]);
+        }
+        most_w = all_max(most_w);
+        most_v = all_max(most_v);
+        if (__any(wrong)) return false;
+        if (greedy) {
+            best = p.vocab;
+#pragma unroll
+            for (int k = 0; k < kMostSegments / 64; ++k)
+                if (lane + 64 * k < segments && a[k] == most_w) best = min(best, (int)s.words[1][lane + 64 * k]);
+            best = all_min(best);
+            return most_w > -INFINITY;
+        }
+        total_w = total_v = 0.0;
+#pragma unroll
+        for (int k = 0; k < kMostSegments / 64; ++k) {
+            const int i = lane + 64 * k;
+            if (i >= segments) continue;
+            const double sum = __longlong_as_double(s.words[1][i]) * weight(a[k], most_w);
+            if (threadIdx.x < 64) s.whole[i] = s.left[i] = sum;
+            total_w += sum;
+            if (draft) total_v += __longlong_as_double(s.words[2][i]) * weight(b[k], most_v);
+        }
+        total_w = all_sum(total_w);
+        if (draft) total_v = all_sum(total_v);
+        left = total_w;
+        return total_w > 0.0 && (!draft || total_v > 0.0);   // (minus infinity everywhere)
+    }
+
+    // A refused child of the row, whose token has r left: what is left then.
+    __device__ __forceinline__ void refuse(int x, double r) {
+        const bool draft = drafted != nullptr;
+        const int of = x / how.size;
+        bool asks = true;
+        __syncthreads();                            // `left` is written
+        if (draft) {
+            used += left / total_w;
+            scale = used * total_w / total_v;
+        } else {
+            // One segment has less.  A difference that is not small beside the sum is as good as a new sum, and needs no exchange.
+            const double after = s.left[of] - r;
+            asks = !(after >= s.whole[of] * 0x1p-10);
+            __syncthreads();                        // `left` is read
+            if (threadIdx.x == 0) {
+                s.refused[refusals] = x;
+                s.left[of] = after;
+            }
+            ++refusals;
+            __syncthreads();
+        }
+        const int only = draft ? -1 : of;
+        if (asks) trade<true>(only);
+        left = 0.0;
+        for (int i = threadIdx.x & 63; i < how.segments; i += 64) {
+            const double sum = asks && (draft || i == of) ? __longlong_as_double(s.words[0][i]) : s.left[i];
+            if (asks && threadIdx.x < 64) s.left[i] = sum;
+            left += sum;
+        }
+        left = all_sum(left);
+    }
+
+    // What a child's token, of logits l and d, has left, and whether it is taken.
+    __device__ __forceinline__ bool takes(int x, float u, float l, float d, double& r) const {
+        r = weight(l, most_w);
+        double of_draft = 1.0;
+        if (drafted) {
+            const double y = weight(d, most_v);
+            of_draft = y / total_v;
+            if (scale > 0.0) r = fmax(r - scale * y, 0.0);
+        }
+        for (int i = 0; i < refusals; ++i)
+            if (s.refused[i] == x) r = 0.0;
+        return (double)u * left * of_draft < r;
+    }
+
+    // Of n sums in order, the one at which they pass a goal, and what is before it; past all, the last that is not zero.
+    __device__ static __forceinline__ int passed(const double* sums, int n, double goal, double& before) {
+        double upto = before, last_before = before;
+        int last = 0;
+        for (int i = 0; i < n; ++i) {
+            const double sum = sums[i];
+            if (sum > 0.0) {
+                last = i;
+                last_before = upto;
+            }
+            if (upto + sum > goal) break;           // (then it is not zero)
+            upto += sum;
+        }
+        before = last_before;
+        return last;
+    }
+
+    // The first token at which the sums in order pass u times all, in the workgroup that has its segment; -1 in others.
+    __device__ __forceinline__ int choose(float u) {
+        __syncthreads();                            // `left` is written
+        const bool none = !(left > 0.0);
+        if (none) {
+            scale = 0.0;
+            refusals = 0;
+        }
+        const double* sums = none ? s.whole : s.left;
         double all = 0.0;
-        for (int w = 0; w < kWaves; ++w) all += sums[w];
+        for (int i = 0; i < how.segments; ++i) all += sums[i];
         const double goal = (double)fminf(fmaxf(u, 0.0f), 1.0f) * all;
         double before = 0.0;
-        int wave = -1, last = 0;
-        double last_before = 0.0;
-        for (int w = 0; w < kWaves && wave < 0; ++w) {
-            if (sums[w] > 0.0) {
-                last = w;
-                last_before = before;
-            }
-            if (before + sums[w] > goal) wave = w;
-            else before += sums[w];
-        }
-        if (wave < 0) {                             // (u is 1)
-            wave = last;
-            before = last_before;
-        }
-        // the share's values, some in order to a thread
-        const int from = begin(wave), end = begin(wave + 1), each = (end - from + kThreads - 1) / kThreads;
-        const int own = min(from + (int)threadIdx.x * each, end), own_end = min(own + each, end);
+        const int segment = passed(sums, how.segments, goal, before);
+        if (segment != own) return -1;
+        uint64_t unused[kWords];
+        measure_left(own, unused);                  // the waves' shares
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int share = passed(s.sums[0], kWaves, goal, before);
+        // of the wave's share some values in order to a thread
+        const int from = share_begin(own, share), end = share_begin(own, share + 1), each = (end - from + kThreads - 1) / kThreads;
+        const int mine = min(from + (int)threadIdx.x * each, end), mine_end = min(mine + each, end);
         double sum = 0.0;
-        for (int i = own; i < own_end; ++i) sum += left_of(z, i);
+        for (int x = mine; x < mine_end; ++x) sum += left_of(x);
         double upto = sum;
+#pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const double below = __shfl_up(upto, o, 64);
-            if ((int)(threadIdx.x & 63) >= o) upto += below;
+            if (lane >= o) upto += below;
         }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) s.scan[threadIdx.x >> 6] = upto;
+        if (lane == 63) s.sums[1][wave] = upto;
         if (threadIdx.x == 0) s.found = p.vocab;
         __syncthreads();
-        double start = before + upto - sum;
-        for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) start += s.scan[w];
-        // a token of the thread that passes it; and the share's last one that is left, where rounding lets none
+        double at = before + upto - sum;
+        for (int i = 0; i < wave; ++i) at += s.sums[1][i];
         int passes = p.vocab, last_left = -1;
-        for (int i = own; i < own_end; ++i) {
-            const double r = left_of(z, i);
-            start += r;
-            if (r > 0.0) {
-                last_left = i;
-                if (start > goal && passes == p.vocab) passes = i;
-            }
+        for (int x = mine; x < mine_end; ++x) {
+            const double r = left_of(x);
+            at += r;
+            if (!(r > 0.0)) continue;
+            last_left = x;
+            if (at > goal && passes == p.vocab) passes = x;
         }
-        atomicMin(&s.found, passes);
+        passes = all_min(passes);
+        if (lane == 0) atomicMin(&s.found, passes);
         __syncthreads();
-        const int found = s.found;
+        passes = s.found;
+        if (passes < p.vocab) return passes;
+        // rounding lets none pass: the share's last token that is left
         __syncthreads();
-        if (found < p.vocab) return found;
         if (threadIdx.x == 0) s.found = -1;
         __syncthreads();
         atomicMax(&s.found, last_left);
@@ -252,123 +517,103 @@ struct Walk {
     }
 };
 
-__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyCall p) {
+__global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How how) {
     __shared__ Shared s;
-    const int request = blockIdx.x, lane = threadIdx.x & 63;
+    const int request = blockIdx.x / how.segments, own = blockIdx.x % how.segments, lane = threadIdx.x & 63;
     const int start = p.batch.starts[request];
     int rows = p.batch.rows[request];
     if (rows < 0 || rows > p.batch.max_rows || start < 0 || start > p.batch.tokens - rows) rows = 0;
     if (rows == 0) {
-        if (threadIdx.x == 0) {
+        if (own == 0 && threadIdx.x == 0) {
             p.kept[request] = 0;
             p.next[request] = -1;
         }
         return;
     }
+    const float temperature = p.temperatures[request];
+    uint64_t* const slots = (uint64_t*)p.workspace + (size_t)2 * start * how.segments * kWords;
+    Walk walk(p, s, how, slots, own, start, temperature);
     for (int i = threadIdx.x; i < rows; i += kThreads) {
         s.parents[i] = p.parents[start + i];
         s.ids[i] = p.ids[start + i];
         s.accept[i] = p.accept[start + i];
-        p.path[start + i] = i ? -1 : 0;
+        if (own == 0) p.path[start + i] = i ? -1 : 0;
     }
     if (threadIdx.x < kTable) s.table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
     __syncthreads();
-    const float temperature = p.temperatures[request];
-    const bool greedy = temperature == 0.0f;
-    const Walk walk{p, s, 1.4426950408889634 / (double)temperature, (p.vocab + kWaves - 1) / kWaves};
-    State z{};
-    bool known = false;                             // the row's distributions are measured
-    int row = 0, kept = 1;
-    auto look = [&]() {
-        const size_t at = (size_t)(start + row) * p.vocab;
-        z.target.logits = p.logits + at;
-        z.draft.logits = p.draft ? p.draft + at : nullptr;
-        z.scale = z.used = 0.0;
-        z.refusals = 0;
-        z.bad = !(temperature >= 0.0f && temperature < INFINITY) || !walk.measure(z.target, z.best, greedy, s.sums);
-        if (!z.bad && !greedy) {
-            z.left = z.target.total;
-            if (threadIdx.x < kWaves) s.whole[threadIdx.x] = s.sums[threadIdx.x];
-            __syncthreads();
+    const bool with_draft = p.draft && !walk.greedy;
+    // The next child of a row, from row i on, that a walk tries or takes without a test; rows: none.
+    auto child_of = [&](int row, int i) {
+        for (int base = i; base < rows; base += 64) {
+            const int at = min(base + lane, rows - 1);
+            const bool fits = base + lane < rows && s.parents[at] == row && (s.accept[at] < 0.0f || (unsigned)s.ids[at] < (unsigned)p.vocab);
+            const uint64_t some = __ballot(fits);
+            if (some) return base + __builtin_ctzll(some);
         }
-        known = true;
+        return rows;
     };
-    bool draft_known = false;
-    for (int i = 1; ; ++i) {
-        // the next child
-        int child = rows;
-        for (int base = i; base < rows && child == rows; base += 64) {
-            const uint64_t some = __ballot(base + lane < rows && s.parents[min(base + lane, rows - 1)] == row);
-            if (some) child = base + __builtin_ctzll(some);
-        }
-        if (child == rows) break;
-        i = child;
-        const int x = s.ids[i];
-        const float u = s.accept[i];
-        bool taken = u < 0.0f;
+    int row = 0, kept = 1;
+    bool known = false, wrong = !(temperature >= 0.0f && temperature < INFINITY);
+    for (int child = child_of(0, 1); ; child = child_of(row, child + 1)) {
+        bool taken = child < rows && s.accept[child] < 0.0f;
         if (!taken) {
-            if (!known) look();
-            if (z.bad) break;
-            if ((unsigned)x >= (unsigned)p.vocab) continue;
-            if (greedy) {
-                taken = x == z.best;
-            } else {
-                double of_draft = 1.0;
-                if (z.draft.logits) {
-                    if (!draft_known) {
-                        int unused;
-                        z.bad = !walk.measure(z.draft, unused, false, s.scan);
-                        if (z.bad) break;
-                        draft_known = true;
-                    }
-                    of_draft = weight(z.draft, x, walk.c, s.table) / z.draft.total;
-                }
-                taken = (double)u * z.left * of_draft < walk.left_of(z, x);
-                if (!taken && z.draft.logits) {
-                    z.used += z.left / z.target.total;
-                    z.scale = z.used * z.target.total / z.draft.total;
-                    z.left = walk.measure_left(z);
-                } else if (!taken) {
-                    __syncthreads();
-                    if (threadIdx.x == 0) s.refused[z.refusals] = x;
-                    ++z.refusals;
-                    __syncthreads();
-                    z.left = walk.measure_share(z, x);
-                }
+            const int x = child < rows ? s.ids[child] : 0;
+            float l = 0.0f, d = 0.0f;
+            if (child < rows && !walk.greedy) {
+                const size_t at = (size_t)(start + row) * p.vocab + x;
+                l = p.logits[at];
+                if (with_draft) d = p.draft[at];
             }
+            if (!known && !wrong) wrong = !walk.look(row, with_draft && child < rows, child < rows ? child : -1);
+            known = true;
+            if (wrong || child == rows) break;
+            double r;
+            taken = walk.greedy ? x == walk.best : walk.takes(x, s.accept[child], l, d, r);
+            if (!taken && !walk.greedy) walk.refuse(x, r);
         }
         if (taken) {
-            if (threadIdx.x == 0) p.path[start + kept] = i;
+            if (own == 0 && threadIdx.x == 0) p.path[start + kept] = child;
             ++kept;
-            row = i;
-            known = draft_known = false;
-            z.bad = false;
+            row = child;
+            known = false;
         }
     }
-    if (!known) look();
     int next = -1;
-    if (!z.bad && greedy) {
-        next = z.best;
-    } else if (!z.bad) {
-        const bool some = z.left > 0.0;
-        if (!some) {
-            z.scale = 0.0;
-            z.refusals = 0;
-        }
-        next = walk.choose(z, p.sample[request], some ? s.sums : s.whole);
-    }
-    if (threadIdx.x == 0) {
-        p.kept[request] = kept;
-        p.next[request] = next;
-    }
+    if (!wrong) next = walk.greedy ? (own == 0 ? walk.best : -1) : walk.choose(p.sample[request]);
+    if (threadIdx.x != 0) return;
+    if (own == 0) p.kept[request] = kept;
+    if (next >= 0 || (wrong && own == 0)) p.next[request] = next;
+}
+
+__global__ void empty_slots_kernel(uint64_t* slots, size_t count) {
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (size_t)gridDim.x * blockDim.x) slots[i] = kEmpty;
+}
+
+// Workgroups that the requests' vocabularies are cut for: as many as the GPU has CUs (each has registers for one), of
+// at least 2048 values each.
+constexpr int kTarget = 256, kLeast = 2048;
+How how_of(const VerifyCall& call) {
+    const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, kTarget / call.batch.requests)});
+    How how{most, 0, 200000};
+    how.size = ((call.vocab + most - 1) / most + kWaves - 1) / kWaves * kWaves;
+    how.segments = (call.vocab + how.size - 1) / how.size;
+    return how;
+}
+size_t slot_words(const VerifyCall& call) {
+    const int segments = how_of(call).segments;
+    return segments > 1 ? (size_t)2 * call.batch.tokens * segments * kWords : 0;
 }
 
 }  // namespace
 
-size_t verify_workspace_bytes(const VerifyCall&) { return 0; }
+size_t verify_workspace_bytes(const VerifyCall& call) { return 8 * slot_words(call); }
 
 void launch_verify(const VerifyCall& call, hipStream_t stream) {
-    verify_kernel<<<call.batch.requests, kThreads, 0, stream>>>(call);
+    How how = how_of(call);
+    if (const char* cycles = std::getenv("LEAF_VERIFY_WAIT")) how.wait = std::atoll(cycles);
+    if (const size_t words = slot_words(call))
+        empty_slots_kernel<<<(int)std::min<size_t>((words + 1023) / 1024, 1024), 256, 0, stream>>>((uint64_t*)call.workspace, words);
+    verify_kernel<<<call.batch.requests * how.segments, kThreads, 0, stream>>>(call, how);
 }
 
 }  // namespace leafhip

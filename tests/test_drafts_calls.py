@@ -52,7 +52,7 @@ def test_refused_arguments(fake_hip):  # noqa: F811
              "attend_tree(workspace=buffer.ptr + 8, bytes=1 << 20)", "attend_tree(batch(tokens=2**20), heads=130)"] +
             [f"verify(batch({n}=None))" for n in ("starts", "rows")] +
             [f"verify(d=drafts({n}=None))" for n in ("logits", "ids", "parents", "temperatures", "accept", "sample", "path", "kept", "next")] +
-            ["verify(d=drafts(vocab=0))", "verify(d=drafts(vocab=2**31 - 1))", "verify(d=drafts(vocab=2**32 - 1))",
+            ["verify(d=drafts(vocab=0))", "verify(d=drafts(vocab=2**30 + 1))", "verify(d=drafts(vocab=2**32 - 1))",
              "verify(workspace=buffer.ptr + 8, bytes=1 << 20)"] +
             [f"compact(batch({n}=None))" for n in ("table", "lengths", "starts", "rows")] +
             ["compact(path=-buffer.ptr)", "compact(kept=-buffer.ptr)", "compact(layers=0)", "compact(layers=65536)",

@@ -476,3 +476,13 @@ def test_keeping_many_requests(rt):
     rng = np.random.default_rng(45)
     requests = [(int(rng.integers(0, 100)), int(rng.integers(1, 40))) for _ in range(4000)]
     check_keep(rt, keep_case(rng, random_paths(rng, requests), 1, 16, 16, ref.INT8, 1), 16, ref.INT8)
+
+
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("vocab", [5000, 32000, 50257])
+def test_verification_without_waiting(rt, monkeypatch, vocab, with_draft):
+    # a workgroup that waits for no other computes all that they owe it, to the same results
+    monkeypatch.setenv("LEAF_VERIFY_WAIT", "0")
+    rng = np.random.default_rng(vocab)
+    for counts in ([6], [8] * 40):
+        check_verify(rt, draft_case(rng, counts, vocab, 3, with_draft, np.where(np.arange(len(counts)) % 5 == 4, 0.0, 0.9), padding=1))
