@@ -457,10 +457,14 @@ lh_status lh_kv_tree(const lh_kv_batch* batch, const int32_t* parents, uint64_t*
  * masks may be others than lh_kv_tree's; bits of rows that the request does not have count for nothing).  With a window, keys at
  * positions up to the row's own less window are hidden, where a step's row stands at positions[t] (at
  * least length - rows; read only then).  A row that sees no key gets zeros.  Otherwise as
- * lh_attention_kv8: the same batch arrays, NaN rules, accuracy and workspace. */
+ * lh_attention_kv8: the same batch arrays, NaN rules and accuracy, and the same rules for a workspace, of
+ * lh_attention_kv8_tree_workspace bytes. */
 lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,
                                 uint32_t window, const uint64_t* masks, float* out, void* workspace, size_t workspace_bytes,
                                 lh_stream stream);
+
+/* Bytes that any call of the batch's sizes needs, whatever the lengths. */
+lh_status lh_attention_kv8_tree_workspace(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads, size_t* bytes);
 
 /* What verification reads and writes: device pointers. */
 typedef struct lh_drafts {

@@ -236,23 +236,23 @@ struct KeyBits {
 
 // A step's scores to weights: acc [tile][r] are the products of key 4 tile + r of the lane's 16.
 // Rescales sum and o where their bases move.
-template <typename Seen, int TILES>
-__device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], Seen seen,
-                                      v8h (&hi)[2], v8h (&lo)[2]) {
+template <typename Seen, int TILES, int NJ>
+__device__ __forceinline__ void weigh(v4f (&acc)[NJ], float c, KeyScales s, Softmax& m, v4f (&o)[TILES], Seen seen,
+                                      v8h (&hi)[NJ / 2], v8h (&lo)[NJ / 2]) {
     constexpr bool MASKED = !Seen::kAll;
     const float e = (float)((int)(__float_as_uint(s.value) >> 23) - 127);
     c *= s.key;
     c = c < 1e-37f ? 1e-37f : c;                    // (a masked key is minus infinity times it)
     if (MASKED) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (!seen(4 * j + r)) acc[j][r] = -INFINITY;
     }
     float top = acc[0][0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[j][r]);
     top *= c;
@@ -276,18 +276,18 @@ __device__ __forceinline__ void weigh(v4f (&acc)[4], float c, KeyScales s, Softm
     if (m.far) {
         const bool far = __builtin_fabsf(m.base) > kFar;           // a row's own: all of its waves weigh a score alike
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[j][r] = far ? (acc[j][r] * c - m.base) + kLift : fmaf(acc[j][r], c, shift);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(acc[j][r], c, shift);
     }
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NJ; ++j) {
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
 // in its products while the other is in its softmax (62 and 143), gave nothing.
 constexpr int kTileRows = 16 * kWaves;
 
-template <int CC, bool FULL, bool E4M3, bool TREE>
+template <int CC, bool FULL, bool E4M3>
 __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
     constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
@@ -657,27 +657,25 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
     const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
     int per;
-    const Item item = find_item<TREE>(p, group, share, blockIdx.x / kv_heads, per);
+    const Item item = find_item<false>(p, group, share, blockIdx.x / kv_heads, per);
     if (item.request < 0) return;
     const Kv8Request& q = item.q;
     const int rows = q.rows * group, w0 = item.tile * kTileRows + 16 * wave;   // the wave's first row
     const int before = q.length - q.rows;                          // position of the first row
-    const Steps seen = steps_of<TREE>(q, group, p.window, kTileRows, item.tile);
+    const Steps seen = steps_of<false>(q, group, p.window, kTileRows, item.tile);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
     if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
     const int begin = seen.begin + (int)((long long)item.part * steps / parts);
     const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
     const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
-    const TreeRow<0> tree = TREE ? TreeRow<0>(p, q, row / group) : TreeRow<0>();
-    const int position = TREE ? tree.position : before + row / group;
+    const int position = before + row / group;
     v8h qh[CC][2], ql[CC][2];
     float c;
     load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
     // of the wave's rows: the first sees every key up to `low`, the last none after `high`
-    // (of a tree's rows: any sees every key before the first's position, none one at or after the length)
-    const int low = TREE ? before : before + min(w0, rows - 1) / group;
-    const int high = w0 >= rows ? -1 : TREE ? q.length - 1 : before + min(w0 + 15, rows - 1) / group;
+    const int low = before + min(w0, rows - 1) / group;
+    const int high = w0 < rows ? before + min(w0 + 15, rows - 1) / group : -1;
 
     // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
     v4u kr[CC], vr[CC];
@@ -749,10 +747,9 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
                 }
             v8h hi[2], lo[2];
             const int at = step * kStep + 16 * lq;
-            if (step * kStep + kStep > low + !TREE || (p.window && step * kStep <= high - p.window)) {
+            if (step * kStep + kStep > low + 1 || (p.window && step * kStep <= high - p.window)) {
                 const int from = p.window ? position + 1 - p.window - at : 0;
-                if (TREE) weigh(acc, c, now, m, o, KeyBits{tree.seen(at, from)}, hi, lo);
-                else weigh(acc, c, now, m, o, KeyRange{from, position + 1 - at}, hi, lo);
+                weigh(acc, c, now, m, o, KeyRange{from, position + 1 - at}, hi, lo);
             } else {
                 weigh(acc, c, now, m, o, EveryKey{}, hi, lo);
             }
@@ -779,12 +776,194 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
     const float sum = add_xor32(add_xor16(m.sum));
     if (w0 + li >= rows) return;
     float* to = p.out + ((size_t)token * p.heads + head) * dim;
-    float scale = TREE ? part_scale(m.lift, sum) : output_scale(m.lift, sum);
+    float scale = output_scale(m.lift, sum);
     if (parts > 1) {
         const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
         to = partial_values(p, share, slot) + (size_t)(16 * wave + li) * dim;
         scale = part_scale(m.lift, sum);
         if (lq == 0) partial_sums(p, share, slot)[16 * wave + li] = v2f{m.base, sum};
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+        if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[t] * scale;
+}
+
+// ---- the same of trees: of up to 32 rows of a KV head two waves for 16 of them, each with half of a step's keys; codes are
+// loaded two steps ahead
+template <int CC, bool FULL, bool E4M3, int SPLIT>
+__global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_kernel(AttentionKv8Call p, Share share) {
+    constexpr int TILES = 4 * CC, NJ = 4 / SPLIT, NH = NJ / 2;     // of a wave: tiles of 16 keys, operands of 32
+    constexpr int kOperand = 64 * 16;                              // bytes of one operand of a wave
+    constexpr int kKeyBytes = 4 * CC * 2 * kOperand, kBuffer = 2 * kKeyBytes;
+    extern __shared__ __align__(16) uint8_t lds[];                 // two of [tile of keys][cc][half][lane], [tile of dims][half][lane]
+    __shared__ float bases[kWaves][16], lifts[kWaves][16], sums[kWaves][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lq = lane >> 4;
+    const int kh = wave % SPLIT;                                   // which of a step's keys are the wave's
+    const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads, dim = FULL ? 64 * CC : p.cache.dim;
+    const int kvh = blockIdx.x % kv_heads, tiles = FULL ? TILES : dim / 16;
+    int per;
+    const Item item = find_item<true>(p, group, share, blockIdx.x / kv_heads, per);
+    if (item.request < 0) return;
+    const Kv8Request& q = item.q;
+    const int rows = q.rows * group, in_tile = 16 * (wave / SPLIT), w0 = item.tile * share.tile_rows + in_tile;   // the wave's first row
+    const int before = q.length - q.rows;
+    const Steps seen = steps_of<true>(q, group, p.window, share.tile_rows, item.tile);
+    const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
+    if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
+    const int begin = seen.begin + (int)((long long)item.part * steps / parts);
+    const int end = seen.begin + (int)((long long)(item.part + 1) * steps / parts);
+    const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
+    const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
+    const TreeRow<0> tree(p, q, row / group);
+
+    // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
+    struct Codes {
+        v4u k[CC], v[CC];
+        bool known;
+    } codes[2];
+    auto load = [&](Codes& c, int step, int ik, int iv) {
+        const uint8_t *kc = keys.key_codes(ik, step), *vc = keys.value_codes(iv, step);
+        c.known = keys.known(iv);
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            c.k[cc] = keys.load_key<FULL>(kc, wave, cc, lq);
+            c.v[cc] = keys.load_value(vc, FULL ? wave + 4 * cc : min(wave + 4 * cc, tiles - 1));
+        }
+    };
+    auto store = [&](Codes& c, int step) {
+        uint8_t* buffer = lds + (step & 1) * kBuffer;
+        // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
+        const bool clear = E4M3 && (step * kStep + kStep > q.length || !__all(c.known));
+#pragma unroll
+        for (int cc = 0; cc < CC; ++cc) {
+            v8h a, b;
+            widen<E4M3>(c.k[cc], a, b);
+            v8h* to = (v8h*)(buffer + ((wave * CC + cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+            if (clear) c.v[cc] = first_codes(c.v[cc], c.known ? q.length - (step * kStep + 16 * lq) : 0);
+            widen<E4M3>(c.v[cc], a, b);
+            to = (v8h*)(buffer + kKeyBytes + ((wave + 4 * cc) * 2) * kOperand) + lane;
+            to[0] = a;
+            to[64] = b;
+        }
+    };
+
+    // Every load is used two steps later and none issued under a condition, after which a wait for an older one would be
+    // for all; past the end they are the last block's and not used.
+    load(codes[0], begin, keys.key_block(begin), keys.value_block(begin));
+    load(codes[1], begin + 1, keys.key_block(begin + 1), keys.value_block(begin + 1));
+    v8h qh[CC][2], ql[CC][2];
+    float c;
+    load_query<CC, FULL>(p.q_heads + ((size_t)head * p.batch.tokens + token) * dim, dim, lq, p.scale, qh, ql, c);
+    v4f o[TILES];
+    Softmax m;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    store(codes[0], begin);
+    load(codes[0], begin + 2, keys.key_block(begin + 2), keys.value_block(begin + 2));
+    KeyScales scales = keys.scales(keys.value_block(begin));
+    int ik = keys.key_block(begin + 3), iv = keys.value_block(begin + 3), is = keys.value_block(begin + 1);
+    lds_barrier();
+    // A step: `later` holds the codes of the next one.
+    auto turn = [&](int step, Codes& later) {
+        const uint8_t* buffer = lds + (step & 1) * kBuffer;
+        store(later, step + 1);
+        load(later, step + 3, ik, iv);
+        ik = keys.key_block(step + 4);
+        iv = keys.value_block(step + 4);
+        KeyScales now = scales.checked();
+        if (w0 < rows) {
+            v4f acc[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            // (no product waits for the one before it)
+#pragma unroll
+            for (int cc = 0; cc < CC; ++cc)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8h k[NJ];
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) k[j] = *((const v8h*)(buffer + (((kh * NJ + j) * CC + cc) * 2 + h) * kOperand) + lane);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], ql[cc][h], acc[j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], qh[cc][h], acc[j], 0, 0, 0);
+                }
+            const int at = step * kStep + 16 * lq;
+            bool spare = false;
+            if (step * kStep + kStep > before || (p.window && step * kStep <= q.length - 1 - p.window)) {
+                const uint32_t bits = tree.seen(at, p.window ? tree.position + 1 - p.window - at : 0) >> (4 * NJ * kh) & ((1u << 4 * NJ) - 1);
+                // (a key that is not seen weighs nothing whatever its block's scales, if they are numbers)
+                spare = bits == 0;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(bits >> (4 * j + r) & 1)) acc[j][r] = -INFINITY;
+            }
+            v8h hi[NH], lo[NH];
+            weigh(acc, spare ? 1.0f : c, spare ? KeyScales{1.0f, 1.0f, true} : now, m, o, EveryKey{}, hi, lo);
+#pragma unroll
+            for (int t0 = 0; t0 < TILES; t0 += 4) {
+                if (!FULL && t0 >= tiles) continue;                // (tiles past the last: copies of it, not kept)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    v8h v[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) v[t] = *((const v8h*)(buffer + kKeyBytes + ((t0 + t) * 2 + kh * NH + h) * kOperand) + lane);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], lo[h], o[t0 + t], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], hi[h], o[t0 + t], 0, 0, 0);
+                }
+            }
+        }
+        scales = keys.scales(is);
+        is = keys.value_block(step + 2);
+        lds_barrier();                                             // (the next loads stay in flight)
+    };
+    for (int step = begin; ; step += 2) {
+        turn(step, codes[1]);
+        if (step + 1 >= end) break;
+        turn(step + 1, codes[0]);
+        if (step + 2 >= end) break;
+    }
+
+    m.sum = add_xor32(add_xor16(m.sum));
+    if (SPLIT > 1) {                                               // the two halves of the keys together, by the first's wave
+        v4f* others = (v4f*)lds + (wave / SPLIT) * TILES * 64 + lane;
+        if (kh == 1) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) others[t * 64] = o[t];
+            if (lq == 0) {
+                bases[wave][li] = m.base;
+                lifts[wave][li] = m.lift;
+                sums[wave][li] = m.sum;
+            }
+        }
+        lds_barrier();
+        if (kh == 1) return;
+        const float base = fmaxf(m.base, bases[wave + 1][li]), below = m.base - base, other = bases[wave + 1][li] - base;
+        const float own_lift = below + m.lift, other_lift = other + lifts[wave + 1][li], lift = fmaxf(own_lift, other_lift);
+        const float a = __builtin_amdgcn_exp2f(own_lift - lift), b = __builtin_amdgcn_exp2f(other_lift - lift);
+        m.sum = fmaf(sums[wave + 1][li], __builtin_amdgcn_exp2f(other), m.sum * __builtin_amdgcn_exp2f(below));
+        m.base = base;
+        m.lift = lift;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const v4f x = others[t * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][r] = fmaf(x[r], b, o[t][r] * a);
+        }
+    }
+    if (w0 + li >= rows) return;
+    float* to = p.out + ((size_t)token * p.heads + head) * dim;
+    const float scale = part_scale(m.lift, m.sum);                 // (a row may see no key)
+    if (parts > 1) {
+        const size_t slot = (size_t)(item.slot + item.part) * kv_heads + kvh;
+        to = partial_values(p, share, slot) + (size_t)(in_tile + li) * dim;
+        if (lq == 0) partial_sums(p, share, slot)[in_tile + li] = v2f{m.base, m.sum};
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
@@ -804,14 +983,13 @@ __device__ __forceinline__ float part_share(v2f part, float base, float inverse)
 
 // ---- rows whose keys were parted, of at most 16 rows of a KV head: a wave for each token and head, every lane four
 // values of one part at a time
-template <bool TREE>
 __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(AttentionKv8Call p, Share share) {
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63;
     const int request = blockIdx.x, kvh = blockIdx.y;
     const Kv8Request q = kv8_request(p.batch, request);
     if (!tiles_of(q, group, share)) return;
     const int* plan = (const int*)p.partial + share.at;
-    const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, 0);
+    const Steps seen = steps_of<false>(q, group, p.window, share.tile_rows, 0);
     const int parts = parts_of(seen.end - seen.begin, plan[0]), item = plan[kHeader + request];
     // (requests that claim the same rows can have more parts than there is room for: such rows stay undefined)
     if (parts == 1 || item < 0 || item > share.slots - parts) return;
@@ -826,8 +1004,7 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
         for (int i = lane; i < parts; i += 64) add_part(sums[i * sum_stride], base, total);
         const float own_base = base;
         base = wave_max_f32(base);
-        total = wave_sum_f32(total * __builtin_amdgcn_exp2f(own_base - base));
-        const float inverse = TREE && total == 0.0f ? 0.0f : 1.0f / total;
+        const float inverse = 1.0f / wave_sum_f32(total * __builtin_amdgcn_exp2f(own_base - base));
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (own < abreast) {
 #pragma unroll 4
@@ -849,7 +1026,6 @@ __global__ __launch_bounds__(1024) void attention_kv8_few_merge_kernel(Attention
 
 // ---- the same of more rows: some workgroups a tile, a thread for four values of a row
 constexpr int kMergeSplit = 4;                      // workgroups of a tile (2 / 4 / 8: a chunk beside decoding requests 45 / 44 / 48 us)
-template <bool TREE>
 __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(AttentionKv8Call p, Share share) {
     __shared__ int sums_of[kWaves], found[5];
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -890,9 +1066,9 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     const Kv8Request q{found[2], found[3], found[4]};
     const int* plan = (const int*)p.partial + share.at;
     const int per = plan[0], first = plan[kHeader + request];
-    const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, tile);
+    const Steps seen = steps_of<false>(q, group, p.window, share.tile_rows, tile);
     const int parts = parts_of(seen.end - seen.begin, per);
-    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps<TREE>(q, group, p.window, share.tile_rows), per);
+    const int item = first + (tiles_of(q, group, share) - 1 - tile) * parts_of(most_steps<false>(q, group, p.window, share.tile_rows), per);
     if (parts == 1 || item < 0 || item > share.slots - parts) return;
     const size_t kv_heads = p.cache.kv_heads, slot = (size_t)item * kv_heads + kvh;
     const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
@@ -905,7 +1081,7 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
         v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) add_part(sums[i * sum_stride], base, total);
-        const float inverse = TREE && total == 0.0f ? 0.0f : 1.0f / total;
+        const float inverse = 1.0f / total;
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) {
             const float share_of = part_share(sums[i * sum_stride], base, inverse);
@@ -917,6 +1093,65 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
     }
 }
 
+// ---- the same of trees, whose tiles have as many parts as each other: a thread for four values of a row
+constexpr int kTreeChunk = 16;
+__global__ __launch_bounds__(kThreads) void attention_kv8_tree_merge_kernel(AttentionKv8Call p, Share share) {
+    const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, quads = dim / 4;
+    const int request = blockIdx.x, kvh = blockIdx.y;
+    const int* plan = (const int*)p.partial + share.at;
+    const int per = plan[0], item = plan[kHeader + request];
+    const Kv8Request q = kv8_request(p.batch, request);
+    const int rows = q.rows * group, tiles = tiles_of(q, group, share);
+    const int unit = blockIdx.z * kThreads + threadIdx.x, row = unit / quads, quad = unit - row * quads;
+    if (!tiles || row >= rows) return;
+    const Steps seen = steps_of<true>(q, group, p.window, share.tile_rows, 0);
+    const int parts = parts_of(seen.end - seen.begin, per);
+    const int tile = row / share.tile_rows, in_tile = row - tile * share.tile_rows, at = item + (tiles - 1 - tile) * parts;
+    // (requests that claim the same rows can have more parts than there is room for: such rows stay undefined)
+    if (parts == 1 || item < 0 || at > share.slots - parts) return;
+    const size_t kv_heads = p.cache.kv_heads, slot = (size_t)at * kv_heads + kvh;
+    const size_t sum_stride = kv_heads * share.tile_rows, stride = sum_stride * dim;
+    const v2f* sums = partial_sums(p, share, slot) + in_tile;
+    const float* values = partial_values(p, share, slot) + (size_t)in_tile * dim + 4 * quad;
+    float base = kNoBase, total = 0.0f;
+    v4f x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](v2f sum, v4f v, float inverse) {
+        const float share_of = part_share(sum, base, inverse);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = fmaf(v[r], share_of, x[r]);
+    };
+    if (parts <= kTreeChunk / 2) {
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) add_part(sums[i * sum_stride], base, total);
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total; // (a row may see no key)
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) add(sums[i * sum_stride], *(const v4f*)(values + i * stride), inverse);
+    } else {
+        // many parts: their loads under way together (the last part's again behind it)
+        v2f s[kTreeChunk];
+        v4f v[kTreeChunk];
+        for (int i0 = 0; i0 < parts; i0 += kTreeChunk) {
+#pragma unroll
+            for (int i = 0; i < kTreeChunk; ++i) s[i] = sums[min(i0 + i, parts - 1) * sum_stride];
+#pragma unroll
+            for (int i = 0; i < kTreeChunk; ++i)
+                if (i0 + i < parts) add_part(s[i], base, total);
+        }
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        for (int i0 = 0; i0 < parts; i0 += kTreeChunk) {
+#pragma unroll
+            for (int i = 0; i < kTreeChunk; ++i) {
+                s[i] = sums[min(i0 + i, parts - 1) * sum_stride];
+                v[i] = *(const v4f*)(values + min(i0 + i, parts - 1) * stride);
+            }
+#pragma unroll
+            for (int i = 0; i < kTreeChunk; ++i)
+                if (i0 + i < parts) add(s[i], v[i], inverse);
+        }
+    }
+    *(v4f*)(p.out + ((size_t)(q.start + row / group) * p.heads + kvh * group + row % group) * dim + 4 * quad) = x;
+}
+
 // Workgroups that a batch's keys are cut for, about those that the GPU holds at once: more are more partial results and
 // more starts, fewer leave CUs idle.  Of few rows, with 512 / 768 / 1024: heads of 64, 100 requests 23 / 26 / 27 us, heads
 // of 128, 64 ragged requests 73 / 68 / 74 and 8 long ones 57 / 67 / 62; of many rows, heads of 64, a prompt of 2048
@@ -926,6 +1161,9 @@ constexpr int rows_target(int cc) { return cc == 1 ? 768 : cc == 2 ? 512 : 256; 
 // Steps of a part at least, with 4 / 8: one request of 4095 tokens 10.9 / 12.5 us (a part's wave has one or two steps);
 // eight prompts of 300 tokens 37 / 27 (none is parted with 8; 16 costs a chunk beside decoding requests 47 for 44).
 constexpr int kFewLeast = 4, kRowsLeast = 8;
+// The same of trees of more than 16 rows, with 512 / 768 / 1024 workgroups: 64 of 20 to 32 rows, heads of 128, 101 / 93 / 101
+// us, 16 of 360 to 512, heads of 64, 110 / 103 / 102; with 4 / 6 / 8 steps 40 of 27 to 39 rows 30 / 23 / 25 us, one of 182 18 / 18 / 20.
+constexpr int kTreeTarget = 768, kTreeLeast = 6;
 // Rows of the step for each request from which the kernel of many rows takes every request: one launch in place of
 // two, one after the other, although it has a request of one token in a tile of 64.  At 13 a request it takes 75 us for 73
 // (heads of 128) and at 8 30 for 40 (heads of 64), at 3.5 203 for 151 and 39 for 45; between 3.5 and 8 nothing was
@@ -965,6 +1203,14 @@ Shares shares_of(const AttentionKv8Call& call) {
     const bool only_many = group > kFewRows || call.batch.tokens / kManyTokens >= call.batch.requests;
     const bool only_few = (size_t)call.batch.max_rows * group <= kFewRows;
     const int cc = (call.cache.dim + 63) / 64;
+    if (call.tree && !only_few) {                   // every request in one launch
+        const bool split = (size_t)call.batch.max_rows * group <= kTileRows / 2;
+        Shares s{{}, {split ? kTileRows / 2 : kTileRows, kTreeTarget, kTreeLeast, 1, INT_MAX, 0, 0, 0}, 0};
+        s.many.items = most_items(call, s.many);
+        s.many.slots = most_slots(call, s.many);
+        s.floats = partial_floats(call, s.many);
+        return s;
+    }
     Shares s{{kFewRows, few_target(cc), kFewLeast, 1, kFewRows, 0, 0, 0},
              {kTileRows, rows_target(cc), kRowsLeast, only_many ? 1 : kFewRows + 1, INT_MAX, 0, 0, 0}, 0};
     if (only_few || !only_many) {
@@ -989,16 +1235,20 @@ void launch(const AttentionKv8Call& call, const Share& share, hipStream_t stream
         return;
     }
     constexpr int kLds = 2 * 16 * CC * 1024;
-    constexpr auto kernel = attention_kv8_rows_kernel<CC, FULL, E4M3, TREE>;
-    if (kLds >= 65536) {                            // more than the default, with the static arrays: allowed once a device
-        static std::atomic<uint64_t> allowed{0};
-        int device = 0;
-        (void)hipGetDevice(&device);
-        if (!(allowed >> (device & 63) & 1) &&
-            hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
-            allowed |= 1ull << (device & 63);
-    }
-    kernel<<<grid, kThreads, kLds, stream>>>(call, share);
+    constexpr auto large = [](const AttentionKv8Call& c, const Share& s, int groups, hipStream_t on, auto kernel, std::atomic<uint64_t>& allowed) {
+        if (kLds >= 65536 - 4096) {                 // more than the default, with the static arrays: allowed once a device
+            int device = 0;
+            (void)hipGetDevice(&device);
+            if (!(allowed >> (device & 63) & 1) &&
+                hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
+                allowed |= 1ull << (device & 63);
+        }
+        kernel<<<groups, kThreads, kLds, on>>>(c, s);
+    };
+    static std::atomic<uint64_t> allowed{0}, allowed_split{0};
+    if (!TREE) large(call, share, grid, stream, attention_kv8_rows_kernel<CC, FULL, E4M3>, allowed);
+    else if (share.tile_rows == kTileRows) large(call, share, grid, stream, attention_kv8_tree_kernel<CC, FULL, E4M3, 1>, allowed);
+    else large(call, share, grid, stream, attention_kv8_tree_kernel<CC, FULL, E4M3, 2>, allowed_split);
 }
 
 template <int CC, bool FULL, bool TREE>
@@ -1030,16 +1280,24 @@ static void launch_attention(const AttentionKv8Call& call, hipStream_t stream) {
     }
     // (no tile is parted that has no more steps than a part at least)
     const size_t steps = ((size_t)call.batch.width << call.batch.block_shift) / kStep + 1;
+    if (TREE) {
+        const Share& share = shares.few.items ? shares.few : shares.many;
+        const int64_t units = (int64_t)group * call.batch.max_rows * (dim / 4);
+        if (steps > (size_t)share.least)
+            attention_kv8_tree_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads, (uint32_t)((units + kThreads - 1) / kThreads)),
+                                              kThreads, 0, stream>>>(call, share);
+        return;
+    }
     if (shares.few.items && steps > (size_t)kFewLeast)
-        attention_kv8_few_merge_kernel<TREE><<<dim3(call.batch.requests, call.cache.kv_heads),
+        attention_kv8_few_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads),
                                          64 * (int)std::min<int64_t>(kFewRows, (int64_t)group * call.batch.max_rows), 0, stream>>>(call, shares.few);
     if (shares.many.items && steps > (size_t)kRowsLeast)
-        attention_kv8_rows_merge_kernel<TREE><<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
+        attention_kv8_rows_merge_kernel<<<most_tiles(call, shares.many) * call.cache.kv_heads * kMergeSplit, kThreads, 0, stream>>>(
             call, shares.many);
 }
 
 void launch_attention_kv8(const AttentionKv8Call& call, hipStream_t stream) {
-    if (call.masks) launch_attention<true>(call, stream);
+    if (call.tree) launch_attention<true>(call, stream);
     else launch_attention<false>(call, stream);
 }
 

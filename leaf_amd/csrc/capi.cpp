@@ -370,7 +370,8 @@ void run_attention_kv8(leafhip::AttentionKv8Call a, const lh_kv8* cache, const f
     const size_t bytes = leafhip::attention_kv8_workspace_bytes(a);
     std::optional<ScratchUse> scratch;
     if (workspace) {
-        require_arg(workspace_bytes >= bytes, "attention workspace is too small (lh_attention_kv8_workspace)");
+        require_arg(workspace_bytes >= bytes, a.tree ? "attention workspace is too small (lh_attention_kv8_tree_workspace)"
+                                                   : "attention workspace is too small (lh_attention_kv8_workspace)");
         a.partial = static_cast<float*>(workspace);
     } else if (bytes) {
         scratch.emplace(stream);
@@ -1056,10 +1057,20 @@ lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, c
         leafhip::AttentionKv8Call a = attention_kv8_call(batch, cache, heads, true);
         tree_view_of(batch);
         require_arg(masks && (!window || a.batch.positions), "attention of trees needs masks, and with a window positions");
+        a.tree = true;
         a.masks = masks;
         a.words = mask_words(batch);
         a.window = int(std::min<uint32_t>(window, 1u << 30));      // (a request has no more keys)
         run_attention_kv8(a, cache, q_heads, out, workspace, workspace_bytes, as_stream(stream));
+    });
+}
+lh_status lh_attention_kv8_tree_workspace(const lh_kv_batch* batch, const lh_kv8* cache, uint32_t heads, size_t* bytes) {
+    return guarded([&] {
+        require_arg(bytes != nullptr, "output pointer is null");
+        leafhip::AttentionKv8Call a = attention_kv8_call(batch, cache, heads, false);
+        tree_view_of(batch);
+        a.tree = true;
+        *bytes = leafhip::attention_kv8_workspace_bytes(a);
     });
 }
 lh_status lh_verify_drafts_workspace(const lh_kv_batch* batch, const lh_drafts* drafts, size_t* bytes) {

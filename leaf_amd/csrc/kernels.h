@@ -280,7 +280,8 @@ struct AttentionKv8Call {
     int heads = 0, window = 0;
     float scale = 1.0f;             // of q.k: 1 / sqrt(dim)
     float* partial = nullptr;       // attention_kv8_workspace_bytes(call) bytes
-    const uint64_t* masks = nullptr;   // of a tree's rows (lh_kv_tree): [tokens][words]; null: causal
+    bool tree = false;              // by masks (lh_kv_tree) [tokens][words], not causal
+    const uint64_t* masks = nullptr;
     int words = 0;
 };
 size_t attention_kv8_workspace_bytes(const AttentionKv8Call& call);

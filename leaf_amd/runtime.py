@@ -155,6 +155,7 @@ def library(path: Path | None = None) -> C.CDLL:
         "lh_attention_kv8_workspace": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, C.POINTER(sz)], i32),
         "lh_kv_tree": ([C.POINTER(KvBatch), vp, vp, vp], i32),
         "lh_attention_kv8_tree": ([C.POINTER(KvBatch), C.POINTER(Kv8), vp, u32, u32, vp, vp, vp, sz, vp], i32),
+        "lh_attention_kv8_tree_workspace": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, C.POINTER(sz)], i32),
         "lh_verify_drafts": ([C.POINTER(KvBatch), C.POINTER(Drafts), vp, sz, vp], i32),
         "lh_verify_drafts_workspace": ([C.POINTER(KvBatch), C.POINTER(Drafts), C.POINTER(sz)], i32),
         "lh_kv8_compact": ([C.POINTER(KvBatch), C.POINTER(Kv8), u32, vp, vp, vp], i32),
@@ -495,6 +496,12 @@ def attention_kv8_tree(batch: KvBatch, cache: Kv8, q_heads: DeviceArray, heads: 
     check(library().lh_attention_kv8_tree(C.byref(batch), C.byref(cache), q_heads.ptr, heads, window, masks.ptr, out.ptr,
                                           workspace.ptr if workspace is not None else None,
                                           workspace.nbytes if workspace is not None else 0, stream))
+
+
+def attention_kv8_tree_workspace(batch: KvBatch, cache: Kv8, heads: int) -> int:
+    n = C.c_size_t()
+    check(library().lh_attention_kv8_tree_workspace(C.byref(batch), C.byref(cache), heads, C.byref(n)))
+    return n.value
 
 
 def verify_drafts(batch: KvBatch, drafts: Drafts, workspace: DeviceArray | None = None, stream=None) -> None:

@@ -95,7 +95,7 @@ def attend_on_gpu(rt, c, block, form, window=0, max_rows=None, workspace=None, s
                        width=c["table"].shape[1], **{k: v.ptr for k, v in d.items()})
     cache = rt.Kv8(*(a.ptr for a in data), c["keys"].shape[1], dim, form)
     if workspace == "own":
-        workspace = rt.DeviceArray((max(16, rt.attention_kv8_workspace(batch, cache, heads)),), np.uint8)
+        workspace = rt.DeviceArray((max(16, rt.attention_kv8_tree_workspace(batch, cache, heads)),), np.uint8)
     rt.attention_kv8_tree(batch, cache, dq, heads, masks, out, window, workspace, stream)
     rt.synchronize()
     return out.numpy()
