@@ -486,3 +486,302 @@ def test_verification_without_waiting(rt, monkeypatch, vocab, with_draft):
     rng = np.random.default_rng(vocab)
     for counts in ([6], [8] * 40):
         check_verify(rt, draft_case(rng, counts, vocab, 3, with_draft, np.where(np.arange(len(counts)) % 5 == 4, 0.0, 0.9), padding=1))
+
+
+# ------------------------------------------------------- all of them together ---
+class Loop:
+    """The device side of a serving loop with drafts: `layers` caches over one pool, a vocabulary, trees of up to `most` rows."""
+
+    def __init__(self, rt, requests, tokens, most, heads, kv, dim, block, blocks, width, layers, vocab, form):
+        self.rt, self.shape, self.vocab = rt, (heads, tokens, dim), vocab
+        self.pool = rt.BlockPool(requests, tokens, block, blocks, width, max_rows=most)
+        self.caches = [rt.BlockCache(self.pool, kv, dim, form) for _ in range(layers)]
+        for cache in self.caches:                           # (codes and scales that no token wrote)
+            for a in (cache.keys, cache.values, cache.key_scales, cache.value_scales):
+                a.zero()
+        floats = {"qkv": (layers, tokens, heads + 2 * kv, dim), "logits": (tokens, vocab), "draft_logits": (tokens, vocab),
+                  "temperatures": (requests,), "accept": (tokens,), "sample": (requests,)}
+        self.data = {k: rt.DeviceArray(s, np.float32) for k, s in floats.items()}
+        self.data.update({k: rt.DeviceArray.of(np.full(n, -1, np.int32)) for k, n in
+                          (("parents", tokens), ("ids", tokens), ("path", tokens), ("kept", requests), ("next", requests))})
+        self.masks = rt.DeviceArray.of(np.zeros((tokens, -(-most // 64)), np.uint64))
+        self.q = [rt.DeviceArray((heads, tokens, dim), np.float32).zero() for _ in range(layers)]
+        self.out = [rt.DeviceArray((tokens, heads, dim), np.float32) for _ in range(layers)]
+        self.drafts = rt.Drafts(vocab=vocab, **{k: self.data[k].ptr for k, _ in rt.Drafts._fields_[1:]})
+        self.cos = self.sin = None
+        rt.synchronize()
+
+    def load(self, fresh, cos, sin, **data):
+        rt = self.rt
+        if self.cos is None:
+            self.cos, self.sin = rt.DeviceArray.of(cos), rt.DeviceArray.of(sin)
+        pairs = [(self.pool.fresh, np.asarray(fresh, np.int32))] + [(o, np.full(o.shape, 7.0, np.float32)) for o in self.out]
+        for d, a in pairs + [(self.data[k], np.asarray(a, self.data[k].dtype)) for k, a in data.items()]:
+            assert a.nbytes == d.nbytes
+            rt.check(rt.library().lh_copy_to_device(d.ptr, np.ascontiguousarray(a).ctypes.data, d.nbytes))
+
+    def launch(self, stream=None, workspaces=(None, None)):
+        rt, batch, d = self.rt, self.pool.batch, self.data
+        heads, _, dim = self.shape
+        layer = d["qkv"].nbytes // len(self.caches)
+        rt.kv_assign(batch, stream)
+        rt.kv_tree(batch, d["parents"], self.masks, stream)
+        for i, cache in enumerate(self.caches):
+            rt.check(rt.library().lh_rope_kv8(batch, cache.desc, d["qkv"].ptr + i * layer, heads, dim, self.cos.ptr, self.sin.ptr,
+                                              self.cos.shape[0], self.q[i].ptr, stream))
+            rt.attention_kv8_tree(batch, cache.desc, self.q[i], heads, self.masks, self.out[i], 0, workspaces[0], stream)
+        rt.verify_drafts(batch, self.drafts, workspaces[1], stream)
+        rt.kv8_compact(batch, [c.desc for c in self.caches], d["path"], d["kept"], stream)
+        rt.kv_keep(batch, d["kept"], stream=stream)
+
+    def results(self):
+        self.rt.synchronize()
+        got = {n: getattr(self.pool, n).numpy() for n in ("lengths", "rows", "starts", "positions", "slots", "table", "free_blocks", "free_count")}
+        got.update({n: self.data[n].numpy() for n in ("path", "kept", "next")})
+        got["out"] = [o.numpy() for o in self.out]
+        got["caches"] = [[a.numpy() for a in (c.keys, c.values, c.key_scales, c.value_scales)] for c in self.caches]
+        return got
+
+
+def serve(rt, loop, steps, requests, tokens, most, heads, kv, dim, block, blocks, width, layers, vocab, form, run):
+    """Steps of trees (each request's rows; negative: it has ended), checked against the plain forms after every step."""
+    rng = np.random.default_rng(51)
+    cos, sin = kv8.tables(rng, width * block, dim // 2)
+    lengths, table, stack, count = np.zeros(requests, int), np.full((requests, width), -1), np.arange(blocks)[::-1].copy(), blocks
+    caches = [[np.zeros(s, np.uint8) for s in ((blocks, kv, block, dim), (blocks, kv, dim, block))] +
+              [np.zeros((blocks, kv), np.float32) for _ in range(2)] for _ in range(layers)]
+    moved = 0
+    for fresh in steps:
+        c = draft_case(rng, [max(n, 0) for n in fresh], vocab, 3, True, rng.choice([0.0, 0.7, 1.2], requests),
+                       padding=tokens - sum(max(n, 0) for n in fresh))
+        qkv = rng.standard_normal((layers, tokens, heads + 2 * kv, dim)).astype(np.float32)
+        given = {k: c[k] for k in ("logits", "draft_logits", "temperatures", "accept", "sample", "parents", "ids")}
+        got = run(fresh, cos, sin, qkv=qkv, **given)
+        plan = ref.assign(lengths, fresh, table, stack, count, block, width, blocks, tokens, most)
+        starts, rows, table = plan["starts"], plan["rows"], plan["table"]
+        seen, positions = [], plan["positions"].copy()
+        for r in range(requests):
+            own = slice(starts[r], starts[r] + rows[r])
+            depth, ancestors = drafts.plan(c["parents"][own])
+            seen.append(ancestors)
+            positions[own] = plan["lengths"][r] - rows[r] + depth
+        path, kept, following = got["path"].copy(), np.zeros(requests, int), np.full(requests, -1)
+        for r in range(requests):
+            if rows[r] == 0:
+                continue
+            own = slice(starts[r], starts[r] + rows[r])
+            one, following[r] = drafts.verify(c["logits"][own], c["draft_logits"][own], c["ids"][own], c["parents"][own], c["temperatures"][r],
+                                              c["accept"][own], c["sample"][r])
+            path[own] = -1
+            path[own.start:own.start + len(one)], kept[r] = one, len(one)
+            moved += any(a != b for a, b in enumerate(one))
+        at = np.maximum(positions, 0)
+        for i in range(layers):
+            keys, values, ks, vs = caches[i]
+            turned = ref.rotated(qkv[i][:, :heads + kv], cos[at][:, None], sin[at][:, None])
+            ref.append(keys, ks, turned[:, heads:], plan["slots"], block, form, False)
+            ref.append(values, vs, qkv[i][:, heads + kv:], plan["slots"], block, form, True)
+            want = np.full((tokens, heads, dim), 7.0)
+            A = drafts.attention(turned[:, :heads].transpose(1, 0, 2), keys, values, ks, vs, table, plan["lengths"], starts, rows, seen, positions,
+                                 block, form, 0, want)
+            largest = np.nanmax(np.abs(ref.decode(values, form))) * vs.max()
+            assert np.max(np.abs(got["out"][i] - want)) <= kv8.bound(A, plan["lengths"].max(), largest)
+            for codes, scales, transposed in ((keys, ks, False), (values, vs, True)):
+                drafts.compact(codes, scales, table, plan["lengths"], starts, rows, path, kept, block, form, transposed)
+            for g, w in zip(got["caches"][i], caches[i]):
+                assert np.array_equal(g, w)
+        lengths, stack, count = drafts.keep(plan["lengths"], rows, kept, table, plan["free_blocks"], int(plan["free_left"][0]), block, blocks)
+        for name, want in (("rows", rows), ("starts", starts), ("positions", positions), ("slots", plan["slots"]), ("table", table),
+                           ("path", path), ("kept", kept), ("next", following), ("lengths", lengths), ("free_count", [count])):
+            assert np.array_equal(got[name], want), name
+        assert np.array_equal(got["free_blocks"][:count], stack[:count])
+    assert moved > 3                                        # (some paths leave rows out)
+
+
+SIZES = dict(requests=4, tokens=90, most=24, heads=8, kv=2, dim=64, block=16, blocks=24, width=8, layers=2, vocab=3000)
+STEPS = [[20, 1, 0, 17], [8, 24, 8, 1], [8, 8, 23, -1], [7, -1, 5, 20], [8, 24, 1, 8], [-1, 8, 8, 8], [24, 8, 24, 24], [9, 9, -1, 9], [8, 1, 24, 8]]
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_serving_loop(rt, form):
+    loop = Loop(rt, *SIZES.values(), form)
+
+    def run(fresh, cos, sin, **data):
+        loop.load(fresh, cos, sin, **data)
+        loop.launch()
+        return loop.results()
+    serve(rt, loop, STEPS, *SIZES.values(), rt.KV8_FORMATS[form], run)
+
+
+@pytest.mark.parametrize("own_workspaces", [False, True])
+def test_serving_loop_captured(rt, own_workspaces):
+    # one graph of a whole step, replayed, with the program's own work and waits between
+    loop, stream, graphs = Loop(rt, *SIZES.values(), "int8"), rt.Stream(), []
+    spaces = (None, None)
+    if own_workspaces:
+        spaces = tuple(rt.DeviceArray((max(16, n),), np.uint8) for n in (
+            rt.attention_kv8_tree_workspace(loop.pool.batch, loop.caches[0].desc, 8), rt.verify_drafts_workspace(loop.pool.batch, loop.drafts)))
+
+    def run(fresh, cos, sin, **data):
+        loop.load(fresh, cos, sin, **data)
+        rt.synchronize()
+        if not graphs and not own_workspaces:
+            loop.launch(stream.handle, spaces)              # eager once: the stream's scratch
+            stream.synchronize()
+            graphs.append(None)
+            return loop.results()
+        if not graphs or graphs[0] is None:
+            graphs[:] = [rt.Graph(stream, lambda: loop.launch(stream.handle, spaces))]
+        between = rt.DeviceArray((1 << 16,), np.float32).zero()
+        rt.synchronize()
+        graphs[0].launch()
+        stream.synchronize()
+        between.free()
+        return loop.results()
+    serve(rt, loop, STEPS, *SIZES.values(), ref.INT8, run)
+    graphs[0].close()
+    stream.close()
+
+
+def test_first_calls_in_a_capture_need_workspaces(rt):
+    rng = np.random.default_rng(52)
+    stream = rt.Stream()
+    starts, rows = ints(rt, [0, 3]), ints(rt, [3])
+    c = draft_case(rng, [3], 40000, 1, True, 0.9)
+    d = {k: rt.DeviceArray.of(c[k]) for k in ("logits", "draft_logits", "temperatures", "accept", "sample")}
+    d.update({k: ints(rt, c[k]) for k in ("ids", "parents")})
+    d.update(path=ints(rt, [-7] * 3), kept=ints(rt, [-7]), next=ints(rt, [-7]))
+    batch = rt.KvBatch(requests=1, tokens=3, max_rows=3, block=16, blocks=1, width=1, starts=starts.ptr, rows=rows.ptr)
+    given = rt.Drafts(vocab=40000, **{k: v.ptr for k, v in d.items()})
+    need = rt.verify_drafts_workspace(batch, given)
+    assert need > 0
+    with pytest.raises(rt.LeafError, match="outside stream capture"):
+        rt.Graph(stream, lambda: rt.verify_drafts(batch, given, None, stream.handle))
+    workspace = rt.DeviceArray((need,), np.uint8)
+    with pytest.raises(rt.LeafError, match="too small"):
+        rt.check(rt.library().lh_verify_drafts(batch, given, workspace.ptr, need - 1, None))
+    want = drafts.verify(c["logits"], c["draft_logits"], c["ids"], c["parents"], c["temperatures"][0], c["accept"], c["sample"][0])
+    graph = rt.Graph(stream, lambda: rt.verify_drafts(batch, given, workspace, stream.handle))
+    for _ in range(3):
+        rt.check(rt.library().lh_copy_to_device(d["next"].ptr, np.array([-7], np.int32).ctypes.data, 4))
+        rt.synchronize()
+        graph.launch()
+        stream.synchronize()
+        assert d["next"].numpy()[0] == want[1] and list(d["path"].numpy()[:len(want[0])]) == want[0]
+    graph.close()
+    stream.close()
+
+
+def test_two_streams_at_once(rt):
+    # attention and verification on two streams, in scratch of their streams and in workspaces of their own; then in two graphs
+    rng = np.random.default_rng(53)
+    streams, calls, outs, want, kept, graphs = [rt.Stream(), rt.Stream()], [], [], [], [], []
+    for n, counts in enumerate(([9] * 12, [30, 5, 17])):
+        c = tree_case(rng, [(1500 + 300 * i, r) for i, r in enumerate(counts)], 8, 2, 64, 32, ref.INT8)
+        v = draft_case(rng, counts, 20000, 3, True, 0.8)
+        want.append([attend_on_gpu(rt, c, 32, ref.INT8), *verify_on_gpu(rt, v)])
+        tokens, words = len(v["ids"]), -(-max(counts) // 64)
+        d = {k: ints(rt, c[k]) for k in ("table", "lengths", "starts", "rows")}
+        data = [rt.DeviceArray.of(c[k]) for k in ("keys", "values", "key_scales", "value_scales", "q")]
+        masks = rt.DeviceArray.of(np.concatenate([drafts.packed(s, words) for s in c["seen"]]))
+        f = {k: rt.DeviceArray.of(v[k]) for k in ("logits", "draft_logits", "temperatures", "accept", "sample")}
+        f.update({k: ints(rt, v[k]) for k in ("ids", "parents")})
+        f.update(path=ints(rt, [0] * tokens), kept=ints(rt, [0] * len(counts)), next=ints(rt, [0] * len(counts)))
+        out = rt.DeviceArray((tokens, 8, 64), np.float32)
+        batch = rt.KvBatch(requests=len(counts), tokens=tokens, max_rows=max(counts), block=32, blocks=len(c["keys"]), width=c["table"].shape[1],
+                           **{k: a.ptr for k, a in d.items()})
+        cache = rt.Kv8(*(a.ptr for a in data[:4]), 2, 64, ref.INT8)
+        given = rt.Drafts(vocab=20000, **{k: a.ptr for k, a in f.items()})
+        spaces = [rt.DeviceArray((max(16, size),), np.uint8) for size in (rt.attention_kv8_tree_workspace(batch, cache, 8),
+                                                                        rt.verify_drafts_workspace(batch, given))]
+        kept.append((d, data, masks, f, spaces))
+        outs.append((out, f["path"], f["kept"], f["next"]))
+
+        def call(stream, own, a=(batch, cache, data[4], masks, out, given, spaces)):
+            batch, cache, q, masks, out, given, spaces = a
+            rt.attention_kv8_tree(batch, cache, q, 8, masks, out, 0, spaces[0] if own else None, stream)
+            rt.verify_drafts(batch, given, spaces[1] if own else None, stream)
+        calls.append(call)
+
+    def check():
+        rt.synchronize()
+        for own, expected in zip(outs, want):
+            assert all(np.array_equal(o.numpy(), w) for o, w in zip(own, expected))
+            for o in own:
+                o.zero()
+        rt.synchronize()
+    for own in (False, True):
+        for _ in range(3):
+            for call, stream in zip(calls, streams):
+                call(stream.handle, own)
+        check()
+    for call in calls:
+        graphs.append(rt.Graph(streams[0], lambda: call(streams[0].handle, True)))
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            rt.check(rt.library().lh_graph_launch(graph.handle, stream.handle))
+        check()
+    for g in graphs + streams:
+        g.close()
+
+
+# ------------------------------------------------------------- far offsets ---
+def test_verification_far_offsets(rt):
+    # logits past 2^31 values from the first
+    vocab, tokens, first = 151936, 14500, 14200
+    rng = np.random.default_rng(54)
+    c = draft_case(rng, [7], vocab, 2, True, 0.9)
+    logits, draft = (rt.DeviceArray((tokens, vocab), np.float32).zero() for _ in range(2))
+    size = 4 * vocab
+    for d, a in ((logits, c["logits"]), (draft, c["draft_logits"])):
+        rt.check(rt.library().lh_copy_to_device(d.ptr + first * size, np.ascontiguousarray(a).ctypes.data, a.nbytes))
+    ids, parents, accept = np.zeros(tokens, np.int32), np.full(tokens, -1, np.int32), np.zeros(tokens, np.float32)
+    ids[first:first + 7], parents[first:first + 7], accept[first:first + 7] = c["ids"], c["parents"], c["accept"]
+    d = {"ids": ints(rt, ids), "parents": ints(rt, parents), "accept": rt.DeviceArray.of(accept), "temperatures": rt.DeviceArray.of(c["temperatures"]),
+         "sample": rt.DeviceArray.of(c["sample"]), "path": ints(rt, ids), "kept": ints(rt, [0]), "next": ints(rt, [0])}
+    starts, rows = ints(rt, [first, tokens]), ints(rt, [7])
+    batch = rt.KvBatch(requests=1, tokens=tokens, max_rows=7, block=16, blocks=1, width=1, starts=starts.ptr, rows=rows.ptr)
+    rt.verify_drafts(batch, rt.Drafts(vocab=vocab, logits=logits.ptr, draft_logits=draft.ptr, **{k: v.ptr for k, v in d.items()}))
+    rt.synchronize()
+    path, following = drafts.verify(c["logits"], c["draft_logits"], c["ids"], c["parents"], c["temperatures"][0], c["accept"], c["sample"][0])
+    assert d["kept"].numpy()[0] == len(path) and d["next"].numpy()[0] == following
+    assert list(d["path"].numpy()[first:first + len(path)]) == path
+
+
+def test_cache_far_offsets(rt):
+    # codes past 4 GiB from the start of the pool: attention of a tree, then its rows kept
+    heads, kv, dim, block = 4, 2, 128, 64
+    blocks = (5 << 30) // (kv * dim * block)
+    rng = np.random.default_rng(55)
+    dk, dv = (rt.DeviceArray((blocks, kv, block, dim), np.uint8) for _ in range(2))
+    flat = np.full((blocks, kv), 2.0 ** -5, np.float32)
+    pages = np.array([blocks - 1, 3, blocks - 2, blocks // 2 + 5])
+    flat[pages[2]] = 2.0 ** -4
+    ks, vs = (rt.DeviceArray.of(flat) for _ in range(2))
+    small = kv8.cache_of(rng, 4, kv, block, dim, ref.INT8)
+    size = kv * dim * block
+    for i, page in enumerate(pages):
+        for d, a in ((dk, small[0]), (dv, small[1])):
+            rt.check(rt.library().lh_copy_to_device(d.ptr + int(page) * size, np.ascontiguousarray(a[i]).ctypes.data, size))
+    rows, length, path = 40, 160, [0, 5, 39]
+    depth, seen = drafts.plan(drafts.random_tree(rng, rows, 4))
+    q = rng.standard_normal((heads, rows, dim)).astype(np.float32)
+    d = {"table": ints(rt, pages[None]), "lengths": ints(rt, [length]), "starts": ints(rt, [0, rows]), "rows": ints(rt, [rows])}
+    dq, out, masks = rt.DeviceArray.of(q), rt.DeviceArray((rows, heads, dim), np.float32), rt.DeviceArray.of(drafts.packed(seen, 1))
+    batch = rt.KvBatch(requests=1, tokens=rows, max_rows=rows, block=block, blocks=blocks, width=4, **{k: v.ptr for k, v in d.items()})
+    cache = rt.Kv8(dk.ptr, dv.ptr, ks.ptr, vs.ptr, kv, dim, ref.INT8)
+    rt.attention_kv8_tree(batch, cache, dq, heads, masks, out)
+    own = np.array([[2.0 ** -5] * kv] * 4, np.float32)
+    own[2] = 2.0 ** -4
+    want, table = np.zeros((rows, heads, dim)), np.arange(4)[None]
+    A = drafts.attention(q, small[0], small[1], own, own, table, [length], [0, rows], [rows], [seen], length - rows + depth, block, ref.INT8, 0, want)
+    assert np.max(np.abs(out.numpy() - want)) <= kv8.bound(A, length, 127 * 2.0 ** -4)
+    rt.kv8_compact(batch, [cache], ints(rt, path + [-1] * (rows - 3)), ints(rt, [3]))
+    rt.synchronize()
+    for d, i, transposed in ((dk, 0, False), (dv, 1, True)):
+        codes, scales = small[i].copy(), own.copy()
+        drafts.compact(codes, scales, table, [length], [0], [rows], np.array(path + [-1] * (rows - 3)), [3], block, ref.INT8, transposed)
+        for j, page in enumerate(pages):
+            got = np.empty_like(codes[j])
+            rt.check(rt.library().lh_copy_to_host(got.ctypes.data, d.ptr + int(page) * size, size))
+            assert np.array_equal(got, codes[j]), (i, j)
