@@ -13,14 +13,24 @@
 // sums in order pass u times all, and among 10^5 tokens an f32 sum would often be
 // on the other side of it.
 //
-// Only the rows on a walk's way are read, and a walk's rows come one after the
-// other.  Several workgroups share a request: each has a segment of the
-// vocabulary, and all of them walk.  What a walk needs of the whole vocabulary (a row's largest value and sums, the sum of
-// what a refusal has left) they exchange through slots in memory, one for each
-// segment and exchange of the walk, each word of which tells by itself whether it
-// has been written.  A workgroup that does not find another's words in time (it
-// may not have started) computes them itself: the same operations on the same
-// values give the same words, and no workgroup depends on another's progress.
+// A walk's rows come one after the other, and only those on its way are read
+// (unless all are few: then a launch measures them beforehand, see kAhead).
+// Several workgroups share a request: each has a segment of the vocabulary, and
+// all of them walk.  What a walk needs of the whole vocabulary (a row's largest
+// value and sums, the sum of what a refusal has left) they exchange through slots
+// in memory, one for each segment and exchange of the walk, each word of which
+// tells by itself whether it has been written.  A workgroup that does not find
+// another's words in time (it may not have started) computes them itself: the
+// same operations on the same values give the same words, and no workgroup
+// depends on another's progress.
+//
+// What bounds it: the latency of an exchange, some 6 us of loads, reductions, a
+// store and the others' loads that see it, for each row and refusal of the longest
+// walk; with 64 requests, 32000 tokens and both models' logits 11 us a row, of
+// which 2 are 64-bit arithmetic (20 instructions a weight).  64 trees of 8 rows take 51 us,
+// 16 of 26 over 151936 tokens 35 to 40, 100 greedy chains of 4 over 49152 31, a chain of 5
+// by itself 18 to 27.  A workgroup of 512 threads with the weights of its segment in
+// registers spilled, and took 91 us for the 51.
 #include <algorithm>
 #include <cfloat>
 #include <cstdlib>
@@ -103,8 +113,17 @@ struct Shared {
 
 struct How {
     int segments, size;                             // of the vocabulary, and values of one: a multiple of kWaves
+    bool ahead;                                     // a launch before the walk measures every row
     long long wait;                                 // cycles until a workgroup computes what others owe
 };
+// The workspace: slots [2 tokens exchanges][segment][kWords], a request's from 2 starts on (a walk looks at each row once
+// at most, and refuses each once at most); behind them, where rows are measured ahead, their words [tokens][segment][kWords].
+__device__ __forceinline__ uint64_t* slots_of(const VerifyCall& p, const How& how, int start) {
+    return (uint64_t*)p.workspace + (size_t)2 * start * how.segments * kWords;
+}
+__device__ __forceinline__ uint64_t* words_of(const VerifyCall& p, const How& how, int token) {
+    return slots_of(p, how, p.batch.tokens) + (size_t)token * how.segments * kWords;
+}
 
 // One walk, by one of its workgroups.  Every workgroup of a request holds the same values here.
 struct Walk {
@@ -348,12 +367,20 @@ struct Walk {
     }
 
     // The distributions at a row; false: there is none.
+    template <bool AHEAD>
     __device__ __forceinline__ bool look(int row, bool draft, int next) {
         target = p.logits + (size_t)(start + row) * p.vocab;
         drafted = draft ? p.draft + (size_t)(start + row) * p.vocab : nullptr;
         scale = used = 0.0;
         refusals = 0;
-        trade<false>(-1, next);
+        if (AHEAD) {
+            __syncthreads();                        // the last exchange is read
+            const uint64_t* words = words_of(p, how, start + row);
+            for (int i = threadIdx.x; i < how.segments * kWords; i += kThreads) s.words[i % kWords][i / kWords] = words[i];
+            __syncthreads();
+        } else {
+            trade<false>(-1, next);
+        }
         const int lane = threadIdx.x & 63, segments = how.segments;
         float a[kMostSegments / 64], b[kMostSegments / 64];
         most_w = greedy ? -INFINITY : -FLT_MAX;
@@ -517,12 +544,46 @@ struct Walk {
     }
 };
 
+// A request's rows, [start, start + rows); rows is 0 where the arrays name rows that the batch has no room for.
+struct Rows {
+    int start, rows;
+};
+__device__ __forceinline__ Rows rows_of(const KvBatchView& b, int request) {
+    Rows r{b.starts[request], b.rows[request]};
+    if (r.rows < 0 || r.rows > b.max_rows || r.start < 0 || r.start > b.tokens - r.rows) r.rows = 0;
+    return r;
+}
+
+// Every row's words, each segment by a workgroup; and the slots that the walk needs, empty.
+__global__ __launch_bounds__(kThreads, 2) void verify_rows_kernel(VerifyCall p, How how) {
+    __shared__ Shared s;
+    const int segment = blockIdx.x % how.segments, row = blockIdx.x / how.segments % p.batch.max_rows;
+    const int request = blockIdx.x / how.segments / p.batch.max_rows;
+    const Rows own = rows_of(p.batch, request);
+    if (row >= own.rows) return;
+    const float temperature = p.temperatures[request];
+    uint64_t* const slots = slots_of(p, how, own.start) + (size_t)2 * row * how.segments * kWords;
+    if (threadIdx.x < 2 * kWords) slots[(threadIdx.x / kWords * how.segments + segment) * kWords + threadIdx.x % kWords] = kEmpty;
+    if (threadIdx.x < kTable) s.table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+    Walk walk(p, s, how, nullptr, segment, own.start, temperature);
+    bool parent = false;                            // of a row behind
+    for (int i = row + 1 + threadIdx.x; i < own.rows; i += kThreads) parent = parent || p.parents[own.start + i] == row;
+    parent = __syncthreads_or(parent);
+    walk.target = p.logits + (size_t)(own.start + row) * p.vocab;
+    walk.drafted = p.draft && parent && !walk.greedy ? p.draft + (size_t)(own.start + row) * p.vocab : nullptr;
+    uint64_t out[kWords];
+    walk.measure(segment, out);
+    if (threadIdx.x == 0)
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) words_of(p, how, own.start + row)[(size_t)segment * kWords + i] = out[i];
+}
+
+template <bool AHEAD>
 __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How how) {
     __shared__ Shared s;
     const int request = blockIdx.x / how.segments, own = blockIdx.x % how.segments, lane = threadIdx.x & 63;
-    const int start = p.batch.starts[request];
-    int rows = p.batch.rows[request];
-    if (rows < 0 || rows > p.batch.max_rows || start < 0 || start > p.batch.tokens - rows) rows = 0;
+    const Rows mine = rows_of(p.batch, request);
+    const int start = mine.start, rows = mine.rows;
     if (rows == 0) {
         if (own == 0 && threadIdx.x == 0) {
             p.kept[request] = 0;
@@ -531,8 +592,7 @@ __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How h
         return;
     }
     const float temperature = p.temperatures[request];
-    uint64_t* const slots = (uint64_t*)p.workspace + (size_t)2 * start * how.segments * kWords;
-    Walk walk(p, s, how, slots, own, start, temperature);
+    Walk walk(p, s, how, slots_of(p, how, start), own, start, temperature);
     for (int i = threadIdx.x; i < rows; i += kThreads) {
         s.parents[i] = p.parents[start + i];
         s.ids[i] = p.ids[start + i];
@@ -564,7 +624,7 @@ __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How h
                 l = p.logits[at];
                 if (with_draft) d = p.draft[at];
             }
-            if (!known && !wrong) wrong = !walk.look(row, with_draft && child < rows, child < rows ? child : -1);
+            if (!known && !wrong) wrong = !walk.look<AHEAD>(row, with_draft && child < rows, child < rows ? child : -1);
             known = true;
             if (wrong || child == rows) break;
             double r;
@@ -592,28 +652,42 @@ __global__ void empty_slots_kernel(uint64_t* slots, size_t count) {
 // Workgroups that the requests' vocabularies are cut for: as many as the GPU has CUs (each has registers for one), of
 // at least 2048 values each.
 constexpr int kTarget = 256, kLeast = 2048;
+// Bytes of logits up to which every row is measured ahead of the walk, side by side, although it may not come to all
+// of them.  Ahead / as the walk comes: one chain of 4 rows over 32000 tokens, both models' logits (1 MB), all taken,
+// 19 / 30 us, 64 of them (65 MB) 39 / 48, 100 greedy chains of 4 over 49152 (79 MB) 27 / 31, 64 trees of 8 over 32000 (115
+// MB) 73 / 50, 16 trees of 26 over 151936 (253 MB) 106 / 40.
+constexpr int64_t kAhead = 64 << 20;
 How how_of(const VerifyCall& call) {
     const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, kTarget / call.batch.requests)});
-    How how{most, 0, 200000};
+    How how{most, 0, false, 200000};
     how.size = ((call.vocab + most - 1) / most + kWaves - 1) / kWaves * kWaves;
     how.segments = (call.vocab + how.size - 1) / how.size;
+    // (not where its workgroups, for max_rows of every request, are mostly for rows that no request has)
+    how.ahead = call.batch.max_rows > 1 && (int64_t)call.batch.tokens * call.vocab * (call.draft ? 8 : 4) <= kAhead &&
+                (int64_t)call.batch.requests * call.batch.max_rows <= 4LL * call.batch.tokens;
     return how;
 }
-size_t slot_words(const VerifyCall& call) {
-    const int segments = how_of(call).segments;
-    return segments > 1 ? (size_t)2 * call.batch.tokens * segments * kWords : 0;
+size_t workspace_words(const VerifyCall& call, const How& how) {
+    if (how.segments == 1 && !how.ahead) return 0;
+    return (size_t)(how.ahead ? 3 : 2) * call.batch.tokens * how.segments * kWords;
 }
 
 }  // namespace
 
-size_t verify_workspace_bytes(const VerifyCall& call) { return 8 * slot_words(call); }
+size_t verify_workspace_bytes(const VerifyCall& call) { return 8 * workspace_words(call, how_of(call)); }
 
 void launch_verify(const VerifyCall& call, hipStream_t stream) {
     How how = how_of(call);
     if (const char* cycles = std::getenv("LEAF_VERIFY_WAIT")) how.wait = std::atoll(cycles);
-    if (const size_t words = slot_words(call))
+    const int grid = call.batch.requests * how.segments;
+    if (how.ahead) {
+        verify_rows_kernel<<<grid * call.batch.max_rows, kThreads, 0, stream>>>(call, how);
+        verify_kernel<true><<<grid, kThreads, 0, stream>>>(call, how);
+        return;
+    }
+    if (const size_t words = workspace_words(call, how))
         empty_slots_kernel<<<(int)std::min<size_t>((words + 1023) / 1024, 1024), 256, 0, stream>>>((uint64_t*)call.workspace, words);
-    verify_kernel<<<call.batch.requests * how.segments, kThreads, 0, stream>>>(call, how);
+    verify_kernel<false><<<grid, kThreads, 0, stream>>>(call, how);
 }
 
 }  // namespace leafhip
