@@ -1097,12 +1097,13 @@ __global__ __launch_bounds__(kThreads) void attention_kv8_rows_merge_kernel(Atte
 constexpr int kTreeChunk = 16;
 __global__ __launch_bounds__(kThreads) void attention_kv8_tree_merge_kernel(AttentionKv8Call p, Share share) {
     const int group = p.heads / p.cache.kv_heads, dim = p.cache.dim, quads = dim / 4;
-    const int request = blockIdx.x, kvh = blockIdx.y;
+    const int request = blockIdx.z, kvh = blockIdx.y;
     const int* plan = (const int*)p.partial + share.at;
     const int per = plan[0], item = plan[kHeader + request];
     const Kv8Request q = kv8_request(p.batch, request);
     const int rows = q.rows * group, tiles = tiles_of(q, group, share);
-    const int unit = blockIdx.z * kThreads + threadIdx.x, row = unit / quads, quad = unit - row * quads;
+    const int64_t unit = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int row = (int)(unit / quads), quad = (int)(unit - (int64_t)row * quads);
     if (!tiles || row >= rows) return;
     const Steps seen = steps_of<true>(q, group, p.window, share.tile_rows, 0);
     const int parts = parts_of(seen.end - seen.begin, per);
@@ -1284,7 +1285,7 @@ static void launch_attention(const AttentionKv8Call& call, hipStream_t stream) {
         const Share& share = shares.few.items ? shares.few : shares.many;
         const int64_t units = (int64_t)group * call.batch.max_rows * (dim / 4);
         if (steps > (size_t)share.least)
-            attention_kv8_tree_merge_kernel<<<dim3(call.batch.requests, call.cache.kv_heads, (uint32_t)((units + kThreads - 1) / kThreads)),
+            attention_kv8_tree_merge_kernel<<<dim3((uint32_t)((units + kThreads - 1) / kThreads), call.cache.kv_heads, call.batch.requests),
                                               kThreads, 0, stream>>>(call, share);
         return;
     }

@@ -332,6 +332,7 @@ struct Walk {
                     uint64_t word = out[0];
                     if (threadIdx.x == 1) word = out[1];
                     if (threadIdx.x == 2) word = out[2];
+                    if (word == kEmpty) word = kNaN;    // (some NaN's bits: no distribution)
                     s.words[threadIdx.x][segment] = word;
                     if (segments > 1 && segment == own)
                         __hip_atomic_store(slot + segment * kWords + threadIdx.x, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -83,6 +83,52 @@ result = [status(s) for s in (lib.lh_kv_tree(None, p, p, None), lib.lh_attention
     assert all(code == 1 and launched == 0 for code, _, launched in results), results
 
 
+@pytest.mark.parametrize("sizes,heads,kernels", [
+    ("requests=64, tokens=512, max_rows=8, width=64", 4, ["few_kernel", "tree_merge"]),        # 16 rows of a KV head
+    ("requests=64, tokens=512, max_rows=8, width=8", 4, ["few_kernel"]),                       # too short to be parted
+    ("requests=64, tokens=512, max_rows=9, width=64", 4, ["tree_kernel", "tree_merge"]),
+    ("requests=64, tokens=512, max_rows=9, width=20", 4, ["tree_kernel"]),
+    ("requests=51, tokens=300, max_rows=200, width=64", 4, ["tree_kernel", "tree_merge"]),
+    ("requests=64, tokens=64, max_rows=1, width=64", 34, ["tree_kernel", "tree_merge"])])      # groups of 17
+def test_attention_routes(fake_hip, sizes, heads, kernels):  # noqa: F811
+    launched = fake_hip(TREE_CALLS + f"""
+b, code = batch({sizes}), None
+code = lib.lh_attention_kv8_tree(C.byref(b), C.byref(cache()), buffer.ptr, {heads}, 0, buffer.ptr, buffer.ptr, None, 0, None)
+result = [code, kernels()]
+""")
+    assert launched[0] == 0 and len(launched[1]) == len(kernels), launched
+    assert all(f"attention_kv8_{name}" in k for name, k in zip(kernels, launched[1])), launched
+
+
+@pytest.mark.parametrize("sizes,vocab,draft,kernels", [
+    ("requests=1, tokens=5, max_rows=5", 32000, True, ["verify_rows", "verify_kernel"]),       # few logits: every row ahead
+    ("requests=64, tokens=512, max_rows=8", 32000, True, ["empty_slots", "verify_kernel"]),
+    ("requests=64, tokens=64, max_rows=1", 32000, False, ["empty_slots", "verify_kernel"]),    # no drafts: sampling alone
+    ("requests=300, tokens=600, max_rows=512", 20000, False, ["verify_kernel"]),               # a workgroup for a request
+    ("requests=1, tokens=1, max_rows=1", 2048, False, ["verify_kernel"]),
+    ("requests=300, tokens=600, max_rows=512", 2000, False, ["verify_kernel"])])               # mostly rows that no request has
+def test_verification_routes(fake_hip, sizes, vocab, draft, kernels):  # noqa: F811
+    launched = fake_hip(TREE_CALLS + f"""
+b, d = batch({sizes}), drafts(vocab={vocab}, draft_logits={"buffer.ptr" if draft else None})
+n = C.c_size_t()
+result = [lib.lh_verify_drafts_workspace(C.byref(b), C.byref(d), C.byref(n)), n.value, lib.lh_verify_drafts(C.byref(b), C.byref(d), None, 0, None), kernels()]
+""")
+    assert launched[0] == launched[2] == 0 and len(launched[3]) == len(kernels), launched
+    assert all(name in k for name, k in zip(kernels, launched[3])), launched
+    assert (launched[1] > 0) == (len(kernels) > 1)
+
+
+def test_workspace_does_not_depend_on_lengths(fake_hip):  # noqa: F811
+    sizes, error = fake_hip(TREE_CALLS + """
+n, result = C.c_size_t(), []
+for width in (64, 4096, 2**20):
+    assert lib.lh_attention_kv8_tree_workspace(C.byref(batch(requests=64, tokens=512, max_rows=9, width=width)), C.byref(cache(keys=None, values=None)), 8, C.byref(n)) == 0
+    result.append(n.value)
+result = [result, lib.lh_attention_kv8_tree_workspace(C.byref(batch()), C.byref(cache()), 8, None)]
+""")
+    assert sizes[1] == sizes[2] <= 64 << 20 and sizes[0] <= sizes[1] and error == 1
+
+
 # ---- the plain forms themselves
 def test_plans():
     depth, seen = drafts.plan([-1, 0, 0, 1, 7, 3])          # row 4's parent is no earlier row
