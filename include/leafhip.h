@@ -496,8 +496,8 @@ typedef struct lh_drafts {
  * A token outside the vocabulary is not taken.  Where a test or the token behind needs logits of
  * which one is NaN or plus infinity or all are minus infinity, or a T that is negative or
  * not finite, the walk ends, with next -1.  A request without rows has kept 0 and next -1.
- * Reads the batch's starts and rows; the rows' entries of requests that have none, and padding's, stay as they were.
- * The workspace is lh_attention_kv8's: the caller's, 16-byte aligned, of lh_verify_drafts_workspace
+ * Reads the batch's starts and rows (requests' rows do not overlap; those that do not fit the batch count as none); padding rows'
+ * entries of path stay as they were.  The workspace is lh_attention_kv8's: the caller's, 16-byte aligned, of lh_verify_drafts_workspace
  * bytes, or with NULL (and 0) the scratch of the stream. */
 lh_status lh_verify_drafts(const lh_kv_batch* batch, const lh_drafts* drafts, void* workspace, size_t workspace_bytes,
                            lh_stream stream);

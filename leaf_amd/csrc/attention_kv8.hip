@@ -31,7 +31,8 @@
 // Two kernels: attention_kv8_few_kernel takes requests of at most 16 rows of a KV
 // head and reads the cache straight into registers; attention_kv8_rows_kernel takes
 // the others, or every request (see kManyTokens), and shares what it widens through
-// LDS.  The keys of a tile of rows are cut into
+// LDS.  (Trees: attention_kv8_few_kernel where no request may have more than 16 rows, else
+// attention_kv8_tree_kernel for every request.)  The keys of a tile of rows are cut into
 // parts where a batch has too few tiles for the GPU, and a second launch joins
 // the parts.  Lengths are known on the device only: every workgroup sums the
 // batch and finds its own part (dependent loads, part of the 7 us that the smallest call takes).
@@ -788,8 +789,16 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
         if (FULL || t < tiles) *(v4f*)(to + 16 * t + 4 * lq) = o[t] * scale;
 }
 
-// ---- the same of trees: of up to 32 rows of a KV head two waves for 16 of them, each with half of a step's keys; codes are
-// loaded two steps ahead
+// ---- the same of trees (lh_attention_kv8_tree): of up to 32 rows of a KV head two waves for 16 of them, each with half of
+// a step's keys; codes are loaded two steps ahead
+// 64 requests of 5 to 8 rows over 200 to 4096 keys, 32 heads of 128 over 8 (INT8): 85 us and 10 for the join, 293 MB at
+// 3.2 TB/s; 16 of 45 to 64 rows over 500 to 8000 keys, 32 heads of 64 over 4 (E4M3): 92 and 10.  The kernel of causal rows
+// with masks took 124 and 110 for these: what two steps of loads in flight, half the keys to a wave where two of four
+// would have no rows, and the join without a search gave.  What bounds them: CUs have waves for some three quarters of the
+// kernel's time (parts are a half to the whole of the longest, and start behind four dependent loads); in it vector
+// instructions take 41% and 48% of the cycles, MFMAs 17% and 22%.  Measured and left: the codes of a step in registers
+// for two or four row tiles of one wave, without LDS or barriers (103 and 107 us, with spills), and the split of keys into
+// more parts (kTreeTarget).
 template <int CC, bool FULL, bool E4M3, int SPLIT>
 __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC, NJ = 4 / SPLIT, NH = NJ / 2;     // of a wave: tiles of 16 keys, operands of 32

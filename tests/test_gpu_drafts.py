@@ -130,6 +130,15 @@ def test_attention(rt, form, batch, heads, kv, dim, block, window):
     check_attention(rt, tree_case(rng, BATCHES[batch], heads, kv, dim, block, form, padding=3), block, form, window)
 
 
+@pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
+@pytest.mark.parametrize("heads,kv,dim,block", [(6, 2, 192, 32), (8, 2, 176, 64), (4, 1, 240, 16), (6, 2, 144, 128), (6, 3, 48, 16), (80, 1, 64, 64)])
+def test_attention_of_other_heads(rt, form, heads, kv, dim, block):
+    # up to 32 rows of a KV head, and more
+    rng = np.random.default_rng(dim + heads)
+    for batch in ([(700, 6), (90, 7), (6, 6)], [(500, 33), (150, 20), (1100, 7)]):
+        check_attention(rt, tree_case(rng, batch, heads, kv, dim, block, form, padding=1), block, form)
+
+
 @pytest.mark.parametrize("requests,heads,kv", [([(900, 1)], 4, 2), ([(300, 1), (64, 1), (2000, 1), (5, 1)], 20, 1),
                                                ([(1 + i % 90, 1 + i % 7) for i in range(600)], 6, 1)])
 @pytest.mark.parametrize("padding", [0, 1000])
