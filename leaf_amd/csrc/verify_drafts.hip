@@ -26,12 +26,13 @@
 //
 // What bounds it: the latency of an exchange, some 6 us of loads, reductions, a
 // store and the others' loads that see it, for each row and refusal of the longest
-// walk; with 64 requests, 32000 tokens and both models' logits 11 us a row, of
-// which 2 are 64-bit arithmetic (20 instructions a weight).  64 trees of 8 rows take 51 us,
-// 16 of 26 over 151936 tokens 35 to 40, 100 greedy chains of 4 over 49152 31, a chain of 5
-// by itself 18 to 27.  A workgroup of 512 threads with the weights of its segment in
-// registers spilled, and took 91 us for the 51.
+// walk; with 64 requests, 32000 tokens and both models' logits 9 us a row, of which 3 to 4 are 16
+// MB of logits and, by count, 2 are 64-bit arithmetic.  64 trees of 8 rows take 41 us, 16 of 26 over 151936
+// tokens 38 to 40, 100 greedy chains of 4 over 49152 28.5, a chain of 5 by itself 18 to 21.  Loading
+// the row that a walk may come to next while it waits made all of them slower (48 us for the 41 with a quarter of it,
+// 67 with all): the words that it waits for come behind those loads.
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cstdlib>
 
@@ -46,6 +47,7 @@ constexpr int kMostSegments = 128;
 constexpr int kWords = 3;                           // of a slot
 constexpr int kBatch = 4;                           // values of a row that a thread has in flight
 constexpr int kTable = 256;                         // powers of two of a step
+constexpr int kHeld = 16;                           // values of a row that a thread keeps the weights of, in LDS
 constexpr uint64_t kEmpty = ~0ull;                  // a word that is not written: no value's bits (NaN is stored as kNaN)
 constexpr uint32_t kNaN = 0x7fc00000u;
 
@@ -126,6 +128,8 @@ __device__ __forceinline__ uint64_t* words_of(const VerifyCall& p, const How& ho
 }
 
 // One walk, by one of its workgroups.  Every workgroup of a request holds the same values here.
+// HELD: a segment has at most kHeld values for a thread, whose weights stay in LDS while the walk is at their row.
+template <bool HELD>
 struct Walk {
     const VerifyCall& p;
     Shared& s;
@@ -143,6 +147,10 @@ struct Walk {
     int best = 0;                                   // greedy: the first largest
     double scale = 0.0, used = 0.0, left = 0.0;     // K, C and the sum of r
     int refusals = 0;
+    // HELD: the segment whose weights are kept, relative to the wave's largest values
+    int held = -1;
+    float held_w = 0.0f, held_v = 0.0f;
+    double* weights = nullptr;                      // [2][kHeld][kThreads]
 
     __device__ __forceinline__ Walk(const VerifyCall& p_, Shared& s_, const How& how_, uint64_t* slots_, int own_, int start_, float temperature)
         : p(p_), s(s_), how(how_), slots(slots_), own(own_), start(start_), c(1.4426950408889634 / (double)temperature),
@@ -207,7 +215,7 @@ struct Walk {
 
     // The words of a segment's slot: largest values (at least -FLT_MAX), and sums of the weights relative to them (in
     // `sums` those of each wave's share).
-    __device__ __forceinline__ void measure(int segment, uint64_t (&out)[kWords]) const {
+    __device__ __forceinline__ void measure(int segment, uint64_t (&out)[kWords]) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const bool draft = drafted != nullptr;
         Part a_w, a_v;
@@ -228,6 +236,38 @@ struct Walk {
             });
             top_w = all_max(a_w.wrong ? INFINITY : a_w.most);      // (plus infinity: no distribution)
             at = all_min(a_w.most == top_w ? at : p.vocab);
+        } else if (HELD && draft) {
+            const int begin = share_begin(segment, wave), end = share_begin(segment, wave + 1);
+            float l[kHeld], d[kHeld];
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const int x = min(begin + lane + 64 * i, p.vocab - 1);
+                l[i] = target[x];
+                d[i] = drafted[x];
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (begin + lane + 64 * i >= end) l[i] = d[i] = -INFINITY;
+                a_w.wrong = a_w.wrong || !(l[i] < INFINITY);
+                a_v.wrong = a_v.wrong || !(d[i] < INFINITY);
+                a_w.most = fmaxf(a_w.most, l[i]);
+                a_v.most = fmaxf(a_v.most, d[i]);
+            }
+            held = segment;
+            held_w = top_w = all_max(a_w.wrong ? INFINITY : a_w.most);
+            held_v = top_v = all_max(a_v.wrong ? INFINITY : a_v.most);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (begin + 64 * i >= end) continue;
+                const double w = weight(l[i], top_w), v = weight(d[i], top_v);
+                weights[i * kThreads + threadIdx.x] = w;
+                weights[(kHeld + i) * kThreads + threadIdx.x] = v;
+                sum_w += w;
+                sum_v += v;
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (more at a time need more registers than there are)
+            }
+            sum_w = all_sum(sum_w);
+            sum_v = all_sum(sum_v);
         } else {
             if (draft)
                 stream<true, kBatch>(segment, [&](const float (&l)[kBatch], const float (&d)[kBatch], int) {
@@ -278,10 +318,18 @@ struct Walk {
     __device__ __forceinline__ double left_of(int x) const { return left_of(x, target[x], scale > 0.0 ? drafted[x] : 0.0f); }
 
     // The sum of what is left of a segment (in `sums` of each wave's share).
-    __device__ __forceinline__ void measure_left(int segment, uint64_t (&out)[kWords]) const {
+    __device__ __forceinline__ void measure_left(int segment, uint64_t (&out)[kWords]) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         double sum = 0.0;
-        if (scale > 0.0)
+        if (HELD && scale > 0.0) {
+            if (held != segment) measure(segment, out);            // (so that whoever computes a word gets its bits)
+            const int begin = share_begin(segment, wave), end = share_begin(segment, wave + 1);
+            const double fw = weight(held_w, most_w), fv = scale * weight(held_v, most_v);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)         // (a value behind the end weighs nothing)
+                if (begin + 64 * i < end)
+                    sum += fmax(weights[i * kThreads + threadIdx.x] * fw - weights[(kHeld + i) * kThreads + threadIdx.x] * fv, 0.0);
+        } else if (scale > 0.0)
             stream<true, kBatch>(segment, [&](const float (&l)[kBatch], const float (&d)[kBatch], int) {
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) sum += fmax(weight(l[i], most_w) - scale * weight(d[i], most_v), 0.0);
@@ -299,23 +347,9 @@ struct Walk {
         out[1] = out[2] = 0;
     }
 
-    // Brings the first values of a row's own segment near, while others' words are waited for.
-    __device__ __forceinline__ void touch(int row, bool draft) const {
-        const int x = min(share_begin(own, threadIdx.x >> 6) + (int)(threadIdx.x & 63), p.vocab - 1);
-        const size_t at = (size_t)(start + row) * p.vocab;
-        float near = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const size_t y = at + min(x + 64 * i, p.vocab - 1);
-            near = fmaxf(near, p.logits[y]);
-            if (draft) near = fmaxf(near, p.draft[y]);
-        }
-        asm volatile("" ::"v"(near));
-    }
-
     // An exchange: of a row's largest values and sums, or (LEFT) of what is left, of every segment or of `only` one.
     template <bool LEFT>
-    __device__ __forceinline__ void trade(int only, int next = -1) {
+    __device__ __forceinline__ void trade(int only) {
         constexpr int words = LEFT ? 1 : kWords;
         const int segments = how.segments;
         uint64_t* const slot = slots + (size_t)exchange * segments * kWords;
@@ -341,7 +375,6 @@ struct Walk {
                 __syncthreads();                    // the last exchange is read
             }
             if (!waited) {
-                if (next >= 0) touch(next, drafted != nullptr);
                 for (int i = threadIdx.x; i < segments * words; i += kThreads) {
                     const int of = i / words, word = i - of * words;
                     if (of == own || (only >= 0 && of != only)) continue;
@@ -369,18 +402,19 @@ struct Walk {
 
     // The distributions at a row; false: there is none.
     template <bool AHEAD>
-    __device__ __forceinline__ bool look(int row, bool draft, int next) {
+    __device__ __forceinline__ bool look(int row, bool draft) {
         target = p.logits + (size_t)(start + row) * p.vocab;
         drafted = draft ? p.draft + (size_t)(start + row) * p.vocab : nullptr;
         scale = used = 0.0;
         refusals = 0;
+        held = -1;
         if (AHEAD) {
             __syncthreads();                        // the last exchange is read
             const uint64_t* words = words_of(p, how, start + row);
             for (int i = threadIdx.x; i < how.segments * kWords; i += kThreads) s.words[i % kWords][i / kWords] = words[i];
             __syncthreads();
         } else {
-            trade<false>(-1, next);
+            trade<false>(-1);
         }
         const int lane = threadIdx.x & 63, segments = how.segments;
         float a[kMostSegments / 64], b[kMostSegments / 64];
@@ -566,7 +600,7 @@ __global__ __launch_bounds__(kThreads, 2) void verify_rows_kernel(VerifyCall p, 
     uint64_t* const slots = slots_of(p, how, own.start) + (size_t)2 * row * how.segments * kWords;
     if (threadIdx.x < 2 * kWords) slots[(threadIdx.x / kWords * how.segments + segment) * kWords + threadIdx.x % kWords] = kEmpty;
     if (threadIdx.x < kTable) s.table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
-    Walk walk(p, s, how, nullptr, segment, own.start, temperature);
+    Walk<false> walk(p, s, how, nullptr, segment, own.start, temperature);
     bool parent = false;                            // of a row behind
     for (int i = row + 1 + threadIdx.x; i < own.rows; i += kThreads) parent = parent || p.parents[own.start + i] == row;
     parent = __syncthreads_or(parent);
@@ -579,9 +613,10 @@ __global__ __launch_bounds__(kThreads, 2) void verify_rows_kernel(VerifyCall p, 
         for (int i = 0; i < kWords; ++i) words_of(p, how, own.start + row)[(size_t)segment * kWords + i] = out[i];
 }
 
-template <bool AHEAD>
+template <bool AHEAD, bool HELD>
 __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How how) {
     __shared__ Shared s;
+    extern __shared__ double weights[];
     const int request = blockIdx.x / how.segments, own = blockIdx.x % how.segments, lane = threadIdx.x & 63;
     const Rows mine = rows_of(p.batch, request);
     const int start = mine.start, rows = mine.rows;
@@ -593,7 +628,8 @@ __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How h
         return;
     }
     const float temperature = p.temperatures[request];
-    Walk walk(p, s, how, slots_of(p, how, start), own, start, temperature);
+    Walk<HELD> walk(p, s, how, slots_of(p, how, start), own, start, temperature);
+    walk.weights = weights;
     for (int i = threadIdx.x; i < rows; i += kThreads) {
         s.parents[i] = p.parents[start + i];
         s.ids[i] = p.ids[start + i];
@@ -625,7 +661,7 @@ __global__ __launch_bounds__(kThreads, 2) void verify_kernel(VerifyCall p, How h
                 l = p.logits[at];
                 if (with_draft) d = p.draft[at];
             }
-            if (!known && !wrong) wrong = !walk.look<AHEAD>(row, with_draft && child < rows, child < rows ? child : -1);
+            if (!known && !wrong) wrong = !walk.template look<AHEAD>(row, with_draft && child < rows);
             known = true;
             if (wrong || child == rows) break;
             double r;
@@ -650,16 +686,18 @@ __global__ void empty_slots_kernel(uint64_t* slots, size_t count) {
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (size_t)gridDim.x * blockDim.x) slots[i] = kEmpty;
 }
 
-// Workgroups that the requests' vocabularies are cut for: as many as the GPU has CUs (each has registers for one), of
-// at least 2048 values each.
-constexpr int kTarget = 256, kLeast = 2048;
+// Workgroups that the requests' vocabularies are cut for: as many as the GPU has CUs, of at least 2048 values each; twice as
+// many where each had more than 32768.  With 256 / 512: 64 trees of 8 rows over 32000 tokens, both models' logits, 41 / 62
+// us, 100 chains of 4 over 49152 greedy 28.5 / 28.8, 100 chains of 4 over 151936 136 / 104.
+constexpr int kTarget = 256, kLeast = 2048, kLong = 32768;
 // Bytes of logits up to which every row is measured ahead of the walk, side by side, although it may not come to all
-// of them.  Ahead / as the walk comes: one chain of 4 rows over 32000 tokens, both models' logits (1 MB), all taken,
-// 19 / 30 us, 64 of them (65 MB) 39 / 48, 100 greedy chains of 4 over 49152 (79 MB) 27 / 31, 64 trees of 8 over 32000 (115
-// MB) 73 / 50, 16 trees of 26 over 151936 (253 MB) 106 / 40.
-constexpr int64_t kAhead = 64 << 20;
+// of them.  Ahead / as the walk comes, over 32000 tokens with both models' logits, chains of 8 rows that all stand: one (2
+// MB) 28 / 59 us, 16 (33 MB) 43 / 61, 64 (131 MB, in an earlier state) 73 / 50 of trees that do not.  Where a third of
+// the rows stands the two are even at about 32 MB.
+constexpr int64_t kAhead = 32 << 20;
 How how_of(const VerifyCall& call) {
-    const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, kTarget / call.batch.requests)});
+    const int each = std::max(1, kTarget / call.batch.requests), target = call.vocab / each > kLong ? 2 * kTarget : kTarget;
+    const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, target / call.batch.requests)});
     How how{most, 0, false, 200000};
     how.size = ((call.vocab + most - 1) / most + kWaves - 1) / kWaves * kWaves;
     how.segments = (call.vocab + how.size - 1) / how.size;
@@ -683,12 +721,23 @@ void launch_verify(const VerifyCall& call, hipStream_t stream) {
     const int grid = call.batch.requests * how.segments;
     if (how.ahead) {
         verify_rows_kernel<<<grid * call.batch.max_rows, kThreads, 0, stream>>>(call, how);
-        verify_kernel<true><<<grid, kThreads, 0, stream>>>(call, how);
+        verify_kernel<true, false><<<grid, kThreads, 0, stream>>>(call, how);
         return;
     }
     if (const size_t words = workspace_words(call, how))
         empty_slots_kernel<<<(int)std::min<size_t>((words + 1023) / 1024, 1024), 256, 0, stream>>>((uint64_t*)call.workspace, words);
-    verify_kernel<false><<<grid, kThreads, 0, stream>>>(call, how);
+    if (!call.draft || how.size > kThreads * kHeld) {
+        verify_kernel<false, false><<<grid, kThreads, 0, stream>>>(call, how);
+        return;
+    }
+    constexpr int kLds = 2 * kHeld * kThreads * (int)sizeof(double);
+    static std::atomic<uint64_t> allowed{0};        // more than the default: allowed once a device
+    int device = 0;
+    (void)hipGetDevice(&device);
+    if (!(allowed >> (device & 63) & 1) &&
+        hipFuncSetAttribute(reinterpret_cast<const void*>(verify_kernel<false, true>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
+        allowed |= 1ull << (device & 63);
+    verify_kernel<false, true><<<grid, kThreads, kLds, stream>>>(call, how);
 }
 
 }  // namespace leafhip
