@@ -791,7 +791,7 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
 
 // ---- the same of trees (lh_attention_kv8_tree): of up to 32 rows of a KV head two waves for 16 of them, each with half of
 // a step's keys; codes are loaded two steps ahead
-// 64 requests of 5 to 8 rows over 200 to 4096 keys, 32 heads of 128 over 8 (INT8): 85 us and 10 for the join, 293 MB at
+// 64 requests of 5 to 8 rows over 200 to 4096 keys, 32 heads of 128 over 8 (INT8): 84 us and 10 for the join, 293 MB at
 // 3.2 TB/s; 16 of 45 to 64 rows over 500 to 8000 keys, 32 heads of 64 over 4 (E4M3): 92 and 10.  The kernel of causal rows
 // with masks took 124 and 110 for these: what two steps of loads in flight, half the keys to a wave where two of four
 // would have no rows, and the join without a search gave.  What bounds them: CUs have waves for some three quarters of the

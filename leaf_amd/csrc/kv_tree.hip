@@ -2,7 +2,8 @@
 // lh_kv_tree, lh_kv_keep).
 //
 // What bounds both is a launch: the plan of 24 trees of 8 rows takes 4.0 us and of
-// 250 of 64 rows 4.1, the lengths and blocks of 16 requests 4.2 and of 64 6.3.
+// 250 of 64 rows 4.1, the lengths and blocks of 16 or 64 requests 3.9 (6.3 where a wave
+// copied one request's blocks after the other's).
 #include <algorithm>
 
 #include "kv8.h"
@@ -60,6 +61,7 @@ __global__ __launch_bounds__(kTreeRows) void kv_tree_kernel(KvTreeCall p) {
 // lh_kv_keep: one workgroup sums the blocks that the requests give back.
 constexpr int kKeepThreads = 1024;
 constexpr int kPerThread = 4;                       // LH_KV_MAX_REQUESTS <= 4 * 1024
+constexpr int kFewBlocks = 4;
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepCall p) {
     const KvBatchView& b = p.batch;
     __shared__ int given[kKeepThreads * kPerThread], first[kKeepThreads * kPerThread];   // before each request; its first table entry
@@ -104,10 +106,20 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepCall p) {
     const int returned = min(all, b.blocks - count);
     if (threadIdx.x == 0) *b.free_left = count + returned;
     __syncthreads();
-    // a wave looks at 64 requests and copies the table entries of those that give blocks back
+    // a wave looks at 64 requests: a lane copies its own's table entries where they are few, the wave those of the others
     for (int base = wave * 64; base < n; base += kKeepThreads) {
         const int r = base + lane, blocks = r >= n ? 0 : (r + 1 < kKeepThreads * kPerThread ? given[r + 1] : all) - given[r];
-        for (uint64_t some = __ballot(blocks > 0); some; some &= some - 1) {
+        const bool few = blocks <= kFewBlocks;
+        if (few && blocks > 0) {
+            const int* row = b.table + (size_t)r * b.width + first[r];
+            int ids[kFewBlocks];
+#pragma unroll
+            for (int j = 0; j < kFewBlocks; ++j) ids[j] = row[min(j, blocks - 1)];
+#pragma unroll
+            for (int j = 0; j < kFewBlocks; ++j)
+                if (j < blocks && given[r] + j < returned) b.free_blocks[count + given[r] + j] = ids[j];
+        }
+        for (uint64_t some = __ballot(!few); some; some &= some - 1) {
             const int from = __builtin_ctzll(some), to = given[base + from];
             const int here = min(__shfl(blocks, from, 64), returned - to);
             const int* row = b.table + (size_t)(base + from) * b.width + first[base + from];
