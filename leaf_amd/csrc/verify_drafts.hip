@@ -694,7 +694,7 @@ constexpr int kTarget = 256, kLeast = 2048, kLong = 32768;
 // of them.  Ahead / as the walk comes, over 32000 tokens with both models' logits, chains of 8 rows that all stand: one (2
 // MB) 28 / 59 us, 16 (33 MB) 43 / 61, 64 (131 MB, in an earlier state) 73 / 50 of trees that do not.  Where a third of
 // the rows stands the two are even at about 32 MB.
-constexpr int64_t kAhead = 32 << 20;
+constexpr double kAhead = 32 << 20;
 How how_of(const VerifyCall& call) {
     const int each = std::max(1, kTarget / call.batch.requests), target = call.vocab / each > kLong ? 2 * kTarget : kTarget;
     const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, target / call.batch.requests)});
@@ -702,7 +702,7 @@ How how_of(const VerifyCall& call) {
     how.size = ((call.vocab + most - 1) / most + kWaves - 1) / kWaves * kWaves;
     how.segments = (call.vocab + how.size - 1) / how.size;
     // (not where its workgroups, for max_rows of every request, are mostly for rows that no request has)
-    how.ahead = call.batch.max_rows > 1 && (int64_t)call.batch.tokens * call.vocab * (call.draft ? 8 : 4) <= kAhead &&
+    how.ahead = call.batch.max_rows > 1 && (double)call.batch.tokens * call.vocab * (call.draft ? 8 : 4) <= kAhead &&
                 (int64_t)call.batch.requests * call.batch.max_rows <= 4LL * call.batch.tokens;
     return how;
 }

@@ -203,6 +203,52 @@ def test_attention_spoilt_queries(rt, what):
     assert np.isnan(got).sum() == 64 and (got[22] == 0).all()
 
 
+@pytest.mark.parametrize("form", [ref.INT8, ref.E4M3])
+@pytest.mark.parametrize("batch", ["small", "trees", "wide", "long"])
+def test_attention_scales_far_apart(rt, form, batch):
+    # blocks whose scales differ by factors up to a million; then huge values under scores of ordinary size
+    rng = np.random.default_rng(27)
+    c = tree_case(rng, BATCHES[batch], 4, 2, 64, 16, form)
+    c["value_scales"] = np.exp2(rng.integers(-20, 1, c["value_scales"].shape)).astype(np.float32)
+    c["key_scales"] = np.exp2(rng.integers(-20, -4, c["key_scales"].shape)).astype(np.float32)
+    check_attention(rt, c, 16, form)
+    c = tree_case(rng, BATCHES[batch], 4, 2, 64, 16, form)
+    c["value_scales"] *= np.float32(2.0 ** 100)
+    c["key_scales"] *= np.float32(2.0 ** -70)
+    c["q"] *= np.float32(2.0 ** 70)
+    check_attention(rt, c, 16, form)
+
+
+@pytest.mark.parametrize("batch", ["small", "trees", "wide"])
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 30.0])
+def test_attention_query_sizes(rt, batch, size):
+    # flat, and sharp with scores up to hundreds
+    rng = np.random.default_rng(28)
+    c = tree_case(rng, BATCHES[batch], 4, 2, 64, 32, ref.INT8)
+    c["q"] *= np.float32(size)
+    check_attention(rt, c, 32, ref.INT8)
+
+
+@pytest.mark.parametrize("heads", [2, 16, 40])
+def test_attention_of_scores_far_from_zero(rt, heads):
+    # scores of 2^24 and more: of keys that are the same, whatever row of the step or cached key they are, each weighs alike
+    rng = np.random.default_rng(29)
+    for scale in (2.0 ** 10, -2.0 ** 12):
+        c = tree_case(rng, [(90, 9), (40, 20)], heads, 1, 64, 16, ref.INT8)
+        c["keys"][:] = c["keys"][0, 0, 0]
+        c["key_scales"][:] = np.float32(2.0 ** 8)
+        c["q"][:] = np.float32(scale) * ref.decode(c["keys"][0, 0, 0], ref.INT8).astype(np.float32)
+        got = attend_on_gpu(rt, c, 16, ref.INT8)
+        # equal scores: the mean of the values that a row sees; 90 weights of 2^-22, sums in f32, a value scale of 2^-3 at most
+        values = ref.decode(c["values"], ref.INT8) * c["value_scales"][:, :, None, None]
+        for r in range(2):
+            v = values[c["table"][r, :-(-c["lengths"][r] // 16)], 0].transpose(0, 2, 1).reshape(-1, 64)[:c["lengths"][r]]
+            before = c["lengths"][r] - c["rows"][r]
+            for i in range(c["rows"][r]):
+                want = v[np.concatenate([np.ones(before, bool), c["seen"][r][i]])].mean(0)
+                assert np.abs(got[c["starts"][r] + i] - want).max() <= 2.0 ** -19 * np.abs(v).max()
+
+
 def test_attention_passes_over_requests_that_do_not_fit(rt):
     rng = np.random.default_rng(25)
     c = tree_case(rng, [(30, 2), (40, 2), (50, 2), (60, 2), (70, 2), (80, 2), (90, 2)], 4, 2, 64, 16, ref.INT8, padding=4)
