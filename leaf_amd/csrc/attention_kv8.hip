@@ -824,6 +824,13 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
     const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
     const TreeRow<0> tree(p, q, row / group);
+    // the last cached key that the window hides from any of the wave's rows, which may stand behind the request's last key
+    int hidden = -1;
+    if (p.window) {
+        hidden = tree.position - p.window;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) hidden = max(hidden, __shfl_xor(hidden, o, 64));
+    }
 
     // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
     struct Codes {
@@ -901,7 +908,7 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
                 }
             const int at = step * kStep + 16 * lq;
             bool spare = false;
-            if (step * kStep + kStep > before || (p.window && step * kStep <= q.length - 1 - p.window)) {
+            if (step * kStep + kStep > before || step * kStep <= hidden) {
                 const uint32_t bits = tree.seen(at, p.window ? tree.position + 1 - p.window - at : 0) >> (4 * NJ * kh) & ((1u << 4 * NJ) - 1);
                 // (a key that is not seen weighs nothing whatever its block's scales, if they are numbers)
                 spare = bits == 0;
