@@ -316,23 +316,24 @@ struct TreeRow {
     uint64_t word = 0;
     const uint64_t* mask = nullptr;
     const int* positions = nullptr;                 // of the request's rows; null without a window
-    int rows = 0, before = 0, position = 0, words = 0, window = 0;
+    int rows = 0, before = 0, words = 0;
+    int first = 0, limit = 0;                       // of a window: the cached keys before `first`, positions up to `limit` are hidden
 
     __device__ __forceinline__ TreeRow() {}
     __device__ __forceinline__ TreeRow(const AttentionKv8Call& p, const Kv8Request& q, int row) {
         mask = p.masks + (size_t)(q.start + row) * p.words;
         words = p.words;
         rows = q.rows;
-        before = position = q.length - q.rows;
-        window = p.window;
+        before = q.length - q.rows;
         if (ONE) word = *mask;
-        if (window) {
+        if (p.window) {
             positions = p.batch.positions + q.start;
-            position = min(max(position, positions[row]), 1 << 30);
+            limit = max(before, positions[row]) - p.window;        // (a window is positive, so no position is too far)
+            first = min(max(limit, -1) + 1, before);
         }
     }
-    // A bit for each of the 16 keys from `at` on, of which those before the step's rows count from key at + `from`.
-    __device__ __forceinline__ uint32_t seen(int at, int from) const {
+    // A bit for each of the 16 keys from `at` on.
+    __device__ __forceinline__ uint32_t seen(int at) const {
         const int j = at - before;                  // the first as a row
         uint32_t bits = 0xFFFF;
         if (j > -16) {
@@ -349,12 +350,12 @@ struct TreeRow {
             if (j < 0) w |= (1u << -j) - 1;
             const int left = rows - j;
             bits = (uint32_t)w & (left >= 16 ? 0xFFFFu : left > 0 ? (1u << left) - 1 : 0u);
-            if (window)                             // (of a row its position counts, not its place)
+            if (positions)                          // (of a row its position counts, not its place)
 #pragma unroll 4
                 for (int k = max(-j, 0); k < min(16, left); ++k)
-                    if (positions[j + k] <= position - window) bits &= ~(1u << k);
+                    if (positions[j + k] <= limit) bits &= ~(1u << k);
         }
-        const int hidden = min(from, -j);
+        const int hidden = first - at;
         return hidden <= 0 ? bits : hidden >= 16 ? 0 : bits >> hidden << hidden;
     }
 };
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
     const int token = q.start + row / group, head = kvh * group + row % group;
     const int low = q.length - q.rows;                             // position of the first row
     const TreeRow<1> tree = TREE ? TreeRow<1>(p, q, row / group) : TreeRow<1>();
-    const int position = TREE ? tree.position : low + row / group;
+    const int position = low + row / group;                        // (not of a tree)
     const Steps seen = steps_of<TREE>(q, group, p.window, share.tile_rows, 0);
     const int steps = seen.end - seen.begin, parts = parts_of(steps, per);
     if (item.part >= parts || (parts > 1 && item.slot > share.slots - parts)) return;
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void atten
         const int at = step * kStep + 16 * lq;                     // the lane's first key
         if (step * kStep + kStep > low + !TREE || p.window) {      // the wave's rows see different keys
             const int from = p.window ? position + 1 - p.window - at : 0;
-            if (TREE) weigh(acc, c, now, m, o, KeyBits{tree.seen(at, from)}, hi, lo);
+            if (TREE) weigh(acc, c, now, m, o, KeyBits{tree.seen(at)}, hi, lo);
             else weigh(acc, c, now, m, o, KeyRange{from, position + 1 - at}, hi, lo);
             // (codes that no token wrote, or of no block, may be NaN, which no weight of zero stops)
             const int written = now.known ? q.length - at : 0;
@@ -824,10 +825,10 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
     const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
     const TreeRow<0> tree(p, q, row / group);
-    // the last cached key that the window hides from any of the wave's rows, which may stand behind the request's last key
-    int hidden = -1;
+    // the window hides cached keys before this one from some of the wave's rows, which may stand behind the request's last key
+    int hidden = 0;
     if (p.window) {
-        hidden = tree.position - p.window;
+        hidden = tree.first;
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) hidden = max(hidden, __shfl_xor(hidden, o, 64));
     }
@@ -908,8 +909,8 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
                 }
             const int at = step * kStep + 16 * lq;
             bool spare = false;
-            if (step * kStep + kStep > before || step * kStep <= hidden) {
-                const uint32_t bits = tree.seen(at, p.window ? tree.position + 1 - p.window - at : 0) >> (4 * NJ * kh) & ((1u << 4 * NJ) - 1);
+            if (step * kStep + kStep > before || step * kStep < hidden) {
+                const uint32_t bits = tree.seen(at) >> (4 * NJ * kh) & ((1u << 4 * NJ) - 1);
                 // (a key that is not seen weighs nothing whatever its block's scales, if they are numbers)
                 spare = bits == 0;
 #pragma unroll

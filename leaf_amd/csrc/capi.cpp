@@ -1060,7 +1060,7 @@ lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, c
         a.tree = true;
         a.masks = masks;
         a.words = mask_words(batch);
-        a.window = int(std::min<uint32_t>(window, 1u << 30));      // (a request has no more keys)
+        a.window = window > 0x7fffffffu ? 0 : int(window);         // (no position is so far behind another)
         run_attention_kv8(a, cache, q_heads, out, workspace, workspace_bytes, as_stream(stream));
     });
 }

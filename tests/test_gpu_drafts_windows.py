@@ -39,3 +39,15 @@ def test_rows_behind_the_last_key(rt, batch, window, form, block):  # noqa: F811
     c["positions"][5] += 5000
     got = check_attention(rt, c, block, form, window)
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("window", [10, 2 ** 30, 2 ** 31 - 300, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1])
+@pytest.mark.parametrize("batch", BATCHES)
+def test_positions_at_the_end_of_their_type(rt, batch, window):  # noqa: F811
+    # a row's own place and its window are exact as far as int32 positions and uint32 windows reach
+    rng = np.random.default_rng(61)
+    c = tree_case(rng, BATCHES[batch], 4, 2, 64, 32, ref.INT8, reach=20)
+    c["positions"] = 2 ** 31 - 1 - rng.integers(0, 60, len(c["positions"]))
+    check_attention(rt, c, 32, ref.INT8, window)
+    c["positions"][::3] = 2 ** 30 + rng.integers(-30, 30, len(c["positions"][::3]))
+    check_attention(rt, c, 32, ref.INT8, window)
