@@ -543,8 +543,17 @@ struct Walk {
         // of the wave's share some values in order to a thread
         const int from = share_begin(own, share), end = share_begin(own, share + 1), each = (end - from + kThreads - 1) / kThreads;
         const int mine = min(from + (int)threadIdx.x * each, end), mine_end = min(mine + each, end);
+        // What is left of a value has to be what measure_left has summed, bit for bit: after many refusals all that is left may
+        // be of the size of a weight's rounding, and a share whose sum is not zero must have a value that is not.
+        const bool kept = HELD && scale > 0.0;
+        const double fw = kept ? weight(s.tops[0][share], most_w) : 0.0, fv = kept ? scale * weight(s.tops[1][share], most_v) : 0.0;
+        auto rest_of = [&](int x) {
+            if (!kept) return left_of(x);
+            const int at = ((x - from) >> 6) * kThreads + 64 * share + ((x - from) & 63);   // of the share's wave: as it was stored
+            return fmax(weights[at] * fw - weights[kHeld * kThreads + at] * fv, 0.0);
+        };
         double sum = 0.0;
-        for (int x = mine; x < mine_end; ++x) sum += left_of(x);
+        for (int x = mine; x < mine_end; ++x) sum += rest_of(x);
         double upto = sum;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -558,7 +567,7 @@ struct Walk {
         for (int i = 0; i < wave; ++i) at += s.sums[1][i];
         int passes = p.vocab, last_left = -1;
         for (int x = mine; x < mine_end; ++x) {
-            const double r = left_of(x);
+            const double r = rest_of(x);
             at += r;
             if (!(r > 0.0)) continue;
             last_left = x;
