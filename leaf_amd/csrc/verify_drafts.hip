@@ -704,10 +704,20 @@ constexpr int kTarget = 256, kLeast = 2048, kLong = 32768;
 // MB) 28 / 59 us, 16 (33 MB) 43 / 61, 64 (131 MB, in an earlier state) 73 / 50 of trees that do not.  Where a third of
 // the rows stands the two are even at about 32 MB.
 constexpr double kAhead = 32 << 20;
+
+// How.wait: LEAF_VERIFY_WAIT as it is when the library is loaded (later launches of any thread do not look at the
+// environment).  Never longer than the default: whoever is waited for may not be able to start before the waiting ones end.
+constexpr long long kLongestWait = 200000;
+const long long kWait = [] {
+    const char* given = std::getenv("LEAF_VERIFY_WAIT");
+    char* end = nullptr;
+    const long long cycles = given ? std::strtoll(given, &end, 10) : kLongestWait;
+    return given && end == given ? kLongestWait : std::clamp(cycles, 0LL, kLongestWait);
+}();
 How how_of(const VerifyCall& call) {
     const int each = std::max(1, kTarget / call.batch.requests), target = call.vocab / each > kLong ? 2 * kTarget : kTarget;
     const int most = std::min({(call.vocab + kLeast - 1) / kLeast, kMostSegments, std::max(1, target / call.batch.requests)});
-    How how{most, 0, false, 200000};
+    How how{most, 0, false, kWait};
     how.size = ((call.vocab + most - 1) / most + kWaves - 1) / kWaves * kWaves;
     how.segments = (call.vocab + how.size - 1) / how.size;
     // (not where its workgroups, for max_rows of every request, are mostly for rows that no request has)
@@ -725,8 +735,7 @@ size_t workspace_words(const VerifyCall& call, const How& how) {
 size_t verify_workspace_bytes(const VerifyCall& call) { return 8 * workspace_words(call, how_of(call)); }
 
 void launch_verify(const VerifyCall& call, hipStream_t stream) {
-    How how = how_of(call);
-    if (const char* cycles = std::getenv("LEAF_VERIFY_WAIT")) how.wait = std::atoll(cycles);
+    const How how = how_of(call);
     const int grid = call.batch.requests * how.segments;
     if (how.ahead) {
         verify_rows_kernel<<<grid * call.batch.max_rows, kThreads, 0, stream>>>(call, how);
