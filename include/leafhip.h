@@ -488,11 +488,14 @@ typedef struct lh_drafts {
  *   sampling  with p = softmax(logits / T) and q = softmax(draft_logits / T) of the parent,
  *             C = 0 and r = p at first, and S the sum of r: a child with token x and
  *             random number u is taken if u S q(x) < r(x).  If not, C becomes C + S and r
- *             max(p - C q, 0), which keeps the tokens that stand distributed as p says.  Without
+ *             max(p - C q, 0).  That keeps the tokens that stand distributed as p says where a row's children
+ *             were drawn from q independently of each other, so that two may be the same token (not
+ *             where they were chosen to differ, as drawn without replacement).  Without
  *             draft_logits (tokens that were not drawn, as the draft's best) x is taken if u S < r(x); if
- *             not, r(x) becomes 0.  The token behind is the first whose sum of r in the tokens' order
+ *             not, r(x) becomes 0, which keeps it whatever the tokens.  The token behind is the first whose sum of r in the tokens' order
  *             passes sample times S (where nothing is left, S = 0, the same of p).
- * All in 64 bits: a random number within 1e-12 of a border may fall to either side.
+ * All in 64 bits: behind n refused children of a row, a random number within (n + 1) 1e-12 / S of a border
+ * may fall to either side (S is 1 before a refusal).
  * A token outside the vocabulary is not taken.  Where a test or the token behind needs logits of
  * which one is NaN or plus infinity or all are minus infinity, or a T that is negative or
  * not finite, the walk ends, with next -1.  A request without rows has kept 0 and next -1.
@@ -505,7 +508,7 @@ lh_status lh_verify_drafts(const lh_kv_batch* batch, const lh_drafts* drafts, vo
 lh_status lh_verify_drafts_workspace(const lh_kv_batch* batch, const lh_drafts* drafts, size_t* bytes);
 
 /* The rows that stand, moved together in `layers` caches (caches is a host array; all of the same
- * heads, dim and format): of each request row path[starts[r] + k] goes to the place of row k, for k
+ * heads, dim and format, no two with an array in common): of each request row path[starts[r] + k] goes to the place of row k, for k
  * < kept[r].  A block that takes in a moved row gets, for keys and for values of each KV head, the largest scale of the blocks that
  * its tokens (cached ones, and rows that stand) come from, and their codes become code * old
  * scale / scale as in lh_rope_kv8; other blocks, and the places behind the rows that stand, stay

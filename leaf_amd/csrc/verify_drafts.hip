@@ -11,7 +11,9 @@
 //
 // All sums and weights are 64-bit: the last token is the one at whose weight the
 // sums in order pass u times all, and among 10^5 tokens an f32 sum would often be
-// on the other side of it.
+// on the other side of it.  p and q are good to some 1.5e-13 of themselves (`power`), so
+// what is left of a token after n refusals is good to some (n + 1) 1e-12 of the whole,
+// not of what is left.
 //
 // A walk's rows come one after the other, and only those on its way are read
 // (unless all are few: then a launch measures them beforehand, see kAhead).
