@@ -316,7 +316,7 @@ struct TreeRow {
     uint64_t word = 0;
     const uint64_t* mask = nullptr;
     const int* positions = nullptr;                 // of the request's rows; null without a window
-    int rows = 0, before = 0, words = 0;
+    int rows = 0, before = 0, words = 0, window = 0;
     int first = 0, limit = 0;                       // of a window: the cached keys before `first`, positions up to `limit` are hidden
 
     __device__ __forceinline__ TreeRow() {}
@@ -325,10 +325,11 @@ struct TreeRow {
         words = p.words;
         rows = q.rows;
         before = q.length - q.rows;
+        window = p.window;
         if (ONE) word = *mask;
-        if (p.window) {
+        if (window) {
             positions = p.batch.positions + q.start;
-            limit = max(before, positions[row]) - p.window;        // (a window is positive, so no position is too far)
+            limit = max(before, positions[row]) - window;          // (a window is positive, so no position is too far)
             first = min(max(limit, -1) + 1, before);
         }
     }
@@ -350,7 +351,7 @@ struct TreeRow {
             if (j < 0) w |= (1u << -j) - 1;
             const int left = rows - j;
             bits = (uint32_t)w & (left >= 16 ? 0xFFFFu : left > 0 ? (1u << left) - 1 : 0u);
-            if (positions)                          // (of a row its position counts, not its place)
+            if (window)                             // (of a row its position counts, not its place)
 #pragma unroll 4
                 for (int k = max(-j, 0); k < min(16, left); ++k)
                     if (positions[j + k] <= limit) bits &= ~(1u << k);
@@ -825,13 +826,6 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
     const Keys keys(p, item.request, kvh, q.length, dim, li, lq);
     const int row = min(w0 + li, rows - 1), token = q.start + row / group, head = kvh * group + row % group;
     const TreeRow<0> tree(p, q, row / group);
-    // the window hides cached keys before this one from some of the wave's rows, which may stand behind the request's last key
-    int hidden = 0;
-    if (p.window) {
-        hidden = tree.first;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) hidden = max(hidden, __shfl_xor(hidden, o, 64));
-    }
 
     // staging: wave w widens tile w of the keys and the tiles w, w + 4.. of the dims
     struct Codes {
@@ -881,6 +875,15 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_tree_
     load(codes[0], begin + 2, keys.key_block(begin + 2), keys.value_block(begin + 2));
     KeyScales scales = keys.scales(keys.value_block(begin));
     int ik = keys.key_block(begin + 3), iv = keys.value_block(begin + 3), is = keys.value_block(begin + 1);
+    // the window hides cached keys before this one from some of the wave's rows, which may stand behind the request's last key
+    // (after the first loads: it waits for the rows' positions)
+    int hidden = 0;
+    if (p.window) {
+        hidden = tree.first;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) hidden = max(hidden, __shfl_xor(hidden, o, 64));
+        hidden = __builtin_amdgcn_readfirstlane(hidden);
+    }
     lds_barrier();
     // A step: `later` holds the codes of the next one.
     auto turn = [&](int step, Codes& later) {
