@@ -455,8 +455,8 @@ lh_status lh_kv_tree(const lh_kv_batch* batch, const int32_t* parents, uint64_t*
 /* lh_attention_kv8 of trees: a row sees the keys of its request before the step's rows,
  * length - rows of them, and of these rows those whose bit is set in its mask, whatever their order (the
  * masks may be others than lh_kv_tree's; bits of rows that the request does not have count for nothing).  With a window, keys at
- * positions up to the row's own less window are hidden, where a step's row stands at positions[t] (at
- * least length - rows; read only then).  A row that sees no key gets zeros.  Otherwise as
+ * positions up to the row's own less window are hidden, where a step's row stands at positions[t] (from
+ * length - rows to the end of its type; read only then).  A row that sees no key gets zeros.  Otherwise as
  * lh_attention_kv8: the same batch arrays, NaN rules and accuracy, and the same rules for a workspace, of
  * lh_attention_kv8_tree_workspace bytes. */
 lh_status lh_attention_kv8_tree(const lh_kv_batch* batch, const lh_kv8* cache, const float* q_heads, uint32_t heads,

@@ -487,6 +487,7 @@ __device__ __forceinline__ v2f* partial_sums(const AttentionKv8Call& p, const Sh
 // dependent loads (its place, the query, the first table entries, the first codes); how
 // much of the rest is these starts and how much parts that end unevenly is not shown.
 // 8 requests of 16000 tokens take 57 us, 4.6 TB/s.
+// Of trees (the join attention_kv8_tree_merge_kernel): 64 chains of 3 to 4 rows, 200 to 4096 keys, 77 us (a trace: 71 and 6).
 template <int CC, bool FULL, bool E4M3, bool TREE>
 __global__ __launch_bounds__(kThreads, CC == 1 ? 3 : CC == 2 ? 2 : 1) void attention_kv8_few_kernel(AttentionKv8Call p, Share share) {
     constexpr int TILES = 4 * CC;
@@ -793,10 +794,14 @@ __global__ __launch_bounds__(kThreads, CC <= 2 ? 2 : 1) void attention_kv8_rows_
 
 // ---- the same of trees (lh_attention_kv8_tree): of up to 32 rows of a KV head two waves for 16 of them, each with half of
 // a step's keys; codes are loaded two steps ahead
-// 64 requests of 5 to 8 rows over 200 to 4096 keys, 32 heads of 128 over 8 (INT8): 84 us and 10 for the join, 293 MB at
-// 3.2 TB/s; 16 of 45 to 64 rows over 500 to 8000 keys, 32 heads of 64 over 4 (E4M3): 92 and 10.  The kernel of causal rows
-// with masks took 124 and 110 for these: what two steps of loads in flight, half the keys to a wave where two of four
-// would have no rows, and the join without a search gave.  What bounds them: CUs have waves for some three quarters of the
+// 64 requests of 5 to 8 rows over 200 to 4096 keys, 32 heads of 128 over 8 (INT8): 93 us with the join's launch, 293 MB of
+// codes, q and out at 3.2 TB/s, of which 156 come from memory and the rest from the last-level cache; 16 of 45 to 64 rows
+// over 500 to 8000 keys, 32 heads of 64 over 4 (E4M3): 103.  (A trace gives 88 and 10 for the two launches of the one, 108 and 10
+// for the other's, slower than a loop without it.)  The kernel of causal rows with masks took 124 and 110 for both launches: what two steps of
+// loads in flight, half the keys to a wave where two of four would have no rows, and the join without a search gave.
+// A step with a prompt is far from these: 384 rows behind 2000 keys, 24 single tokens and 16 trees of 8 rows over 200 to 4096, heads
+// of 128, take 172 us for the causal call's 124 (heads of 64 87 for 60).  Each single token has a tile of 64 rows, a prompt's
+// tiles see every key, and the join has workgroups for the prompt's rows of every request (72 us of a trace).  What bounds them: CUs have waves for some three quarters of the
 // kernel's time (parts are a half to the whole of the longest, and start behind four dependent loads); in it vector
 // instructions take 41% and 48% of the cycles, MFMAs 17% and 22%.  Measured and left: the codes of a step in registers
 // for two or four row tiles of one wave, without LDS or barriers (103 and 107 us, with spills), and the split of keys into
@@ -1185,6 +1190,10 @@ constexpr int kFewLeast = 4, kRowsLeast = 8;
 // The same of trees of more than 16 rows, with 512 / 768 / 1024 workgroups: 64 of 20 to 32 rows, heads of 128, 101 / 93 / 101
 // us, 16 of 360 to 512, heads of 64, 110 / 103 / 102; with 4 / 6 / 8 steps 40 of 27 to 39 rows 30 / 23 / 25 us, one of 182 18 / 18 / 20.
 constexpr int kTreeTarget = 768, kTreeLeast = 6;
+// Trees of at most 16 rows of a KV head take the kernel of few rows.  It / the kernel of trees, chains, us: 64 of 3 to 4
+// rows, 32 heads of 128 over 8, 200 to 4096 keys 77 / 83; 64 of 2, 32 heads of 64 over 4 (E4M3) 24.5 / 30; 8 of 4, 16000 keys 59 / 74;
+// one of 4, 4095 keys 17 / 20; 400 of 3 to 4, 20 to 200 keys 76 / 86; but 100 of 4 to 5, 30 to 600 keys in a window of 300,
+// 15 heads of 64 over 5, 18.3 / 17.6.
 // Rows of the step for each request from which the kernel of many rows takes every request: one launch in place of
 // two, one after the other, although it has a request of one token in a tile of 64.  At 13 a request it takes 75 us for 73
 // (heads of 128) and at 8 30 for 40 (heads of 64), at 3.5 203 for 151 and 39 for 45; between 3.5 and 8 nothing was

@@ -702,9 +702,12 @@ __global__ void empty_slots_kernel(uint64_t* slots, size_t count) {
 // us, 100 chains of 4 over 49152 greedy 28.5 / 28.8, 100 chains of 4 over 151936 136 / 104.
 constexpr int kTarget = 256, kLeast = 2048, kLong = 32768;
 // Bytes of logits up to which every row is measured ahead of the walk, side by side, although it may not come to all
-// of them.  Ahead / as the walk comes, over 32000 tokens with both models' logits, chains of 8 rows that all stand: one (2
-// MB) 28 / 59 us, 16 (33 MB) 43 / 61, 64 (131 MB, in an earlier state) 73 / 50 of trees that do not.  Where a third of
-// the rows stands the two are even at about 32 MB.
+// of them.  Ahead / as the walk comes, us.  Both models' logits, 32000 tokens: a chain of 8 rows that all stand (2 MB) 28 / 59,
+// 16 (33 MB) 43 / 61 and 43 / 60 where half stand, 64 (131 MB, which stay in the last-level cache) 66 / 75, 71 / 74; but 64 trees of 8 rows in
+// three states in turn (3 times 113 MB) 75 / 41.  One model's: 40 chains of 4 over 49152 (31 MB) sampled 30 / 34, greedy
+// 17.5 / 21.6; 100 (79 MB) 49 / 58 and 26 / 29; 100 greedy over 151936 (243 MB) 53 / 50, 52.5 / 46 where they end early; 16 trees of 26 rows over
+// 151936 sampled (214 MB) 107 / 41.  So wide trees decide: ahead reads rows that no walk comes to.  Between 33 and 113 MB trees were not
+// measured, and chains, above all greedy ones, would gain some us up to about 100.
 constexpr double kAhead = 32 << 20;
 
 // How.wait: LEAF_VERIFY_WAIT as it is when the library is loaded (later launches of any thread do not look at the
